@@ -660,6 +660,126 @@ int32_t pkv_spec_accept(const float* target_logits, const float* draft_logits, i
                         int32_t* n_accepted, int32_t* tickets, void* workspace, int64_t workspace_bytes,
                         void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Losses over vocabulary rows, with gradients, and a row's top logits.  No
+ * kernel counterpart in the reference (its trainer's clipped objective,
+ * agentrl/core/trainer.py:72-167, is torch operations over a [B, L, vocab]
+ * log_softmax).
+ *
+ * Rows are [batch][length] positions of `vocab` logits (fp32, f16 or bf16),
+ * element strides batch_stride / row_stride, columns contiguous.  A row whose
+ * mask byte is 0 is not scored: it is never read, its outputs are 0 and its
+ * gradient row is zeros.  With `grad` non-NULL the loss call writes the
+ * gradient of `loss` too (the logits' dtype, rows that do not overlap), each
+ * logits row crossing HBM once; without it the call leaves what a later
+ * *_backward call needs in the workspace (keep it, and the logits, until
+ * then), which multiplies by the device scalar *upstream.  Gradients of rows
+ * and the loss are the same bits from call to call.  A scored row whose token
+ * lies outside [0, vocab) makes its log-probability, its gradient row and the
+ * loss NaN.  The workspace is device scratch of
+ * pkv_loss_workspace_bytes(batch, length) bytes, 256-byte aligned, no initial
+ * contents needed; calls sharing one run in stream order.
+ * ------------------------------------------------------------------------- */
+
+enum pkv_reduction {
+  PKV_TOKEN_MEAN = 0,    /* mean over all scored rows */
+  PKV_SEQUENCE_MEAN = 1, /* mean over the sequences with a scored row of the mean over their rows */
+  PKV_SUM = 2
+};
+
+/* Most entries of a row's top list. */
+#define PKV_MAX_TOP 256
+
+typedef struct pkv_loss_rows {
+  const void* logits;
+  int64_t batch_stride, row_stride;
+  void* grad;                 /* or NULL */
+  int64_t grad_batch_stride, grad_row_stride;
+  const uint8_t* mask;        /* [batch][length] with element strides, or NULL: every row is scored */
+  int64_t mask_batch_stride, mask_row_stride;
+  int32_t batch, length, vocab;
+  int32_t dtype;              /* enum pkv_dtype */
+  float temperature;          /* rows are logits / temperature */
+} pkv_loss_rows;
+
+/* One value a row: [batch][length] with element strides (0 broadcasts); data NULL: absent. */
+typedef struct pkv_token_array {
+  const void* data;
+  int64_t batch_stride, row_stride;
+} pkv_token_array;
+
+/* Per scored row, with logp the log-probability of its token:
+ *   r = exp(logp - old)  (old absent: r = 1, with gradient)
+ *   l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *       + kl_coef (exp(ref - logp) - (ref - logp) - 1)     (ref absent: 0)
+ *       - entropy_coef H(softmax(logits / temperature))
+ * loss = scale x the reduction of l. */
+typedef struct pkv_policy_terms {
+  pkv_token_array tokens;        /* int64 */
+  pkv_token_array advantages;    /* float */
+  pkv_token_array old_logprobs;  /* float, or absent */
+  pkv_token_array ref_logprobs;  /* float, or absent */
+  float clip_low, clip_high, kl_coef, entropy_coef;
+  int32_t reduction;             /* enum pkv_reduction */
+  float scale;
+} pkv_policy_terms;
+
+/* Sequences 0 .. batch/2 - 1 are the chosen answers, the others the rejected
+ * ones of the same prompts.  S = sum (or mean, length_normalised) of a
+ * sequence's scored log-probabilities, R = ref_logprobs (NULL: 0),
+ *   m = beta ((S_c - R_c) - (S_r - R_r)),
+ *   loss = scale mean_pairs(-(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m)). */
+typedef struct pkv_preference_terms {
+  pkv_token_array tokens;        /* int64 */
+  const float* ref_logprobs;     /* [batch], or NULL */
+  float beta, label_smoothing;
+  int32_t length_normalised;
+  float scale;
+} pkv_preference_terms;
+
+/* Per scored row, over its k teacher entries (an id < 0 or a logit of -inf is
+ * an absent one): log q = t / T - N, N the log-sum-exp of the list's t / T or
+ * teacher_lse (the teacher's own, of its whole row at temperature T), and
+ *   l = T^2 sum q (log q - log p[id]);   loss = scale x the reduction of l.
+ * An id may come more than once. */
+typedef struct pkv_distillation_terms {
+  const int64_t* ids;            /* [batch][length][k], the last dimension contiguous */
+  int64_t ids_batch_stride, ids_row_stride;
+  const float* teacher_logits;   /* [batch][length][k] */
+  int64_t logits_batch_stride, logits_row_stride;
+  int32_t k;                     /* 1 .. PKV_MAX_TOP */
+  pkv_token_array teacher_lse;   /* float, or absent */
+  int32_t reduction;
+  float scale;
+} pkv_distillation_terms;
+
+int64_t pkv_loss_workspace_bytes(int32_t batch, int32_t length);
+
+/* The clipped policy loss.  loss: one float; logprobs, kl, entropy: float
+ * [batch][length] contiguous (kl and entropy may be NULL). */
+int32_t pkv_policy_loss(const pkv_loss_rows* rows, const pkv_policy_terms* terms, float* loss, float* logprobs,
+                        float* kl, float* entropy, void* workspace, int64_t workspace_bytes, void* stream);
+int32_t pkv_policy_loss_backward(const pkv_loss_rows* rows, const pkv_policy_terms* terms, const float* upstream,
+                                 void* workspace, int64_t workspace_bytes, void* stream);
+/* The preference loss.  logprobs: float [batch] (S); margins: float [batch / 2] (m). */
+int32_t pkv_preference_loss(const pkv_loss_rows* rows, const pkv_preference_terms* terms, float* loss, float* logprobs,
+                            float* margins, void* workspace, int64_t workspace_bytes, void* stream);
+int32_t pkv_preference_loss_backward(const pkv_loss_rows* rows, const pkv_preference_terms* terms,
+                                     const float* upstream, void* workspace, int64_t workspace_bytes, void* stream);
+/* The distillation loss.  kl: float [batch][length] (l). */
+int32_t pkv_distillation_loss(const pkv_loss_rows* rows, const pkv_distillation_terms* terms, float* loss, float* kl,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+int32_t pkv_distillation_loss_backward(const pkv_loss_rows* rows, const pkv_distillation_terms* terms,
+                                       const float* upstream, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The k largest logits of each row, largest first, equal ones by their column
+ * (NaN counts as the largest, -0 as 0): values float and columns int64
+ * [batch][length][k], lse_out float [batch][length] the log-sum-exp of logits
+ * / temperature.  1 <= k <= min(vocab, PKV_MAX_TOP); the mask and grad of
+ * `rows` are not used. */
+int32_t pkv_top_logits(const pkv_loss_rows* rows, int32_t k, float* values_out, int64_t* tokens_out, float* lse_out,
+                       void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

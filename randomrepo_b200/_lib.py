@@ -225,6 +225,17 @@ _SIGNATURES: dict[str, tuple] = {
          c_int64, c_uint64, c_uint64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
          c_void_p],
     ),
+    # pkv_loss_rows and the terms of a loss go in packed (randomrepo_b200/losses.py), by address.
+    "pkv_loss_workspace_bytes": (c_int64, [c_int32, c_int32]),
+    "pkv_policy_loss": (
+        c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]
+    ),
+    "pkv_policy_loss_backward": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "pkv_preference_loss": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "pkv_preference_loss_backward": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "pkv_distillation_loss": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "pkv_distillation_loss_backward": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "pkv_top_logits": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
 }
 
 # Entry points added after the first build; bound when present.

@@ -1,0 +1,153 @@
+// Parts shared by the vocabulary-row kernels with f32 / f16 / bf16 logits
+// (losses.cu, top_logits.cu): conversions, a row's aligned body, the running
+// log-sum-exp of a row.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "pkv_b200.h"
+
+namespace pkv {
+
+// PKV_OK, or the status and error message for rows a call named `who` cannot take.
+int32_t check_vocab_rows(const pkv_loss_rows* r, const char* who);
+
+constexpr double kLn2d = 0.6931471805599453;
+constexpr double kLog2ed = 1.4426950408889634;
+
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// k = log2(e) / T to about 48 bits.  The second float matters to a sum over
+// many columns: its relative error would shift every log-probability the same way.
+struct Scale2 {
+  float hi, lo;
+};
+
+__device__ __forceinline__ float ex2(float y) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
+  return e;
+}
+
+// The running sums of a set of columns x: m = max x, s = sum 2^y and w = sum 2^y y, y = (x - m) k.  (The maximum is
+// subtracted before the scaling: a type's lowest finite value times k would be -inf.)
+struct RowSum {
+  float m, s, w;
+};
+
+__device__ __forceinline__ void sum_rescale(RowSum& a, float m_new, Scale2 k) {
+  const float d = (a.m - m_new) * k.hi, f = ex2(d);
+  a.w = f > 0.f ? f * fmaf(d, a.s, a.w) : 0.f;  // (a NaN stays in s)
+  a.s *= f;
+  a.m = m_new;
+}
+
+__device__ __forceinline__ void sum_merge(RowSum& a, RowSum b, Scale2 k) {
+  const float mn = fmaxf(a.m, b.m);
+  if (mn == -INFINITY) {
+    a.s += b.s;  // 0, or the NaN of a NaN column
+    return;
+  }
+  // (the larger one's factor is 2^0: exact)
+  sum_rescale(a, mn, k);
+  sum_rescale(b, mn, k);
+  a.s += b.s;
+  a.w += b.w;
+}
+
+// log2 of a positive float to about 1e-7 absolute: the exponent apart, so that a large sum costs no digits.
+__device__ __forceinline__ double log2_of(float s) {
+  int e;
+  const float f = frexpf(s, &e);
+  return (double)e + (double)log2f(f);
+}
+
+// Columns [0, head) and [head + VE nvec, vocab) of a row are outside its 16-byte-aligned body.
+template <typename T>
+struct RowSplit {
+  static constexpr int VE = 16 / sizeof(T);
+  int head, nvec;
+  __device__ RowSplit(const T* row, int vocab) {
+    head = min(vocab, (int)(((16 - ((uintptr_t)row & 15)) & 15) / sizeof(T)));
+    nvec = (vocab - head) / VE;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack(uint4 v, float (&f)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = __uint_as_float(v.x);
+    f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z);
+    f[3] = __uint_as_float(v.w);
+  } else {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        f[2 * i] = __uint_as_float(u[i] << 16);
+        f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      } else {
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float (&f)[16 / sizeof(T)]) {
+  uint4 v;
+  if constexpr (sizeof(T) == 4) {
+    v = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  } else {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        u[i] = *reinterpret_cast<const uint32_t*>(&p);
+      } else {
+        const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        u[i] = *reinterpret_cast<const uint32_t*>(&p);
+      }
+    }
+    v = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  return v;
+}
+
+template <bool ENT, int N>
+__device__ __forceinline__ void fold(RowSum& a, const float (&x)[N], Scale2 k) {
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+  if (!(top > -INFINITY)) {  // nothing but -inf, or NaN
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (x[i] != x[i]) a.s = NAN;
+    return;
+  }
+  if (top > a.m) sum_rescale(a, top, k);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = x[i] - a.m, y = fmaf(d, k.lo, d * k.hi);
+    const float e = ex2(y);
+    a.s += e;
+    if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
+  }
+}
+
+}  // namespace pkv

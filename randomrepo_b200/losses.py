@@ -1,0 +1,409 @@
+"""Losses over vocabulary rows, with their gradients, and a row's top logits (``libpkv_b200``).
+
+What follows a rollout is training on it.  AgentRL's trainer does that with torch operations over a
+[B, L, vocab] log_softmax (agentrl/core/trainer.py:72-167); here a row of logits is read once for its
+statistics and, where a gradient is asked for, once more out of shared memory or L2 to write it:
+
+* ``policy_loss`` -- the clipped policy loss of PPO / GRPO, with a KL term to a reference policy and an
+  entropy bonus;
+* ``preference_loss`` -- the paired log-ratio loss of chosen against rejected answers;
+* ``distillation_loss`` -- a student's divergence from a teacher's top logits, as it keeps a speculative
+  draft model close to the policy it drafts for; ``top_logits`` picks those logits from the teacher's rows.
+
+Each loss comes in two forms.  ``*_loss(logits, ...)`` is differentiable in ``logits``: its backward pass
+reads the logits a second time.  ``*_loss_and_grad(logits, ...)`` returns the loss and its gradient from one
+call, reading the logits from HBM once (policy and distillation): ``logits.backward(dlogits)`` continues
+from there.  ``scale`` multiplies the loss and the gradient before its rounding to the logits' type (a
+gradient accumulation factor, or a loss scale for float16).
+
+``logits`` are ``[B, T, V]`` or ``[T, V]`` CUDA tensors of float32, float16 or bfloat16 with contiguous
+columns (any batch and row strides, so that ``logits[:, :-1]`` needs no copy); per-row inputs are ``[B, T]``
+(``[T]``).  A row whose mask is 0 is not scored: its logits are not read, its outputs and its gradient are
+0; tokens there may be anything.  No scored row at all gives a loss of 0.  Losses and per-row outputs are
+float32; sums over rows are taken in 64 bits, in a fixed order.  Calls launch on the current stream of the
+logits' device, never synchronise, and can be captured in a CUDA graph.  There is no CPU path.
+"""
+
+from __future__ import annotations
+
+import struct
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import lib
+
+__all__ = ["PolicyLoss", "PreferenceLoss", "DistillationLoss", "policy_loss", "policy_loss_and_grad",
+           "preference_loss", "preference_loss_and_grad", "distillation_loss", "distillation_loss_and_grad",
+           "top_logits"]
+
+_DTYPES = {torch.float32: _lib.PKV_F32, torch.float16: _lib.PKV_F16, torch.bfloat16: _lib.PKV_BF16}
+_REDUCTIONS = {"token_mean": 0, "sequence_mean": 1, "sum": 2}
+_MAX_TOP = 256
+
+# The structs of the C ABI (pkv_loss_rows and the terms of each loss), packed with native alignment.
+_ROWS = struct.Struct("@PqqPqqPqqiiiif")
+_POLICY = struct.Struct("@PqqPqqPqqPqqffffif")
+_PREFERENCE = struct.Struct("@PqqPffif")
+_DISTILLATION = struct.Struct("@PqqPqqiPqqif")
+
+
+class PolicyLoss(NamedTuple):
+    """loss (scalar), and per row: the token's log-probability, the KL estimate against the reference
+    (None without one) and the entropy (None unless ``entropy_coef`` is set)."""
+
+    loss: torch.Tensor
+    logprobs: torch.Tensor
+    kl: torch.Tensor | None
+    entropy: torch.Tensor | None
+
+
+class PreferenceLoss(NamedTuple):
+    """loss (scalar), the sequences' summed (or mean) log-probabilities [B], the pairs' margins [B / 2]."""
+
+    loss: torch.Tensor
+    logprobs: torch.Tensor
+    margins: torch.Tensor
+
+
+class DistillationLoss(NamedTuple):
+    """loss (scalar) and each row's T^2-scaled divergence."""
+
+    loss: torch.Tensor
+    kl: torch.Tensor
+
+
+def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
+    """``logits`` as [B, T, V], checked."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise ValueError(f"{what}: logits must be a CUDA tensor (the vocabulary kernels have no CPU path)")
+    if logits.dtype not in _DTYPES:
+        raise ValueError(f"{what}: logits must be float32, float16 or bfloat16")
+    if logits.dim() not in (2, 3) or logits.shape[-1] < 1:
+        raise ValueError(f"{what}: logits must be [batch, length, vocab] or [length, vocab]")
+    if logits.shape[-1] > 1 and logits.stride(-1) != 1:
+        raise ValueError(f"{what}: logits must have a contiguous vocabulary dim")
+    return logits.unsqueeze(0) if logits.dim() == 2 else logits
+
+
+def _rows_like(t: torch.Tensor, x: torch.Tensor, dtype: torch.dtype, what: str, name: str,
+               broadcast: bool = False) -> torch.Tensor:
+    """A per-row input as [B, T] of ``dtype`` on the logits' device (``broadcast``: [B] or [B, 1] too)."""
+    b, n = x.shape[0], x.shape[1]
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what}: {name} must be a tensor")
+    if t.device != x.device:
+        raise ValueError(f"{what}: {name} must be on the logits' device")
+    if broadcast and t.dim() == 1 and t.shape[0] == b and not (b == 1 and n != 1 and t.shape[0] == n):
+        t = t.unsqueeze(1)
+    if t.dim() == 1 and b == 1 and t.shape[0] == n:
+        t = t.unsqueeze(0)
+    if tuple(t.shape) != (b, n):
+        if not (broadcast and tuple(t.shape) == (b, 1)):
+            raise ValueError(f"{what}: {name} must have one value per logits row, got {tuple(t.shape)}")
+        t = t.expand(b, n)
+    if t.dtype != dtype:
+        if dtype == torch.int64 and (t.is_floating_point() or t.dtype == torch.bool):
+            raise ValueError(f"{what}: {name} must be integers")
+        t = t.to(dtype)
+    return t
+
+
+def _mask(mask: torch.Tensor | None, x: torch.Tensor, what: str) -> torch.Tensor | None:
+    """The mask as bytes [B, T] (anything but 0 is scored)."""
+    if mask is None:
+        return None
+    if isinstance(mask, torch.Tensor) and mask.dtype not in (torch.bool, torch.uint8):
+        mask = mask != 0
+    m = _rows_like(mask, x, mask.dtype if isinstance(mask, torch.Tensor) else torch.bool, what, "mask")
+    return m.view(torch.uint8) if m.dtype == torch.bool else m
+
+
+def _array(t: torch.Tensor | None) -> tuple[int, int, int]:
+    return (0, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _reduction(name: str, what: str) -> int:
+    if name not in _REDUCTIONS:
+        raise ValueError(f"{what}: reduction must be one of {sorted(_REDUCTIONS)}, got {name!r}")
+    return _REDUCTIONS[name]
+
+
+def _grad_like(x: torch.Tensor) -> torch.Tensor:
+    """An uninitialised gradient for logits [B, T, V] whose rows start as many bytes past a 16-byte boundary as
+    the logits' do, so that both move in 16-byte vectors: dense where whole rows are such vectors or the logits
+    are dense themselves, else with the logits' strides."""
+    b, n, v = x.shape
+    dense = v * x.element_size() % 16 == 0 or (x.is_contiguous() and x.data_ptr() % 16 == 0)
+    if dense or x.numel() == 0:
+        return torch.empty((b, n, v), dtype=x.dtype, device=x.device)
+    sb, sn = (x.stride(0) if b > 1 else 0), (x.stride(1) if n > 1 else 0)
+    span = (n - 1) * sn + v
+    if (n > 1 and sn < v) or (b > 1 and sb < span) or (b - 1) * sb + span > 2 * x.numel() + 64:
+        return torch.empty((b, n, v), dtype=x.dtype, device=x.device)  # overlapping or sparse rows
+    at = x.data_ptr() % 16 // x.element_size()
+    flat = torch.empty((b - 1) * sb + span + 16, dtype=x.dtype, device=x.device)
+    return flat.as_strided((b, n, v), (max(sb, span), max(sn, v), 1), at)
+
+
+class _Call:
+    """One loss call: the packed rows and terms, its tensors, and the workspace a backward pass reads."""
+
+    __slots__ = ("x", "mask", "temperature", "terms", "keep", "ws", "backward")
+
+    def rows(self, grad: torch.Tensor | None) -> bytes:
+        x = self.x
+        return _ROWS.pack(x.data_ptr(), x.stride(0), x.stride(1), *_array(grad), *_array(self.mask), x.shape[0],
+                          x.shape[1], x.shape[2], _DTYPES[x.dtype], self.temperature)
+
+
+def _call(x: torch.Tensor, mask, temperature: float, terms: bytes, keep: tuple, backward, what: str) -> _Call:
+    temperature = float(temperature)
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"{what}: the temperature must be positive and finite")
+    c = _Call()
+    c.x, c.mask, c.temperature, c.terms, c.keep, c.backward = x, mask, temperature, terms, keep, backward
+    nbytes = lib.pkv_loss_workspace_bytes(x.shape[0], x.shape[1])
+    if nbytes < 0:
+        raise ValueError(f"{what}: too many rows")
+    c.ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    return c
+
+
+def _stream(x: torch.Tensor) -> int:
+    return torch.cuda.current_stream(x.device).cuda_stream
+
+
+def _launch(fn, c: _Call, grad, outputs: tuple) -> None:
+    """``fn(rows, terms, *outputs, workspace)`` on the logits' device and its current stream."""
+    x = c.x
+    args = (c.rows(grad), c.terms, *[t if t is None else t.data_ptr() for t in outputs], c.ws.data_ptr(),
+            c.ws.numel(), _stream(x))
+    if x.device.index == torch.cuda.current_device():
+        st = fn(*args)
+    else:
+        with torch.cuda.device(x.device):
+            st = fn(*args)
+    if st:
+        _lib.raise_for_status(st)
+
+
+class _RowLoss(torch.autograd.Function):
+    """Forward: the loss call without a gradient.  Backward: the rows again, times the upstream gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, x, call, fn, outputs):
+        with torch.no_grad():
+            _launch(fn, call, None, outputs)
+        ctx.call = call
+        ctx.save_for_backward(logits, call.ws, *[t for t in call.keep if t is not None])
+        ctx.mark_non_differentiable(*[t for t in outputs[1:] if t is not None])
+        return outputs[:1] + tuple(t for t in outputs[1:] if t is not None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss, *_):
+        logits = ctx.saved_tensors[0]  # (also checks that nothing was changed in place since)
+        c = ctx.call
+        grad = _grad_like(c.x)
+        up = grad_loss.to(dtype=torch.float32, device=c.x.device)
+        _launch(c.backward, c, grad, (up,))
+        return grad.view(logits.shape) if grad.shape != logits.shape else grad, None, None, None, None
+
+
+def _run(fn, c: _Call, logits: torch.Tensor, outputs: tuple):
+    """The outputs of a differentiable call."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        got = iter(_RowLoss.apply(logits, c.x, c, fn, outputs))
+        return tuple(None if t is None else next(got) for t in outputs)
+    _launch(fn, c, None, outputs)
+    return outputs
+
+
+def _run_with_grad(fn, c: _Call, logits: torch.Tensor, outputs: tuple) -> torch.Tensor:
+    grad = _grad_like(c.x)
+    _launch(fn, c, grad, outputs)
+    return grad if grad.shape == logits.shape else grad.squeeze(0)
+
+
+def _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef, entropy_coef,
+            temperature, reduction, scale):
+    what = "policy_loss"
+    x = _logits(logits.detach() if isinstance(logits, torch.Tensor) else logits, what)
+    if not (clip_low >= 0 and clip_high >= 0):
+        raise ValueError(f"{what}: clip_low and clip_high must be >= 0")
+    tok = _rows_like(tokens, x, torch.int64, what, "tokens")
+    adv = _rows_like(advantages, x, torch.float32, what, "advantages", broadcast=True)
+    old = None if old_logprobs is None else _rows_like(old_logprobs, x, torch.float32, what, "old_logprobs")
+    ref = None if ref_logprobs is None else _rows_like(ref_logprobs, x, torch.float32, what, "ref_logprobs")
+    m = _mask(mask, x, what)
+    terms = _POLICY.pack(*_array(tok), *_array(adv), *_array(old), *_array(ref), clip_low, clip_high, kl_coef,
+                         entropy_coef, _reduction(reduction, what), scale)
+    c = _call(x, m, temperature, terms, (tok, adv, old, ref, m), lib.pkv_policy_loss_backward, what)
+    shape = logits.shape[:-1]
+    new = lambda: torch.empty(shape, dtype=torch.float32, device=x.device)  # noqa: E731
+    outputs = (torch.empty((), dtype=torch.float32, device=x.device), new(), None if ref is None else new(),
+               new() if entropy_coef else None)
+    return c, outputs
+
+
+def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Tensor,
+                old_logprobs: torch.Tensor | None = None, mask: torch.Tensor | None = None, *,
+                ref_logprobs: torch.Tensor | None = None, clip_low: float = 0.2, clip_high: float = 0.2,
+                kl_coef: float = 0.0, entropy_coef: float = 0.0, temperature: float = 1.0,
+                reduction: str = "token_mean", scale: float = 1.0) -> PolicyLoss:
+    """Clipped policy loss, differentiable in ``logits``.
+
+    With z = logits / temperature, lp = log_softmax(z)[token] and r = exp(lp - old_logprobs) a scored row's loss is
+
+        -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(ref - lp) - (ref - lp) - 1) - entropy_coef H
+
+    ``advantages`` are [B, T], or [B] (one a sequence).  ``old_logprobs=None`` is the step right after the rollout:
+    r is 1, with the gradient of lp.  ``reduction``: "token_mean" over all scored rows, "sequence_mean" the mean over
+    sequences with a scored row of their rows' mean, or "sum".  All inputs but ``logits`` are constants.
+    """
+    c, outputs = _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef,
+                         entropy_coef, temperature, reduction, scale)
+    return PolicyLoss(*_run(lib.pkv_policy_loss, c, logits, outputs))
+
+
+def policy_loss_and_grad(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Tensor,
+                         old_logprobs: torch.Tensor | None = None, mask: torch.Tensor | None = None, *,
+                         ref_logprobs: torch.Tensor | None = None, clip_low: float = 0.2, clip_high: float = 0.2,
+                         kl_coef: float = 0.0, entropy_coef: float = 0.0, temperature: float = 1.0,
+                         reduction: str = "token_mean", scale: float = 1.0) -> tuple[PolicyLoss, torch.Tensor]:
+    """``policy_loss`` and its gradient with respect to ``logits`` (their type), in one pass over HBM."""
+    c, outputs = _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef,
+                         entropy_coef, temperature, reduction, scale)
+    grad = _run_with_grad(lib.pkv_policy_loss, c, logits, outputs)
+    return PolicyLoss(*outputs), grad
+
+
+def _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, length_normalised, scale):
+    what = "preference_loss"
+    x = _logits(logits.detach() if isinstance(logits, torch.Tensor) else logits, what)
+    if logits.dim() != 3 or x.shape[0] % 2:
+        raise ValueError(f"{what}: logits must be [2 * pairs, length, vocab], the chosen answers first")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"{what}: label_smoothing must lie in [0, 1]")
+    tok = _rows_like(tokens, x, torch.int64, what, "tokens")
+    m = _mask(mask, x, what)
+    ref = ref_logprobs
+    if ref is not None:
+        if not isinstance(ref, torch.Tensor) or ref.device != x.device or tuple(ref.shape) != (x.shape[0],):
+            raise ValueError(f"{what}: ref_logprobs must be [2 * pairs] on the logits' device")
+        ref = ref.to(torch.float32).contiguous()
+    terms = _PREFERENCE.pack(*_array(tok), 0 if ref is None else ref.data_ptr(), beta, label_smoothing,
+                             int(bool(length_normalised)), scale)
+    c = _call(x, m, 1.0, terms, (tok, ref, m), lib.pkv_preference_loss_backward, what)
+    new = lambda *s: torch.empty(s, dtype=torch.float32, device=x.device)  # noqa: E731
+    return c, (new(), new(x.shape[0]), new(x.shape[0] // 2))
+
+
+def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | None = None,
+                    ref_logprobs: torch.Tensor | None = None, *, beta: float = 0.1, label_smoothing: float = 0.0,
+                    length_normalised: bool = False, scale: float = 1.0) -> PreferenceLoss:
+    """Preference loss over pairs of answers, differentiable in ``logits`` [2P, T, V].
+
+    Sequences 0 .. P-1 are the chosen answers, P .. 2P-1 the rejected ones.  S is the sum of a sequence's scored
+    token log-probabilities (their mean with ``length_normalised``), R the reference policy's
+    (``ref_logprobs`` [2P], None for 0), and a pair's loss
+
+        m = beta ((S_c - R_c) - (S_r - R_r)),  -(1 - label_smoothing) log sigmoid(m) - label_smoothing log sigmoid(-m)
+
+    averaged over the pairs.  A sequence without a scored row has S = 0.
+    """
+    c, outputs = _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, length_normalised, scale)
+    return PreferenceLoss(*_run(lib.pkv_preference_loss, c, logits, outputs))
+
+
+def preference_loss_and_grad(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | None = None,
+                             ref_logprobs: torch.Tensor | None = None, *, beta: float = 0.1,
+                             label_smoothing: float = 0.0, length_normalised: bool = False,
+                             scale: float = 1.0) -> tuple[PreferenceLoss, torch.Tensor]:
+    """``preference_loss`` and its gradient with respect to ``logits`` (their type)."""
+    c, outputs = _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, length_normalised, scale)
+    grad = _run_with_grad(lib.pkv_preference_loss, c, logits, outputs)
+    return PreferenceLoss(*outputs), grad
+
+
+def _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale):
+    what = "distillation_loss"
+    x = _logits(logits.detach() if isinstance(logits, torch.Tensor) else logits, what)
+    lists = []
+    for t, name, dtype in ((teacher_ids, "teacher_ids", torch.int64), (teacher_logits, "teacher_logits", torch.float32)):
+        if not isinstance(t, torch.Tensor) or t.device != x.device:
+            raise ValueError(f"{what}: {name} must be on the logits' device")
+        if t.dim() != logits.dim() or t.shape[:-1] != logits.shape[:-1] or not 1 <= t.shape[-1] <= _MAX_TOP:
+            raise ValueError(f"{what}: {name} must be {list(logits.shape[:-1])} + [k], k from 1 to {_MAX_TOP}, got "
+                             f"{tuple(t.shape)}")
+        if dtype == torch.int64 and (t.is_floating_point() or t.dtype == torch.bool):
+            raise ValueError(f"{what}: {name} must be integers")
+        t = t.unsqueeze(0) if t.dim() == 2 else t
+        t = t.to(dtype)
+        lists.append(t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous())
+    ids, tl = lists
+    if ids.shape != tl.shape:
+        raise ValueError(f"{what}: teacher_ids and teacher_logits must have the same shape")
+    lse = None if teacher_lse is None else _rows_like(teacher_lse, x, torch.float32, what, "teacher_lse")
+    m = _mask(mask, x, what)
+    terms = _DISTILLATION.pack(ids.data_ptr(), ids.stride(0), ids.stride(1), tl.data_ptr(), tl.stride(0), tl.stride(1),
+                               ids.shape[-1], *_array(lse), _reduction(reduction, what), scale)
+    c = _call(x, m, temperature, terms, (ids, tl, lse, m), lib.pkv_distillation_loss_backward, what)
+    return c, (torch.empty((), dtype=torch.float32, device=x.device),
+               torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device))
+
+
+def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                      mask: torch.Tensor | None = None, *, teacher_lse: torch.Tensor | None = None,
+                      temperature: float = 1.0, reduction: str = "token_mean", scale: float = 1.0) -> DistillationLoss:
+    """Divergence of the student's rows from a teacher's top logits, differentiable in ``logits``.
+
+    ``teacher_ids`` / ``teacher_logits`` [B, T, k] (k <= 256) list a row's likely tokens at the teacher and their
+    logits (``top_logits`` makes them); an id below 0 or a logit of -inf is an absent entry, an id may come twice.
+    q is the softmax of the list's logits / temperature, or, with ``teacher_lse`` (the log-sum-exp of the teacher's
+    whole row / temperature), the teacher's own probabilities, which then sum to less than 1.  A scored row's loss is
+
+        T^2 sum_k q_k (log q_k - log_softmax(logits / T)[id_k])
+
+    and 0 for a row whose entries are all absent (it counts in the means).  An id past the vocabulary makes the
+    loss and its row's gradient NaN.  ``reduction`` as in ``policy_loss``.
+    """
+    c, outputs = _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale)
+    return DistillationLoss(*_run(lib.pkv_distillation_loss, c, logits, outputs))
+
+
+def distillation_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                               mask: torch.Tensor | None = None, *, teacher_lse: torch.Tensor | None = None,
+                               temperature: float = 1.0, reduction: str = "token_mean",
+                               scale: float = 1.0) -> tuple[DistillationLoss, torch.Tensor]:
+    """``distillation_loss`` and its gradient with respect to ``logits`` (their type), in one pass over HBM."""
+    c, outputs = _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale)
+    grad = _run_with_grad(lib.pkv_distillation_loss, c, logits, outputs)
+    return DistillationLoss(*outputs), grad
+
+
+def top_logits(logits: torch.Tensor, k: int, *,
+               temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The k largest logits of each row (k <= 256): (values float32 [..., k], tokens int64 [..., k], the log-sum-exp
+    of logits / temperature [...]), largest first, equal ones by their column.  NaN counts as the largest value."""
+    what = "top_logits"
+    x = _logits(logits.detach() if isinstance(logits, torch.Tensor) else logits, what)
+    k = int(k)
+    if not 1 <= k <= min(_MAX_TOP, x.shape[-1]):
+        raise ValueError(f"{what}: k must be from 1 to {min(_MAX_TOP, x.shape[-1])}")
+    temperature = float(temperature)
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"{what}: the temperature must be positive and finite")
+    shape = logits.shape[:-1]
+    values = torch.empty((*shape, k), dtype=torch.float32, device=x.device)
+    tokens = torch.empty((*shape, k), dtype=torch.int64, device=x.device)
+    lse = torch.empty(shape, dtype=torch.float32, device=x.device)
+    rows = _ROWS.pack(x.data_ptr(), x.stride(0), x.stride(1), 0, 0, 0, 0, 0, 0, x.shape[0], x.shape[1], x.shape[2],
+                      _DTYPES[x.dtype], temperature)
+    with torch.cuda.device(x.device):
+        _lib.raise_for_status(lib.pkv_top_logits(rows, k, values.data_ptr(), tokens.data_ptr(), lse.data_ptr(),
+                                                 _stream(x)))
+    return values, tokens, lse
