@@ -129,6 +129,36 @@ __device__ __forceinline__ uint4 pack(const float (&f)[16 / sizeof(T)]) {
   return v;
 }
 
+// Two columns at once (sm_100's packed float32 operations).
+using f32x2 = unsigned long long;
+
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Add N columns to the running sums.
 template <bool ENT, int N>
 __device__ __forceinline__ void fold(RowSum& a, const float (&x)[N], Scale2 k) {
   float top = x[0];
@@ -141,12 +171,28 @@ __device__ __forceinline__ void fold(RowSum& a, const float (&x)[N], Scale2 k) {
     return;
   }
   if (top > a.m) sum_rescale(a, top, k);
+  if constexpr (N % 4 == 0) {
+    const f32x2 neg = pair(-a.m, -a.m), hi = pair(k.hi, k.hi), lo = pair(k.lo, k.lo);
+    f32x2 s[2] = {pair(a.s, 0.f), 0ull}, w = pair(a.w, 0.f);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = x[i] - a.m, y = fmaf(d, k.lo, d * k.hi);
-    const float e = ex2(y);
-    a.s += e;
-    if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
+    for (int i = 0; i < N; i += 2) {
+      const f32x2 d = add2(pair(x[i], x[i + 1]), neg);
+      const float2 y = unpair(fma2(d, lo, mul2(d, hi)));
+      const f32x2 e = pair(ex2(y.x), ex2(y.y));
+      s[(i / 2) & 1] = add2(s[(i / 2) & 1], e);
+      if (ENT) w = fma2(e, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), w);
+    }
+    const float2 t = unpair(add2(s[0], s[1])), u = unpair(w);
+    a.s = t.x + t.y;
+    if (ENT) a.w = u.x + u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = x[i] - a.m, y = fmaf(d, k.lo, d * k.hi);
+      const float e = ex2(y);
+      a.s += e;
+      if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
+    }
   }
 }
 

@@ -24,13 +24,18 @@
 
 #include "loss_rows.cuh"
 #include "pkv_b200.h"
+#include "pkv_device.cuh"
 #include "pkv_error.h"
 
 namespace pkv {
 namespace {
 
-constexpr int kLossThreads = 512;
+constexpr int kLossThreads = 512;  // consumers
 constexpr int kLossWarps = kLossThreads / 32;
+constexpr int kCtaThreads = kLossThreads + 64;  // + the copying warp and the teacher's warp
+constexpr int kChunkVecs = 1024;                // 16-byte vectors in a ring slot
+constexpr int kSlots = 13;
+constexpr int kMaxCluster = 8;
 constexpr float kLn2 = 0.6931471805599453f;
 
 enum Kind { kPolicy = 0, kPreference = 1, kDistill = 2 };
@@ -47,6 +52,7 @@ struct Tokens2 {
 struct LossHeader {
   int32_t n_active;
   int32_t ticket;
+  int32_t error;  // a bounded wait gave up: the loss becomes NaN
 };
 
 struct LossArgs {
@@ -76,23 +82,6 @@ struct LossArgs {
   float4* rec;            // [rows] {m, a, b, h} for a later backward pass (distillation: {m, a, w T, log q's norm})
   const float* upstream;  // device scalar the gradient is multiplied by, or null
 };
-
-__device__ __forceinline__ RowSum cta_sum(RowSum a, RowSum* smem, Scale2 k) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    RowSum b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, off);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, off);
-    b.w = __shfl_xor_sync(0xffffffffu, a.w, off);
-    sum_merge(a, b, k);
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = a;
-  __syncthreads();
-  a = smem[0];
-  for (int i = 1; i < kLossWarps; ++i) sum_merge(a, smem[i], k);
-  return a;
-}
 
 // What a row's gradient needs: dx_j = e_j (a + b y_j), + h at the token.
 struct RowGrad {
@@ -161,6 +150,7 @@ struct PlanArgs {
 __global__ void __launch_bounds__(1024) loss_plan_kernel(const PlanArgs A) {
   __shared__ int s_warp[33], s_full, s_total;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int n = A.batch * A.length;
   auto scored = [&](int b, int t) { return A.mask == nullptr || A.mask[b * A.mb + t * A.mt] != 0; };
   if (tid == 0) s_full = 0;
@@ -215,11 +205,30 @@ __global__ void __launch_bounds__(1024) loss_plan_kernel(const PlanArgs A) {
   if (tid == 0) {
     A.hdr->n_active = total;
     A.hdr->ticket = 0;
+    A.hdr->error = 0;
   }
 }
 
 // ---------------------------------------------------------------------------
 // Rows.
+
+// A vector of the gradient, the list's columns apart.
+template <bool ENT, typename T>
+__device__ __forceinline__ void grad_vec(float (&x)[16 / sizeof(T)], const RowGrad& o, Scale2 k) {
+  const f32x2 neg = pair(-o.m, -o.m), hi = pair(k.hi, k.hi), lo = pair(k.lo, k.lo), a = pair(o.a, o.a);
+#pragma unroll
+  for (int i = 0; i < 16 / (int)sizeof(T); i += 2) {
+    const f32x2 d = add2(pair(x[i], x[i + 1]), neg);
+    f32x2 y2 = mul2(d, hi);
+    if (sizeof(T) == 4) y2 = fma2(d, lo, y2);  // (half a step of 16 bits hides it)
+    const float2 y = unpair(y2);
+    const f32x2 e = pair(ex2(y.x), ex2(y.y));
+    f32x2 c = a;
+    if (ENT) c = fma2(pair(o.b, o.b), pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), a);
+    const float2 v = unpair(mul2(e, c));
+    x[i] = v.x, x[i + 1] = v.y;
+  }
+}
 
 template <bool ENT>
 __device__ __forceinline__ float grad_of(float x, const RowGrad& o, Scale2 k) {
@@ -233,186 +242,465 @@ __device__ __forceinline__ float teacher_logit(const LossArgs& A, int b, int t, 
   return id < 0 ? -INFINITY : v;  // an absent entry
 }
 
-__device__ double cta_sum_d(double v, double* smem) {
+// A row's teacher list as its warp leaves it for the others.
+struct TeacherRow {
+  double norm;             // log q = t / T - norm
+  double q_sum, qx, qlogq; // sums over the list of q, q x[id] and q log q (a NaN: an id past the vocabulary)
+  int32_t id[PKV_MAX_TOP]; // -1: not a column
+  float q[PKV_MAX_TOP];
+};
+
+struct alignas(128) LossShared {
+  uint64_t full[kSlots], empty[kSlots];
+  uint64_t teacher_full[2], teacher_empty[2], peers[2];
+  RowSum part[2][kLossWarps];
+  float4 peer[2][kMaxCluster];
+  double sum[kLossWarps];
+  int last, gave_up;
+  TeacherRow teacher[2];
+};
+
+// mbar_try_wait that also sees what other CTAs of the cluster sent.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Waits are bounded.  One that gives up marks the CTA: every later wait of it passes at once, so that all roles run
+// to their ends (their barriers included) and the loss is made NaN.
+template <bool CLUSTER = false>
+__device__ __forceinline__ void wait_or_mark(uint64_t* bar, uint32_t parity, LossShared& sh) {
+  auto passed = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+  if (passed()) return;
+  const long long start = clock64();
+  while (!passed()) {
+    if (*(volatile int*)&sh.gave_up) return;
+    if (clock64() - start > kWaitLimitCycles) {
+      *(volatile int*)&sh.gave_up = 1;
+      return;
+    }
+  }
+}
+
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kLossThreads) : "memory"); }
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// 16 bytes into the same shared-memory place of CTA `rank` of the cluster, counted on its barrier.
+__device__ __forceinline__ void send_peer(void* dst, uint64_t* bar, uint32_t rank, float4 v) {
+  uint32_t d, b;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_u32(dst)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(d),
+               "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(b)
+               : "memory");
+}
+
+__device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = smem[0];
-  for (int i = 1; i < kLossWarps; ++i) v += smem[i];
   return v;
 }
 
-// The log-sum-exp of a row's teacher logits / T over its list, or the teacher's own.  Computed in 64 bits: log q
-// would lose digits to a rounded norm.
-__device__ double teacher_norm(const LossArgs& A, int b, int t, double* smem) {
-  if (A.tlse.p) return (double)A.tlse.at(b, t);
-  int64_t id;
-  float top = -INFINITY;
-  for (int e = 0; e < A.k; ++e) top = fmaxf(top, teacher_logit(A, b, t, e, id));
-  if (top == -INFINITY) return 0.0;
-  double sum = 0.0;
-  for (int e = threadIdx.x; e < A.k; e += kLossThreads) {
-    const float v = teacher_logit(A, b, t, e, id);
-    if (v != -INFINITY) sum += (double)expf((float)(((double)v - (double)top) * A.inv_td));
+__device__ __forceinline__ RowSum warp_merge(RowSum a, int width, Scale2 k) {
+  for (int off = width / 2; off > 0; off >>= 1) {
+    RowSum b;
+    b.m = __shfl_xor_sync(0xffffffffu, a.m, off);
+    b.s = __shfl_xor_sync(0xffffffffu, a.s, off);
+    b.w = __shfl_xor_sync(0xffffffffu, a.w, off);
+    sum_merge(a, b, k);
   }
-  sum = cta_sum_d(sum, smem);
-  return (double)top * A.inv_td + log(sum);
+  return a;
 }
 
-template <typename T, int KIND, bool ENT, int PASS>
-__global__ void __launch_bounds__(kLossThreads) loss_rows_kernel(const LossArgs A) {
-  constexpr int VE = 16 / sizeof(T);
-  __shared__ RowSum s_sum[kLossWarps];
-  __shared__ double s_d[kLossWarps];
-  __shared__ int s_last;
-  const int tid = threadIdx.x;
-  const int n = A.batch * A.length, n_active = A.hdr->n_active;
-  const float up = A.upstream ? *A.upstream : 1.f;
-  for (int i = blockIdx.x; i < n; i += gridDim.x) {
-    const int row = A.list[i], b = row / A.length, t = row - b * A.length;
-    const T* x = (const T*)A.x + b * A.xb + t * A.xr;
-    T* g = (T*)A.g + b * A.gb + t * A.gr;
+// A row's place in memory and the part of it this CTA of its cluster has.
+template <typename T>
+struct RowPart {
+  int row, b, t;
+  const T* x;
+  int head, nvec;      // the row's aligned body, in vectors
+  int v0, nv, chunks;  // this CTA's vectors
+  __device__ RowPart(const LossArgs& A, int row_, int rank, int size) {
+    row = row_;
+    b = row / A.length, t = row - b * A.length;
+    x = (const T*)A.x + b * A.xb + t * A.xr;
     const RowSplit<T> sp(x, A.vocab);
-    const int edge = A.vocab - sp.nvec * VE;  // columns outside the body
-    RowGrad o{0.f, 0.f, 0.f, 0.f, -1, i >= n_active};
-    float wt = 0.f;
-    double qnorm = 0.0;
-    if (i >= n_active) {
-      if (PASS != kBackward && tid == 0) {
-        if (A.logprobs) A.logprobs[row] = 0.f;
-        if (A.kl_out) A.kl_out[row] = 0.f;
-        if (ENT && A.entropy) A.entropy[row] = 0.f;
-        A.row_val[row] = 0.0;
+    head = sp.head, nvec = sp.nvec;
+    const int per = (nvec + size - 1) / size;
+    v0 = min(nvec, rank * per);
+    nv = min(nvec, v0 + per) - v0;
+    chunks = (nv + kChunkVecs - 1) / kChunkVecs;
+  }
+  __device__ const uint4* body() const { return reinterpret_cast<const uint4*>(x + head) + v0; }
+};
+
+// The copying warp's and the consumers' common order of a row's chunks through the ring: the forward part takes
+// chunks 0 .. n-1 and leaves the last min(n, kSlots) in their slots; the gradient part takes those first, then the
+// others again (from L2).  Slots are filled and freed strictly in turn.
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == kSlots) slot = 0, phase ^= 1;
+  }
+  __device__ __forceinline__ void back(int n) {  // n <= kSlots
+    slot -= n;
+    if (slot < 0) slot += kSlots, phase ^= 1;
+  }
+};
+
+// Rows of a loss: forward sums, the row's terms, its gradient.
+//
+// Bound by HBM: a scored row is read once and its gradient written once.  One CTA an SM keeps 208 KB of rows in
+// flight or resident in a ring of 16 KB bulk copies: a row's gradient is made from the copy in shared memory (what
+// does not fit is read again while it is still in L2), and the next row's copies fly meanwhile.  Few rows are spread
+// over clusters: each CTA has a part of the columns, and the parts' sums cross by distributed shared memory.
+template <typename T, int KIND, bool ENT, int PASS>
+__global__ void __launch_bounds__(kCtaThreads, 1) loss_rows_kernel(const LossArgs A) {
+  constexpr int VE = 16 / sizeof(T);
+  extern __shared__ __align__(128) uint8_t dyn[];
+  uint4* slots = reinterpret_cast<uint4*>(dyn);
+  LossShared& sh = *reinterpret_cast<LossShared*>(dyn + kSlots * kChunkVecs * 16);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = cluster_rank(), size = cluster_size();
+  if (tid == 0) {
+    for (int i = 0; i < kSlots; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], kLossWarps);
+    for (int i = 0; i < 2; ++i)
+      mbar_init(&sh.teacher_full[i], 1), mbar_init(&sh.teacher_empty[i], kLossWarps), mbar_init(&sh.peers[i], 1);
+    sh.gave_up = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (size > 1) cluster_sync_all();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int n = A.batch * A.length, n_active = A.hdr->n_active;
+  const int first = blockIdx.x / size, step = gridDim.x / size;
+
+  if (warp == kLossWarps) {
+    if (lane == 0) {
+      Ring r;
+      int filled = 0;  // slots in use at the start are none
+      int row = first < n_active ? A.list[first] : 0;
+      for (int i = first; i < n_active; i += step) {
+        const RowPart<T> p(A, row, rank, size);
+        if (i + step < n_active) row = A.list[i + step];
+        const int kept = min(p.chunks, kSlots);
+        const int total = PASS == kFused ? 2 * p.chunks - kept : p.chunks;
+        for (int c = 0; c < total; ++c) {
+          const int at = c < p.chunks ? c : c - p.chunks;
+          if (filled == kSlots)
+            wait_or_mark(&sh.empty[r.slot], r.phase ^ 1, sh);
+          else
+            ++filled;
+          if (*(volatile int*)&sh.gave_up) break;
+          const int nv = min(kChunkVecs, p.nv - at * kChunkVecs);
+          mbar_arrive_expect_tx(&sh.full[r.slot], nv * 16);
+          bulk_copy_g2s(slots + r.slot * kChunkVecs, p.body() + at * kChunkVecs, nv * 16, &sh.full[r.slot]);
+          r.next();
+        }
+        if (*(volatile int*)&sh.gave_up) break;
       }
-      if (PASS == kForward) continue;
-    } else if (PASS == kBackward) {
-      const float4 r = A.rec[row];
-      const float f = up * (A.seq_g ? A.seq_g[b] : 1.f);
-      o = RowGrad{r.x, r.y * f, r.z * f, r.w * f, -1, false};
-      if (KIND == kDistill) {
-        o.b = 0.f;
-        wt = r.z * f;
-        qnorm = teacher_norm(A, b, t, s_d);
-        o.zero = f == 0.f;
+      if (*(volatile int*)&sh.gave_up) {
+        // Copies still in flight end before the CTA's shared memory goes.
+        for (int i = 0; i < kSlots; ++i)
+          if (i < r.slot || filled == kSlots) mbar_wait_bounded(&sh.full[i], i < r.slot ? r.phase : r.phase ^ 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kLossWarps + 1) {
+    if (KIND == kDistill) {
+      // The teacher's warp: q and its sums, a row or two ahead of the consumers.
+      int it = 0;
+      for (int i = first; i < n_active; i += step, ++it) {
+        const RowPart<T> p(A, A.list[i], rank, size);
+        TeacherRow& o = sh.teacher[it & 1];
+        if (it >= 2) wait_or_mark(&sh.teacher_empty[it & 1], ((it >> 1) & 1) ^ 1, sh);
+        constexpr int kPer = PKV_MAX_TOP / 32;
+        float v[kPer], x[kPer];
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const int j = lane + 32 * e;
+          v[e] = -INFINITY, x[e] = 0.f;
+          if (j < A.k) {
+            int64_t id;
+            v[e] = teacher_logit(A, p.b, p.t, j, id);
+            const bool column = id >= 0 && id < A.vocab;
+            if (PASS != kBackward && v[e] != -INFINITY) x[e] = column ? as_float(p.x[id]) : NAN;
+            o.id[j] = column ? (int32_t)id : -1;
+            top = fmaxf(top, v[e]);
+          }
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        // The norm in 64 bits: log q would lose digits to a rounded one.
+        double norm = 0.0;
+        if (A.tlse.p) {
+          norm = (double)A.tlse.at(p.b, p.t);
+        } else if (top > -INFINITY) {
+          double sum = 0.0;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e)
+            if (v[e] != -INFINITY) sum += (double)expf((float)(((double)v[e] - (double)top) * A.inv_td));
+          norm = (double)top * A.inv_td + log(warp_sum_d(sum));
+        }
+        double qs = 0.0, qx = 0.0, ql = 0.0;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const int j = lane + 32 * e;
+          float q = 0.f;
+          if (v[e] != -INFINITY) {
+            const double lq = (double)v[e] * A.inv_td - norm;
+            q = expf((float)lq);
+            qs += (double)q;
+            if (q != 0.f || x[e] != x[e]) {
+              qx += (double)q * (double)x[e];
+              ql += (double)q * lq;
+            }
+          }
+          if (j < A.k) o.q[j] = q;
+        }
+        qs = warp_sum_d(qs), qx = warp_sum_d(qx), ql = warp_sum_d(ql);
+        if (lane == 0) o.norm = norm, o.q_sum = qs, o.qx = qx, o.qlogq = ql;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.teacher_full[it & 1]);
+      }
+    }
+  } else {
+    const float up = A.upstream ? *A.upstream : 1.f;
+    const Scale2 ks = A.ks;
+    Ring r;
+    int it = 0;  // scored rows so far
+    int row_next = first < n ? A.list[first] : 0;
+    for (int i = first; i < n; i += step) {
+      const RowPart<T> p(A, row_next, rank, size);
+      if (i + step < n) row_next = A.list[i + step];
+      const int row = p.row, b = p.b, t = p.t;
+      // The columns outside the body are the first CTA's.
+      const int edge = rank == 0 ? A.vocab - p.nvec * VE : 0;
+      const int edge_col = tid < p.head ? tid : tid + p.nvec * VE;
+      const int kept = min(p.chunks, kSlots);
+      RowGrad o{0.f, 0.f, 0.f, 0.f, -1, i >= n_active};
+      float wt = 0.f;
+      const bool scored = i < n_active;
+      if (!scored) {
+        if (PASS != kBackward && tid == 0 && rank == 0) {
+          if (A.logprobs) A.logprobs[row] = 0.f;
+          if (A.kl_out) A.kl_out[row] = 0.f;
+          if (ENT && A.entropy) A.entropy[row] = 0.f;
+          A.row_val[row] = 0.0;
+        }
+        if (PASS == kForward) continue;
+      } else if (PASS == kBackward) {
+        const float4 rec = A.rec[row];
+        const float f = up * (A.seq_g ? A.seq_g[b] : 1.f);
+        o = RowGrad{rec.x, rec.y * f, rec.z * f, rec.w * f, -1, false};
+        if (KIND == kDistill) {
+          o.b = o.h = 0.f;
+          wt = rec.z * f;
+          o.zero = f == 0.f;
+          wait_or_mark(&sh.teacher_full[it & 1], (it >> 1) & 1, sh);
+        } else {
+          const int64_t tok = A.tokens.at(b, t);
+          o.tok = tok >= 0 && tok < A.vocab ? (int)tok : -1;
+          o.zero = o.a == 0.f && o.b == 0.f && o.h == 0.f;
+        }
       } else {
-        const int64_t tok = A.tokens.at(b, t);
-        o.tok = tok >= 0 && tok < A.vocab ? (int)tok : -1;
-        o.zero = o.a == 0.f && o.b == 0.f && o.h == 0.f;
+        // What the row's terms need is loaded now and used after the sums.
+        int64_t tok = 0;
+        float xt = 0.f;
+        if (KIND != kDistill) {
+          tok = A.tokens.at(b, t);
+          xt = tok >= 0 && tok < A.vocab ? as_float(p.x[tok]) : NAN;
+        }
+        RowSum a{-INFINITY, 0.f, 0.f};
+        for (int c = 0; c < p.chunks; ++c) {
+          wait_or_mark(&sh.full[r.slot], r.phase, sh);
+          const uint4* in = slots + r.slot * kChunkVecs;
+          const int nv = min(kChunkVecs, p.nv - c * kChunkVecs);
+          if (nv == kChunkVecs) {
+            float f[2 * VE];
+            float (&lo)[VE] = *reinterpret_cast<float (*)[VE]>(f);
+            float (&hi)[VE] = *reinterpret_cast<float (*)[VE]>(f + VE);
+            unpack<T>(in[tid], lo);
+            unpack<T>(in[tid + kLossThreads], hi);
+            fold<ENT>(a, f, ks);
+          } else {
+            for (int j = tid; j < nv; j += kLossThreads) {
+              float f[VE];
+              unpack<T>(in[j], f);
+              fold<ENT>(a, f, ks);
+            }
+          }
+          if (PASS == kForward || c < p.chunks - kept) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.empty[r.slot]);
+          }
+          r.next();
+        }
+        if (PASS == kFused) r.back(kept);
+        if (tid < edge) {
+          const float f[1] = {as_float(p.x[edge_col])};
+          fold<ENT>(a, f, ks);
+        }
+        // The CTA's sum: warps, then (every warp for itself) the warps' sums, then the cluster's.
+        a = warp_merge(a, 32, ks);
+        if (lane == 0) sh.part[it & 1][warp] = a;
+        consumers_sync();
+        a = warp_merge(sh.part[it & 1][lane & (kLossWarps - 1)], kLossWarps, ks);
+        if (size > 1) {
+          if (tid == 0) {
+            mbar_arrive_expect_tx(&sh.peers[it & 1], 16 * size);
+            for (int q = 0; q < size; ++q)
+              send_peer(&sh.peer[it & 1][rank], &sh.peers[it & 1], q, make_float4(a.m, a.s, a.w, 0.f));
+          }
+          wait_or_mark<true>(&sh.peers[it & 1], (it >> 1) & 1, sh);
+          const float4 v = sh.peer[it & 1][lane & (size - 1)];
+          a = warp_merge(RowSum{v.x, v.y, v.z}, size, ks);
+        }
+        const bool write = tid == 0 && rank == 0;
+        if (KIND == kPolicy) {
+          o = policy_tail<ENT>(A, row, b, t, a, xt, tok, write);
+        } else if (KIND == kPreference) {
+          const bool known = tok >= 0 && tok < A.vocab;
+          o = RowGrad{a.m, -1.f / a.s, 0.f, 1.f, 0, false};
+          if (write) A.row_val[row] = known ? (((double)xt - (double)a.m) * A.kd - log2_of(a.s)) * kLn2d : (double)NAN;
+        } else {
+          wait_or_mark(&sh.teacher_full[it & 1], (it >> 1) & 1, sh);
+          const TeacherRow& q = sh.teacher[it & 1];
+          // sum q (log q - log p), log p = ((x - m) k - log2 s) ln 2
+          const double w = (double)A.seq_w[b], tt = (double)A.temperature;
+          const double l = tt * tt * (q.qlogq - ((q.qx - q.q_sum * (double)a.m) * A.kd - q.q_sum * log2_of(a.s)) * kLn2d);
+          wt = (float)(w * tt);
+          o = RowGrad{a.m, l == l ? wt * (float)q.q_sum / a.s : NAN, 0.f, 0.f, -1, false};
+          if (write) {
+            A.kl_out[row] = (float)l;
+            A.row_val[row] = w * l;
+          }
+        }
+        if (PASS == kForward) {
+          if (write && A.rec)
+            A.rec[row] = KIND == kDistill ? make_float4(o.m, o.a, wt, 0.f) : make_float4(o.m, o.a, o.b, o.h);
+          if (KIND == kDistill) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.teacher_empty[it & 1]);
+          }
+          ++it;
+          continue;
+        }
       }
-    } else {
-      RowSum r{-INFINITY, 0.f, 0.f};
-      const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
-      for (int j = tid; j < sp.nvec; j += kLossThreads) {
-        float f[VE];
-        unpack<T>(body[j], f);
-        fold<ENT>(r, f, A.ks);
+      T* g = (T*)A.g + b * A.gb + t * A.gr;
+      uint4* out = reinterpret_cast<uint4*>(g + p.head) + p.v0;
+      const bool vec = ((uintptr_t)out & 15) == 0;
+      auto store = [&](int j, const float (&f)[VE]) {
+        if (vec) {
+          __stcs(out + j, pack<T>(f));
+        } else {
+#pragma unroll
+          for (int q = 0; q < VE; ++q) put(g + p.head + (p.v0 + j) * VE + q, f[q]);
+        }
+      };
+      if (!scored) {
+        const float f[VE] = {};
+        for (int j = tid; j < p.nv; j += kLossThreads) store(j, f);
+      } else {
+        const int hot_vec = o.tok < 0 ? -1 : (o.tok - p.head >= 0 ? (o.tok - p.head) / VE - p.v0 : -1);
+        for (int c = 0; c < p.chunks; ++c) {
+          const int at = PASS == kBackward ? c : (c < kept ? p.chunks - kept + c : c - kept);
+          wait_or_mark(&sh.full[r.slot], r.phase, sh);
+          const uint4* in = slots + r.slot * kChunkVecs;
+          const int nv = min(kChunkVecs, p.nv - at * kChunkVecs);
+          for (int j = tid; j < nv; j += kLossThreads) {
+            float f[VE] = {};
+            if (!o.zero) {
+              unpack<T>(in[j], f);
+              grad_vec<ENT, T>(f, o, ks);
+              if (at * kChunkVecs + j == hot_vec) {
+                const int hot = o.tok - p.head - (p.v0 + at * kChunkVecs + j) * VE;
+#pragma unroll
+                for (int q = 0; q < VE; ++q)
+                  if (q == hot) f[q] += o.h;
+              }
+            }
+            store(at * kChunkVecs + j, f);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[r.slot]);
+          r.next();
+        }
       }
       if (tid < edge) {
-        const float f[1] = {as_float(x[tid < sp.head ? tid : tid + sp.nvec * VE])};
-        fold<ENT>(r, f, A.ks);
+        float v = o.zero ? 0.f : grad_of<ENT>(as_float(p.x[edge_col]), o, ks);
+        if (!o.zero && edge_col == o.tok) v += o.h;
+        put(g + edge_col, v);
       }
-      r = cta_sum(r, s_sum, A.ks);
-      if (KIND == kPolicy) {
-        const int64_t tok = A.tokens.at(b, t);
-        const float xt = tok >= 0 && tok < A.vocab ? as_float(x[tok]) : NAN;
-        o = policy_tail<ENT>(A, row, b, t, r, xt, tok, tid == 0);
-      } else if (KIND == kPreference) {
-        const int64_t tok = A.tokens.at(b, t);
-        const bool known = tok >= 0 && tok < A.vocab;
-        const double lp = known ? (((double)as_float(x[tok]) - (double)r.m) * A.kd - log2_of(r.s)) * kLn2d
-                                : (double)NAN;
-        o = RowGrad{r.m, -1.f / r.s, 0.f, 1.f, 0, false};
-        if (tid == 0) A.row_val[row] = lp;
-      } else {
-        // sum q (log q - log p) over the teacher's list.
-        qnorm = teacher_norm(A, b, t, s_d);
-        double l = 0.0, q_sum = 0.0;
-        int64_t id;
-        for (int e = tid; e < A.k; e += kLossThreads) {
-          const float v = teacher_logit(A, b, t, e, id);
-          if (v == -INFINITY) continue;
-          const double lq = (double)v * A.inv_td - qnorm;
-          const double lp = id < A.vocab ? (((double)as_float(x[id]) - (double)r.m) * A.kd - log2_of(r.s)) * kLn2d : (double)NAN;
-          const float q = expf((float)lq);
-          l += q == 0.f && lp == lp ? 0.0 : (double)q * (lq - lp);
-          q_sum += (double)q;
+      if (KIND == kDistill && scored) {
+        // The list's columns, over what their vectors wrote.  An id that comes twice is written once, with both shares.
+        consumers_sync();
+        const TeacherRow& q = sh.teacher[it & 1];
+        const int c0 = p.head + p.v0 * VE, c1 = c0 + p.nv * VE;
+        if (tid < A.k && !o.zero) {
+          const int id = q.id[tid];
+          if (id >= 0 && ((id >= c0 && id < c1) || (rank == 0 && (id < p.head || id >= p.head + p.nvec * VE)))) {
+            float sum = 0.f;
+            int firstly = tid;
+            for (int f = 0; f < A.k; ++f) {
+              if (q.id[f] != id) continue;
+              firstly = min(firstly, f);
+              sum += q.q[f];
+            }
+            if (firstly == tid) put(g + id, grad_of<false>(as_float(p.x[id]), o, ks) - wt * sum);
+          }
         }
-        l = cta_sum_d(l, s_d);
-        q_sum = cta_sum_d(q_sum, s_d);
-        const float w = A.seq_w[b];
-        wt = w * A.temperature;
-        l *= (double)A.temperature * (double)A.temperature;
-        o = RowGrad{r.m, wt * (float)q_sum / r.s, 0.f, 0.f, -1, false};
-        if (l != l) o.a = NAN;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.teacher_empty[it & 1]);
+      }
+      if (scored) ++it;
+    }
+    if (tid == 0 && *(volatile int*)&sh.gave_up) atomicExch(&A.hdr->error, 1);
+    if (PASS != kBackward && KIND != kPreference) {
+      // The last CTA adds the rows' losses, always in the same order.
+      consumers_sync();
+      if (tid == 0) {
+        __threadfence();
+        sh.last = atomicAdd(&A.hdr->ticket, 1) == (int)gridDim.x - 1;
+      }
+      consumers_sync();
+      if (sh.last) {
+        __threadfence();
+        double sum = 0.0;
+        for (int i = tid; i < n_active; i += kLossThreads) sum += __ldcg(A.row_val + A.list[i]);
+        sum = warp_sum_d(sum);
+        if (lane == 0) sh.sum[warp] = sum;
+        consumers_sync();
         if (tid == 0) {
-          A.kl_out[row] = (float)l;
-          A.row_val[row] = (double)w * l;
+          for (int i = 1; i < kLossWarps; ++i) sum += sh.sum[i];
+          *A.loss = __ldcg(&A.hdr->error) ? NAN : (float)sum;
         }
-      }
-      if (PASS == kForward) {
-        if (tid == 0 && A.rec)
-          A.rec[row] = KIND == kDistill ? make_float4(o.m, o.a, wt, 0.f) : make_float4(o.m, o.a, o.b, o.h);
-        continue;
-      }
-    }
-    uint4* out = reinterpret_cast<uint4*>(g + sp.head);
-    const bool vec = ((uintptr_t)out & 15) == 0;
-    const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
-    for (int j = tid; j < sp.nvec; j += kLossThreads) {
-      float f[VE] = {};
-      if (!o.zero) {
-        unpack<T>(body[j], f);
-        const int hot = o.tok - (sp.head + j * VE);
-#pragma unroll
-        for (int q = 0; q < VE; ++q) f[q] = grad_of<ENT>(f[q], o, A.ks) + (q == hot ? o.h : 0.f);
-      }
-      if (vec) {
-        out[j] = pack<T>(f);
-      } else {
-#pragma unroll
-        for (int q = 0; q < VE; ++q) put(g + sp.head + j * VE + q, f[q]);
-      }
-    }
-    if (tid < edge) {
-      const int j = tid < sp.head ? tid : tid + sp.nvec * VE;
-      put(g + j, o.zero ? 0.f : grad_of<ENT>(as_float(x[j]), o, A.ks) + (j == o.tok ? o.h : 0.f));
-    }
-    if (KIND == kDistill && i < n_active && !o.zero) {
-      // The list's columns: an id that comes twice is written once, with both its shares.
-      __syncthreads();
-      for (int e = tid; e < A.k; e += kLossThreads) {
-        int64_t id, other;
-        const float v = teacher_logit(A, b, t, e, id);
-        if (id < 0 || id >= A.vocab) continue;
-        float q = expf((float)((double)v * A.inv_td - qnorm));
-        bool first = true;
-        for (int f = 0; f < A.k; ++f) {
-          if (f == e) continue;
-          const float u = teacher_logit(A, b, t, f, other);
-          if (other != id) continue;
-          first = first && f > e;
-          q += expf((float)((double)u * A.inv_td - qnorm));
-        }
-        if (first) put(g + id, grad_of<false>(as_float(x[id]), o, A.ks) - wt * q);
       }
     }
   }
-  if (PASS == kBackward || KIND == kPreference) return;
-  // The last CTA adds the rows' losses, always in the same order.
-  __syncthreads();
-  if (tid == 0) {
-    __threadfence();
-    s_last = atomicAdd(&A.hdr->ticket, 1) == (int)gridDim.x - 1;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  double sum = 0.0;
-  for (int i = tid; i < n_active; i += kLossThreads) sum += __ldcg(A.row_val + A.list[i]);
-  sum = cta_sum_d(sum, s_d);
-  if (tid == 0) *A.loss = (float)sum;
+  __syncwarp();
+  if (size > 1) cluster_sync_all();  // no CTA leaves while its peers may still send to it
 }
 
 // ---------------------------------------------------------------------------
@@ -508,20 +796,74 @@ Layout layout(int64_t batch, int64_t length) {
   return l;
 }
 
+constexpr int kDynBytes = kSlots * kChunkVecs * 16 + (int)sizeof(LossShared);
+static_assert(kDynBytes <= 232448, "a CTA's shared memory");
+
+int32_t sm_count(int* sms) {
+  static int counts[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status("device query");
+  if (dev < 64 && counts[dev]) {
+    *sms = counts[dev];
+    return PKV_OK;
+  }
+  if (cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return cuda_status("device query");
+  if (dev < 64) counts[dev] = *sms;
+  return PKV_OK;
+}
+
+// Launch `kernel` behind the kernel before it on the stream (it waits for that one itself).
+template <typename K, typename Args>
+int32_t launch_after(K kernel, int grid, int threads, int cluster, int smem, const Args& a, cudaStream_t st,
+                     const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kernel, a);
+  return cuda_status(what);
+}
+
+// CTAs that share a row: few rows are spread over the SMs by columns, as long as a CTA keeps at least a chunk.
+int row_cluster(int64_t rows, int64_t row_bytes, int sms) {
+  int c = 1;
+  while (c < kMaxCluster && rows * (2 * c) <= sms && row_bytes / (2 * c) >= kChunkVecs * 16) c *= 2;
+  return c;
+}
+
+template <typename T, int KIND, bool ENT, int PASS>
+int32_t launch_typed(const LossArgs& a, cudaStream_t st) {
+  int sms = 0;
+  const int32_t e = sm_count(&sms);
+  if (e != PKV_OK) return e;
+  auto* kernel = loss_rows_kernel<T, KIND, ENT, PASS>;
+  static bool ready[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !ready[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDynBytes) != cudaSuccess)
+      return cuda_status("loss rows shared memory");
+    if (dev < 64) ready[dev] = true;
+  }
+  const int64_t rows = (int64_t)a.batch * a.length;
+  const int c = row_cluster(rows, (int64_t)a.vocab * sizeof(T), sms);
+  const int grid = (int)std::min<int64_t>(rows, sms / c) * c;
+  return launch_after(kernel, grid, kCtaThreads, c, kDynBytes, a, st, "loss rows launch");
+}
+
 template <int KIND, bool ENT, int PASS>
 int32_t launch_rows(const LossArgs& a, int32_t dtype, cudaStream_t st) {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return cuda_status("device query");
-  const int grid = (int)std::min<int64_t>((int64_t)a.batch * a.length, 4ll * sms);
-  if (dtype == PKV_F32)
-    loss_rows_kernel<float, KIND, ENT, PASS><<<grid, kLossThreads, 0, st>>>(a);
-  else if (dtype == PKV_F16)
-    loss_rows_kernel<__half, KIND, ENT, PASS><<<grid, kLossThreads, 0, st>>>(a);
-  else
-    loss_rows_kernel<__nv_bfloat16, KIND, ENT, PASS><<<grid, kLossThreads, 0, st>>>(a);
-  return cuda_status("loss rows launch");
+  if (dtype == PKV_F32) return launch_typed<float, KIND, ENT, PASS>(a, st);
+  if (dtype == PKV_F16) return launch_typed<__half, KIND, ENT, PASS>(a, st);
+  return launch_typed<__nv_bfloat16, KIND, ENT, PASS>(a, st);
 }
 
 LossArgs row_args(const pkv_loss_rows* r, const Layout& l, uint8_t* ws) {
