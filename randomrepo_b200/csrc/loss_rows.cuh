@@ -28,11 +28,20 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// k = log2(e) / T to about 48 bits.  The second float matters to a sum over
-// many columns: its relative error would shift every log-probability the same way.
+// k = log2(e) / T, as a pair of floats where one is off by more than 2e-8 of
+// it (at T = 1 it is not): a sum over many columns shows the scale's error as
+// that much of log p, which is up to about 20.
 struct Scale2 {
   float hi, lo;
 };
+inline Scale2 scale_for(float temperature, double* kd) {
+  const double k = kLog2ed / (double)temperature;
+  Scale2 s{(float)k, 0.f};
+  if ((double)s.hi > k) s.hi = nextafterf(s.hi, 0.f);  // lo >= 0: a column of -inf stays -inf in x hi + x lo
+  if (k - (double)s.hi > 2e-8 * k) s.lo = (float)(k - (double)s.hi);
+  *kd = (double)s.hi + (double)s.lo;
+  return s;
+}
 
 __device__ __forceinline__ float ex2(float y) {
   float e;
@@ -40,14 +49,20 @@ __device__ __forceinline__ float ex2(float y) {
   return e;
 }
 
-// The running sums of a set of columns x: m = max x, s = sum 2^y and w = sum 2^y y, y = (x - m) k.  (The maximum is
-// subtracted before the scaling: a type's lowest finite value times k would be -inf.)
+// Columns x of a row are taken as y = x k + c, c = -(max x) k rounded once:
+// one fused multiply-add a column, and what is made of y later starts from
+// the same c.  Where max x k leaves the range in which that is safe (masks of
+// a type's lowest value everywhere), y = (x - max x) k.
+__device__ __forceinline__ float center(float m, Scale2 k) { return __fmul_rn(-m, k.hi); }  // (rounded: never part of another FMA)
+__device__ __forceinline__ bool far_out(float c) { return !(fabsf(c) < 1e30f); }
+// The running sums of a set of columns: m = max x, s = sum 2^y, w = sum 2^y y.
 struct RowSum {
   float m, s, w;
 };
 
 __device__ __forceinline__ void sum_rescale(RowSum& a, float m_new, Scale2 k) {
-  const float d = (a.m - m_new) * k.hi, f = ex2(d);
+  const float c = center(m_new, k);
+  const float d = far_out(c) ? (a.m - m_new) * k.hi : c - center(a.m, k), f = ex2(d);
   a.w = f > 0.f ? f * fmaf(d, a.s, a.w) : 0.f;  // (a NaN stays in s)
   a.s *= f;
   a.m = m_new;
@@ -158,26 +173,45 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   return r;
 }
 
-// Add N columns to the running sums.
-template <bool ENT, int N>
-__device__ __forceinline__ void fold(RowSum& a, const float (&x)[N], Scale2 k) {
-  float top = x[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-  if (!(top > -INFINITY)) {  // nothing but -inf, or NaN
+// The largest of N columns.  16-bit ones are compared two at a time as they come.
+template <typename T, int N>
+__device__ __forceinline__ float top_of(const uint4 (&v)[N]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (x[i] != x[i]) a.s = NAN;
-    return;
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v[i].x), __uint_as_float(v[i].y)),
+                         fmaxf(__uint_as_float(v[i].z), __uint_as_float(v[i].w))));
+    return m;
+  } else {
+    using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+    auto as2 = [](const uint32_t& u) { return *reinterpret_cast<const T2*>(&u); };
+    T2 m = as2(v[0].x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = __hmax2(m, __hmax2(__hmax2(as2(v[i].x), as2(v[i].y)), __hmax2(as2(v[i].z), as2(v[i].w))));
+    return fmaxf(as_float(m.x), as_float(m.y));
   }
-  if (top > a.m) sum_rescale(a, top, k);
-  if constexpr (N % 4 == 0) {
-    const f32x2 neg = pair(-a.m, -a.m), hi = pair(k.hi, k.hi), lo = pair(k.lo, k.lo);
+}
+
+// Add columns whose largest is `top` to the running sums.  LO: the scale has a second float.
+template <bool ENT, bool LO, int N>
+__device__ __forceinline__ void fold_near(RowSum& a, const float (&x)[N], float c, Scale2 k) {
+  if constexpr (N == 1) {
+    float y = fmaf(x[0], k.hi, c);
+    if (LO) y = fmaf(x[0], k.lo, y);
+    const float e = ex2(y);
+    a.s += e;
+    if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
+  } else {
+    static_assert(N % 2 == 0, "columns go in pairs");
+    const f32x2 cc = pair(c, c), hi = pair(k.hi, k.hi), lo = pair(k.lo, k.lo);
     f32x2 s[2] = {pair(a.s, 0.f), 0ull}, w = pair(a.w, 0.f);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      const f32x2 d = add2(pair(x[i], x[i + 1]), neg);
-      const float2 y = unpair(fma2(d, lo, mul2(d, hi)));
+      const f32x2 xx = pair(x[i], x[i + 1]);
+      f32x2 y2 = fma2(xx, hi, cc);
+      if (LO) y2 = fma2(xx, lo, y2);
+      const float2 y = unpair(y2);
       const f32x2 e = pair(ex2(y.x), ex2(y.y));
       s[(i / 2) & 1] = add2(s[(i / 2) & 1], e);
       if (ENT) w = fma2(e, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), w);
@@ -185,15 +219,41 @@ __device__ __forceinline__ void fold(RowSum& a, const float (&x)[N], Scale2 k) {
     const float2 t = unpair(add2(s[0], s[1])), u = unpair(w);
     a.s = t.x + t.y;
     if (ENT) a.w = u.x + u.y;
-  } else {
+  }
+}
+
+template <bool ENT, int N>
+__device__ __forceinline__ void fold(RowSum& a, const float (&x)[N], float top, Scale2 k) {
+  if (!(top > -INFINITY)) {  // nothing but -inf, or NaN
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (x[i] != x[i]) a.s = NAN;
+    return;
+  }
+  if (top > a.m) sum_rescale(a, top, k);
+  const float c = center(a.m, k);
+  if (far_out(c)) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float d = x[i] - a.m, y = fmaf(d, k.lo, d * k.hi);
-      const float e = ex2(y);
+      const float y = (x[i] - a.m) * k.hi, e = ex2(y);
       a.s += e;
       if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
     }
+  } else if (k.lo == 0.f) {
+    fold_near<ENT, false>(a, x, c, k);
+  } else {
+    fold_near<ENT, true>(a, x, c, k);
   }
+}
+
+// N vectors of a row's body.
+template <bool ENT, typename T, int N>
+__device__ __forceinline__ void fold_vecs(RowSum& a, const uint4 (&v)[N], Scale2 k) {
+  constexpr int VE = 16 / sizeof(T);
+  float f[N * VE];
+#pragma unroll
+  for (int i = 0; i < N; ++i) unpack<T>(v[i], *reinterpret_cast<float (*)[VE]>(f + i * VE));
+  fold<ENT>(a, f, top_of<T>(v), k);
 }
 
 }  // namespace pkv

@@ -4,7 +4,7 @@
 //
 // A row is one position's `vocab` logits x.  With z = x / T everything a loss
 // needs of a row is its base-2 log-sum-exp pair (m, s): m = max x, y_j =
-// (x_j - m) k, k = log2(e) / T, e_j = 2^y_j, s = sum e_j, p_j = e_j / s (and
+// x_j k - m k, k = log2(e) / T, e_j = 2^y_j, s = sum e_j, p_j = e_j / s (and
 // w = sum e_j y_j where the entropy H = ln 2 (log2 s - w / s) is asked for), plus a few
 // single logits (the token's, the teacher's list).  The gradient of every
 // loss here has the form
@@ -30,11 +30,6 @@
 namespace pkv {
 namespace {
 
-constexpr int kLossThreads = 512;  // consumers
-constexpr int kLossWarps = kLossThreads / 32;
-constexpr int kCtaThreads = kLossThreads + 64;  // + the copying warp and the teacher's warp
-constexpr int kChunkVecs = 1024;                // 16-byte vectors in a ring slot
-constexpr int kSlots = 13;
 constexpr int kMaxCluster = 8;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -90,13 +85,26 @@ struct RowGrad {
   bool zero;  // the gradient is zero whatever the logits
 };
 
+// log2 of a column's probability, in 64 bits.
+__device__ __forceinline__ double log2_prob(const LossArgs& A, const RowSum& r, float x) {
+  const float c = center(r.m, A.ks);
+  return (far_out(c) ? ((double)x - (double)r.m) * A.kd : (double)x * A.kd + (double)c) - log2_of(r.s);
+}
+
+// A scored row's own inputs, loaded before its sums are made.
+struct RowTerms {
+  int64_t tok;
+  float x_tok, w, adv, old, ref;
+};
+
 template <bool ENT>
-__device__ RowGrad policy_tail(const LossArgs& A, int row, int b, int t, RowSum r, float x_tok, int64_t tok, bool write) {
+__device__ __forceinline__ RowGrad policy_tail(const LossArgs& A, int row, RowSum r, const RowTerms& q, bool write) {
+  const int64_t tok = q.tok;
   const bool known = tok >= 0 && tok < A.vocab;
   const double log2s = log2_of(r.s);
-  const double lp = known ? (((double)x_tok - (double)r.m) * A.kd - log2s) * kLn2d : (double)NAN;
-  const float w = A.seq_w[b], adv = A.adv.at(b, t);
-  const float ratio = A.old.p ? expf((float)(lp - (double)A.old.at(b, t))) : (lp == lp ? 1.f : NAN);
+  const double lp = known ? log2_prob(A, r, q.x_tok) * kLn2d : (double)NAN;
+  const float w = q.w, adv = q.adv;
+  const float ratio = A.old.p ? expf((float)(lp - (double)q.old)) : (lp == lp ? 1.f : NAN);
   // -min(r A, clip(r) A): the clipped branch is the smaller one above the border for A > 0, below it for A < 0.
   const bool cut = (adv > 0.f && ratio > A.ratio_high) || (adv < 0.f && ratio < A.ratio_low);
   const float used = cut ? (adv > 0.f ? A.ratio_high : A.ratio_low) : ratio;
@@ -105,7 +113,7 @@ __device__ RowGrad policy_tail(const LossArgs& A, int row, int b, int t, RowSum 
   if (!(lp == lp)) l = g = NAN;
   float kl = 0.f;
   if (A.ref.p) {
-    const float d = (float)((double)A.ref.at(b, t) - lp);
+    const float d = (float)((double)q.ref - lp);
     const float em = expm1f(d);
     kl = em - d;
     l = fmaf(A.kl_coef, kl, l);
@@ -212,28 +220,31 @@ __global__ void __launch_bounds__(1024) loss_plan_kernel(const PlanArgs A) {
 // ---------------------------------------------------------------------------
 // Rows.
 
-// A vector of the gradient, the list's columns apart.
-template <bool ENT, typename T>
-__device__ __forceinline__ void grad_vec(float (&x)[16 / sizeof(T)], const RowGrad& o, Scale2 k) {
-  const f32x2 neg = pair(-o.m, -o.m), hi = pair(k.hi, k.hi), lo = pair(k.lo, k.lo), a = pair(o.a, o.a);
+// N columns of the gradient, the list's columns apart.
+template <bool ENT, typename T, int N>
+__device__ __forceinline__ void grad_columns(float (&x)[N], const RowGrad& o, Scale2 k) {
+  const float c = center(o.m, k);
+  if (far_out(c)) {
 #pragma unroll
-  for (int i = 0; i < 16 / (int)sizeof(T); i += 2) {
-    const f32x2 d = add2(pair(x[i], x[i + 1]), neg);
-    f32x2 y2 = mul2(d, hi);
-    if (sizeof(T) == 4) y2 = fma2(d, lo, y2);  // (half a step of 16 bits hides it)
-    const float2 y = unpair(y2);
-    const f32x2 e = pair(ex2(y.x), ex2(y.y));
-    f32x2 c = a;
-    if (ENT) c = fma2(pair(o.b, o.b), pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), a);
-    const float2 v = unpair(mul2(e, c));
-    x[i] = v.x, x[i + 1] = v.y;
+    for (int i = 0; i < N; ++i) {
+      const float y = (x[i] - o.m) * k.hi;
+      x[i] = ex2(y) * (ENT ? fmaf(o.b, fmaxf(y, -1e30f), o.a) : o.a);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float y = fmaf(x[i], k.hi, c);
+    if (sizeof(T) == 4 && k.lo != 0.f) y = fmaf(x[i], k.lo, y);  // (half a step of 16 bits hides it)
+    x[i] = ex2(y) * (ENT ? fmaf(o.b, fmaxf(y, -1e30f), o.a) : o.a);
   }
 }
 
-template <bool ENT>
+template <bool ENT, typename T>
 __device__ __forceinline__ float grad_of(float x, const RowGrad& o, Scale2 k) {
-  const float d = x - o.m, y = fmaf(d, k.lo, d * k.hi);
-  return ex2(y) * (ENT ? fmaf(o.b, fmaxf(y, -1e30f), o.a) : o.a);
+  float v[1] = {x};
+  grad_columns<ENT, T>(v, o, k);
+  return v[0];
 }
 
 __device__ __forceinline__ float teacher_logit(const LossArgs& A, int b, int t, int i, int64_t& id) {
@@ -244,18 +255,39 @@ __device__ __forceinline__ float teacher_logit(const LossArgs& A, int b, int t, 
 
 // A row's teacher list as its warp leaves it for the others.
 struct TeacherRow {
-  double norm;             // log q = t / T - norm
   double q_sum, qx, qlogq; // sums over the list of q, q x[id] and q log q (a NaN: an id past the vocabulary)
   int32_t id[PKV_MAX_TOP]; // -1: not a column
   float q[PKV_MAX_TOP];
 };
 
+// Shape of a launch: threads that work on the columns, 16-byte vectors of a ring slot each takes, ring slots, CTAs an SM.
+template <int THREADS, int VECS, int SLOTS, int CTAS>
+struct Shape {
+  static constexpr int kGroup = THREADS, kVecs = VECS, kSlots = SLOTS, kCtas = CTAS;
+  static constexpr int kChunk = VECS * THREADS;  // vectors of a slot
+  static constexpr int kWarps = THREADS / 32;
+  static constexpr int kCopyWarp = kWarps, kTeacherWarp = kWarps + 1, kTermsWarp = kWarps + 2;
+  static constexpr int kThreads = THREADS + 96;
+  static constexpr int kRingBytes = SLOTS * kChunk * 16;
+};
+// Measured on rows of 151 936 columns.  Sums or gradient alone: four CTAs of 128 threads that take 8 vectors at a time
+// (16-bit sums of 4 096 rows 227 us; 256 threads x 2 CTAs 238, 512 threads x 4 vectors x 1 CTA 275).  Both in one
+// launch: two CTAs an SM hide each other's turns between the passes, and a larger chunk its waits (499 us; one CTA of
+// 768 threads 494, of 512 threads with 2 vectors 580) -- but for float32, whose rows in flight would then overflow L2
+// before they are read again, one CTA (8 192 rows 1.85 ms against 2.23 ms).
+template <typename T, int PASS> struct ShapeOf : Shape<128, 8, 3, 4> {};
+template <typename T> struct ShapeOf<T, kFused> : Shape<384, 4, 4, 2> {};
+template <> struct ShapeOf<float, kFused> : Shape<512, 4, 6, 1> {};
+
+template <typename S>
 struct alignas(128) LossShared {
-  uint64_t full[kSlots], empty[kSlots];
-  uint64_t teacher_full[2], teacher_empty[2], peers[2];
-  RowSum part[2][kLossWarps];
+  uint64_t full[S::kSlots], empty[S::kSlots];
+  uint64_t part_full[2], part_empty[2], grad_full[2], grad_empty[2], teacher_full[2], teacher_empty[2], peers[2];
   float4 peer[2][kMaxCluster];
-  double sum[kLossWarps];
+  RowSum part[2][32];
+  RowGrad grad[2];
+  float grad_wt[2];
+  double sum[32];
   int last, gave_up;
   TeacherRow teacher[2];
 };
@@ -275,8 +307,8 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
 
 // Waits are bounded.  One that gives up marks the CTA: every later wait of it passes at once, so that all roles run
 // to their ends (their barriers included) and the loss is made NaN.
-template <bool CLUSTER = false>
-__device__ __forceinline__ void wait_or_mark(uint64_t* bar, uint32_t parity, LossShared& sh) {
+template <bool CLUSTER = false, typename Sh>
+__device__ __forceinline__ void wait_or_mark(uint64_t* bar, uint32_t parity, Sh& sh) {
   auto passed = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
   if (passed()) return;
   const long long start = clock64();
@@ -288,8 +320,6 @@ __device__ __forceinline__ void wait_or_mark(uint64_t* bar, uint32_t parity, Los
     }
   }
 }
-
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kLossThreads) : "memory"); }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -333,7 +363,7 @@ __device__ __forceinline__ RowSum warp_merge(RowSum a, int width, Scale2 k) {
 }
 
 // A row's place in memory and the part of it this CTA of its cluster has.
-template <typename T>
+template <typename T, int CHUNK>
 struct RowPart {
   int row, b, t;
   const T* x;
@@ -348,44 +378,407 @@ struct RowPart {
     const int per = (nvec + size - 1) / size;
     v0 = min(nvec, rank * per);
     nv = min(nvec, v0 + per) - v0;
-    chunks = (nv + kChunkVecs - 1) / kChunkVecs;
+    chunks = (nv + CHUNK - 1) / CHUNK;
   }
   __device__ const uint4* body() const { return reinterpret_cast<const uint4*>(x + head) + v0; }
 };
 
-// The copying warp's and the consumers' common order of a row's chunks through the ring: the forward part takes
-// chunks 0 .. n-1 and leaves the last min(n, kSlots) in their slots; the gradient part takes those first, then the
-// others again (from L2).  Slots are filled and freed strictly in turn.
+// A place in the ring.  Slots are filled, looked at and freed strictly in turn: a row's chunks 0 .. n-1 for its sums,
+// the last min(n, kSlots) of which stay in their slots for its gradient, which takes them first; then, behind those,
+// the others again (from L2).
+template <int SLOTS>
 struct Ring {
   int slot = 0;
   uint32_t phase = 0;
   __device__ __forceinline__ void next() {
-    if (++slot == kSlots) slot = 0, phase ^= 1;
+    if (++slot == SLOTS) slot = 0, phase ^= 1;
   }
-  __device__ __forceinline__ void back(int n) {  // n <= kSlots
+  __device__ __forceinline__ void back(int n) {  // n <= SLOTS
     slot -= n;
-    if (slot < 0) slot += kSlots, phase ^= 1;
+    if (slot < 0) slot += SLOTS, phase ^= 1;
   }
 };
 
-// Rows of a loss: forward sums, the row's terms, its gradient.
-//
-// Bound by HBM: a scored row is read once and its gradient written once.  One CTA an SM keeps 208 KB of rows in
-// flight or resident in a ring of 16 KB bulk copies: a row's gradient is made from the copy in shared memory (what
-// does not fit is read again while it is still in L2), and the next row's copies fly meanwhile.  Few rows are spread
-// over clusters: each CTA has a part of the columns, and the parts' sums cross by distributed shared memory.
-template <typename T, int KIND, bool ENT, int PASS>
-__global__ void __launch_bounds__(kCtaThreads, 1) loss_rows_kernel(const LossArgs A) {
+// The copying warp (one lane of it).
+template <typename T, int PASS, typename S, typename Sh>
+__device__ __forceinline__ void copy_rows(const LossArgs& A, Sh& sh, uint4* slots, int rank, int size, int first,
+                                          int step, int n_active) {
+  Ring<S::kSlots> r;
+  int filled = 0;
+  // Chunks read twice are asked to stay in L2 until then; the others leave it first.
+  uint64_t keep_policy;
+  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep_policy));
+  const uint64_t once_policy = l2_evict_first_policy();
+  int row = first < n_active ? A.list[first] : 0;
+  for (int i = first; i < n_active; i += step) {
+    const RowPart<T, S::kChunk> p(A, row, rank, size);
+    if (i + step < n_active) row = A.list[i + step];
+    const int again = PASS == kFused ? p.chunks - min(p.chunks, S::kSlots) : 0;
+    for (int c = 0; c < p.chunks + again; ++c) {
+      const int at = c < p.chunks ? c : c - p.chunks;
+      if (filled == S::kSlots)
+        wait_or_mark(&sh.empty[r.slot], r.phase ^ 1, sh);
+      else
+        ++filled;
+      if (*(volatile int*)&sh.gave_up) {
+        // Copies still in flight end before the CTA's shared memory goes.
+        for (int k = 0; k < S::kSlots; ++k)
+          if (k < r.slot || filled == S::kSlots) mbar_wait_bounded(&sh.full[k], k < r.slot ? r.phase : r.phase ^ 1);
+        return;
+      }
+      const int nv = min(S::kChunk, p.nv - at * S::kChunk);
+      mbar_arrive_expect_tx(&sh.full[r.slot], nv * 16);
+      bulk_copy_g2s_hint(slots + r.slot * S::kChunk, p.body() + at * S::kChunk, nv * 16, &sh.full[r.slot],
+                         c < again ? keep_policy : once_policy);
+      r.next();
+    }
+  }
+}
+
+// The teacher's warp: q and its sums, a row or two ahead.
+template <typename T, int PASS, typename S, typename Sh>
+__device__ __forceinline__ void teacher_rows(const LossArgs& A, Sh& sh, int rank, int size, int first, int step,
+                                             int n_active, int lane) {
+  int it = 0;
+  for (int i = first; i < n_active; i += step, ++it) {
+    const RowPart<T, S::kChunk> p(A, A.list[i], rank, size);
+    TeacherRow& o = sh.teacher[it & 1];
+    if (it >= 2) wait_or_mark(&sh.teacher_empty[it & 1], ((it >> 1) & 1) ^ 1, sh);
+    constexpr int kPer = PKV_MAX_TOP / 32;
+    float v[kPer], x[kPer];
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int j = lane + 32 * e;
+      v[e] = -INFINITY, x[e] = 0.f;
+      if (j < A.k) {
+        int64_t id;
+        v[e] = teacher_logit(A, p.b, p.t, j, id);
+        const bool column = id >= 0 && id < A.vocab;
+        if (PASS != kBackward && v[e] != -INFINITY) x[e] = column ? as_float(p.x[id]) : NAN;
+        o.id[j] = column ? (int32_t)id : -1;
+        top = fmaxf(top, v[e]);
+      }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    // The norm in 64 bits: log q would lose digits to a rounded one.
+    double norm = 0.0;
+    if (A.tlse.p) {
+      norm = (double)A.tlse.at(p.b, p.t);
+    } else if (top > -INFINITY) {
+      double sum = 0.0;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (v[e] != -INFINITY) sum += (double)expf((float)(((double)v[e] - (double)top) * A.inv_td));
+      norm = (double)top * A.inv_td + log(warp_sum_d(sum));
+    }
+    double qs = 0.0, qx = 0.0, ql = 0.0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int j = lane + 32 * e;
+      float q = 0.f;
+      if (v[e] != -INFINITY) {
+        const double lq = (double)v[e] * A.inv_td - norm;
+        q = expf((float)lq);
+        qs += (double)q;
+        if (q != 0.f || x[e] != x[e]) {
+          qx += (double)q * (double)x[e];
+          ql += (double)q * lq;
+        }
+      }
+      if (j < A.k) o.q[j] = q;
+    }
+    qs = warp_sum_d(qs), qx = warp_sum_d(qx), ql = warp_sum_d(ql);
+    if (lane == 0) o.q_sum = qs, o.qx = qx, o.qlogq = ql;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.teacher_full[it & 1]);
+  }
+}
+
+// The warp of the rows' terms: it has a row's own inputs in hand when its sums are done, and hands on its gradient's
+// coefficients (in the backward pass, those the forward pass left).
+template <typename T, int KIND, bool ENT, int PASS, typename S, typename Sh>
+__device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, int size, int first, int step,
+                                          int n_active, int n, int lane) {
+  const bool write = lane == 0 && rank == 0;
+  const Scale2 ks = A.ks;
+  const float up = A.upstream ? *A.upstream : 1.f;
+  int row_next = first < n_active ? A.list[first] : 0;
+  int64_t tok_next = 0;
+  if (KIND != kDistill && first < n_active) tok_next = A.tokens.at(row_next / A.length, row_next % A.length);
+  for (int i = first, it = 0; i < n_active; i += step, ++it) {
+    const int row = row_next, b = row / A.length, t = row - b * A.length, par = it & 1;
+    const uint32_t phase = (it >> 1) & 1;
+    if (i + step < n_active) row_next = A.list[i + step];
+    RowTerms q{tok_next, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const bool known = q.tok >= 0 && q.tok < A.vocab;
+    if (KIND != kDistill && i + step < n_active) tok_next = A.tokens.at(row_next / A.length, row_next % A.length);
+    RowGrad o{0.f, 0.f, 0.f, 0.f, -1, false};
+    float wt = 0.f;
+    if (PASS == kBackward) {
+      const float4 rec = A.rec[row];
+      const float f = up * (A.seq_g ? A.seq_g[b] : 1.f);
+      if (KIND == kDistill) {
+        o = RowGrad{rec.x, rec.y * f, 0.f, 0.f, -1, f == 0.f};
+        wt = rec.z * f;
+      } else {
+        o = RowGrad{rec.x, rec.y * f, rec.z * f, rec.w * f, known ? (int)q.tok : -1, false};
+        o.zero = o.a == 0.f && o.b == 0.f && o.h == 0.f;
+      }
+    } else {
+      const T* x = (const T*)A.x + b * A.xb + t * A.xr;
+      if (KIND != kPreference) q.w = A.seq_w[b];
+      if (KIND != kDistill) q.x_tok = known ? as_float(x[q.tok]) : NAN;
+      if (KIND == kPolicy) {
+        q.adv = A.adv.at(b, t);
+        if (A.old.p) q.old = A.old.at(b, t);
+        if (A.ref.p) q.ref = A.ref.at(b, t);
+      }
+      wait_or_mark(&sh.part_full[par], phase, sh);
+      RowSum a = warp_merge(lane < S::kWarps ? sh.part[par][lane] : RowSum{-INFINITY, 0.f, 0.f}, 32, ks);
+      if (lane == 0) mbar_arrive(&sh.part_empty[par]);
+      if (size > 1) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sh.peers[par], 16 * size);
+          for (int c = 0; c < size; ++c)
+            send_peer(&sh.peer[par][rank], &sh.peers[par], c, make_float4(a.m, a.s, a.w, 0.f));
+        }
+        __syncwarp();
+        wait_or_mark<true>(&sh.peers[par], phase, sh);
+        const float4 v = sh.peer[par][lane & (size - 1)];
+        a = warp_merge(RowSum{v.x, v.y, v.z}, size, ks);
+      }
+      if (KIND == kPolicy) {
+        o = policy_tail<ENT>(A, row, a, q, write);
+      } else if (KIND == kPreference) {
+        o = RowGrad{a.m, -1.f / a.s, 0.f, 1.f, 0, false};
+        if (write) A.row_val[row] = known ? log2_prob(A, a, q.x_tok) * kLn2d : (double)NAN;
+      } else {
+        wait_or_mark(&sh.teacher_full[par], phase, sh);
+        const TeacherRow& te = sh.teacher[par];
+        // sum q (log q - log p), log p = (x k + c - log2 s) ln 2
+        const double w = (double)q.w, tt = (double)A.temperature;
+        const float c = center(a.m, ks);
+        double qp = te.qx * A.kd + te.q_sum * ((double)c - log2_of(a.s));  // sum q log2 p
+        if (far_out(c) && qp == qp) {
+          qp = 0.0;
+          for (int f = 0; f < A.k; ++f)
+            if (te.id[f] >= 0 && te.q[f] > 0.f) qp += (double)te.q[f] * log2_prob(A, a, as_float(x[te.id[f]]));
+        }
+        const double l = tt * tt * (te.qlogq - qp * kLn2d);
+        wt = (float)(w * tt);
+        o = RowGrad{a.m, l == l ? wt * (float)te.q_sum / a.s : NAN, 0.f, 0.f, -1, false};
+        if (write) {
+          A.kl_out[row] = (float)l;
+          A.row_val[row] = w * l;
+        }
+      }
+      if (PASS == kForward) {
+        if (write && A.rec)
+          A.rec[row] = KIND == kDistill ? make_float4(o.m, o.a, wt, 0.f) : make_float4(o.m, o.a, o.b, o.h);
+        if (KIND == kDistill) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.teacher_empty[par]);
+        }
+        continue;
+      }
+    }
+    if (it >= 2) wait_or_mark(&sh.grad_empty[par], phase ^ 1, sh);
+    if (lane == 0) {
+      sh.grad[par] = o;
+      sh.grad_wt[par] = wt;
+      mbar_arrive(&sh.grad_full[par]);
+    }
+  }
+  // Rows that are not scored have zeros.
+  if (PASS != kBackward && rank == 0) {
+    for (int i = n_active + first + step * lane; i < n; i += 32 * step) {
+      const int row = A.list[i];
+      if (A.logprobs) A.logprobs[row] = 0.f;
+      if (A.kl_out) A.kl_out[row] = 0.f;
+      if (ENT && A.entropy) A.entropy[row] = 0.f;
+      A.row_val[row] = 0.0;
+    }
+  }
+}
+
+// The warps that work on the columns: a row's sums, then its gradient.
+template <typename T, int KIND, bool ENT, int PASS, typename S, typename Sh>
+__device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uint4* slots, int rank, int size,
+                                            int first, int step, int n_active, int n, int tid) {
   constexpr int VE = 16 / sizeof(T);
+  const int lane = tid & 31, warp = tid >> 5;
+  const Scale2 ks = A.ks;
+  Ring<S::kSlots> r;
+  const int end = PASS == kForward ? n_active : n;
+  int row = first < end ? A.list[first] : 0;
+  for (int i = first, it = 0; i < end; i += step) {
+    const RowPart<T, S::kChunk> p(A, row, rank, size);
+    if (i + step < end) row = A.list[i + step];
+    // The columns outside the body are the cluster's first CTA's.
+    const int edge = rank == 0 ? A.vocab - p.nvec * VE : 0;
+    const int edge_col = tid < p.head ? tid : tid + p.nvec * VE;
+    const int par = it & 1;
+    const uint32_t phase = (it >> 1) & 1;
+    const int again = PASS == kFused ? p.chunks - min(p.chunks, S::kSlots) : 0;
+    if (PASS != kBackward && i < n_active) {
+      RowSum a{-INFINITY, 0.f, 0.f};
+      for (int c = 0; c < p.chunks; ++c) {
+        wait_or_mark(&sh.full[r.slot], r.phase, sh);
+        const uint4* in = slots + r.slot * S::kChunk;
+        const int nv = min(S::kChunk, p.nv - c * S::kChunk);
+        if (nv == S::kChunk) {
+          constexpr int kAtOnce = 4;
+          static_assert(S::kVecs % kAtOnce == 0, "vectors are taken four at a time");
+#pragma unroll
+          for (int h = 0; h < S::kVecs; h += kAtOnce) {
+            uint4 v[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) v[u] = in[tid + (h + u) * S::kGroup];
+            fold_vecs<ENT, T>(a, v, ks);
+          }
+        } else {
+          for (int j = tid; j < nv; j += S::kGroup) {
+            const uint4 v[1] = {in[j]};
+            fold_vecs<ENT, T>(a, v, ks);
+          }
+        }
+        if (PASS == kForward || c < again) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[r.slot]);
+        }
+        r.next();
+      }
+      if (PASS == kFused) r.back(p.chunks - again);
+      if (tid < edge) {
+        const float f[1] = {as_float(p.x[edge_col])};
+        fold<ENT>(a, f, f[0], ks);
+      }
+      a = warp_merge(a, 32, ks);
+      if (it >= 2) wait_or_mark(&sh.part_empty[par], phase ^ 1, sh);
+      if (lane == 0) {
+        sh.part[par][warp] = a;
+        mbar_arrive(&sh.part_full[par]);
+      }
+    }
+    if (PASS == kForward) {
+      ++it;
+      continue;
+    }
+    T* g = (T*)A.g + p.b * A.gb + p.t * A.gr;
+    uint4* out = reinterpret_cast<uint4*>(g + p.head) + p.v0;
+    const bool vec = ((uintptr_t)out & 15) == 0;
+    // (Rows whose gradient starts elsewhere in its 16 bytes are stored a column at a time.)
+    auto store = [&](int j, uint4 v) {
+      if (vec) {
+        __stcs(out + j, v);
+      } else {
+        const T* f = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int q = 0; q < VE; ++q) g[p.head + (p.v0 + j) * VE + q] = f[q];
+      }
+    };
+    if (i >= n_active) {
+      for (int j = tid; j < p.nv; j += S::kGroup) store(j, make_uint4(0u, 0u, 0u, 0u));
+      if (tid < edge) put(g + edge_col, 0.f);
+      continue;
+    }
+    ++it;
+    wait_or_mark(&sh.grad_full[par], phase, sh);
+    const RowGrad o = sh.grad[par];
+    const float wt = KIND == kDistill ? sh.grad_wt[par] : 0.f;
+    const int hot_vec = o.tok < p.head ? -1 : (o.tok - p.head) / VE - p.v0;
+    for (int c = 0; c < p.chunks; ++c) {
+      const int at = c + again < p.chunks ? c + again : c + again - p.chunks;
+      wait_or_mark(&sh.full[r.slot], r.phase, sh);
+      const uint4* in = slots + r.slot * S::kChunk;
+      const int j0 = at * S::kChunk, nv = min(S::kChunk, p.nv - j0);
+      const bool hot_here = (unsigned)(hot_vec - j0) < (unsigned)nv;
+      if (vec && !o.zero && nv == S::kChunk && !hot_here) {
+#pragma unroll
+        for (int u = 0; u < S::kVecs; ++u) {
+          float f[VE];
+          unpack<T>(in[tid + u * S::kGroup], f);
+          grad_columns<ENT, T>(f, o, ks);
+          __stcs(out + j0 + tid + u * S::kGroup, pack<T>(f));
+        }
+      } else {
+        for (int j = tid; j < nv; j += S::kGroup) {
+          float f[VE] = {};
+          if (!o.zero) {
+            unpack<T>(in[j], f);
+            grad_columns<ENT, T>(f, o, ks);
+            if (j0 + j == hot_vec) {
+              const int hot = (o.tok - p.head) % VE;
+#pragma unroll
+              for (int q = 0; q < VE; ++q)
+                if (q == hot) f[q] += o.h;
+            }
+          }
+          store(j0 + j, pack<T>(f));
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[r.slot]);
+      r.next();
+    }
+    if (tid < edge) {
+      float v = o.zero ? 0.f : grad_of<ENT, T>(as_float(p.x[edge_col]), o, ks);
+      if (!o.zero && edge_col == o.tok) v += o.h;
+      put(g + edge_col, v);
+    }
+    if (KIND == kDistill) {
+      // The list's columns, over what their vectors wrote.  An id that comes twice is written once, with both shares.
+      if (PASS == kBackward) wait_or_mark(&sh.teacher_full[par], phase, sh);
+      asm volatile("bar.sync 1, %0;" ::"n"(S::kGroup) : "memory");
+      const TeacherRow& q = sh.teacher[par];
+      const int c0 = p.head + p.v0 * VE, c1 = c0 + p.nv * VE;
+      for (int e = tid; e < A.k && !o.zero; e += S::kGroup) {
+        const int id = q.id[e];
+        if (id < 0 || !((id >= c0 && id < c1) || (rank == 0 && (id < p.head || id >= p.head + p.nvec * VE)))) continue;
+        float sum = 0.f;
+        int firstly = e;
+        for (int f = 0; f < A.k; ++f) {
+          if (q.id[f] != id) continue;
+          firstly = min(firstly, f);
+          sum += q.q[f];
+        }
+        if (firstly == e) put(g + id, grad_of<false, T>(as_float(p.x[id]), o, ks) - wt * sum);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(&sh.grad_empty[par]);
+      if (KIND == kDistill) mbar_arrive(&sh.teacher_empty[par]);
+    }
+  }
+}
+
+// Rows of a loss: sums, terms, gradient.
+//
+// Bound by HBM and the exponentials: a scored row is read once and its gradient written once, with two exponentials a
+// column.  A CTA keeps its rows in a ring of bulk copies: the gradient is made mostly from the chunks still in the
+// ring, the rest is read again while it is in L2.  One warp copies, one takes a finished row's sums to its
+// coefficients, the others work on the columns.  Few rows are spread over clusters: each CTA has a part of the
+// columns, and the parts' sums cross by distributed shared memory.
+template <typename T, int KIND, bool ENT, int PASS>
+__global__ void __launch_bounds__(ShapeOf<T, PASS>::kThreads, ShapeOf<T, PASS>::kCtas) loss_rows_kernel(const LossArgs A) {
+  using S = ShapeOf<T, PASS>;
+  using Sh = LossShared<S>;
   extern __shared__ __align__(128) uint8_t dyn[];
   uint4* slots = reinterpret_cast<uint4*>(dyn);
-  LossShared& sh = *reinterpret_cast<LossShared*>(dyn + kSlots * kChunkVecs * 16);
+  Sh& sh = *reinterpret_cast<Sh*>(dyn + S::kRingBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = cluster_rank(), size = cluster_size();
   if (tid == 0) {
-    for (int i = 0; i < kSlots; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], kLossWarps);
-    for (int i = 0; i < 2; ++i)
-      mbar_init(&sh.teacher_full[i], 1), mbar_init(&sh.teacher_empty[i], kLossWarps), mbar_init(&sh.peers[i], 1);
+    for (int i = 0; i < S::kSlots; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], S::kWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.part_full[i], S::kWarps), mbar_init(&sh.part_empty[i], 1);
+      mbar_init(&sh.grad_full[i], 1), mbar_init(&sh.grad_empty[i], S::kWarps);
+      mbar_init(&sh.teacher_full[i], 1), mbar_init(&sh.teacher_empty[i], PASS == kForward ? 1 : S::kWarps);
+      mbar_init(&sh.peers[i], 1);
+    }
     sh.gave_up = 0;
     fence_barrier_init();
   }
@@ -394,313 +787,39 @@ __global__ void __launch_bounds__(kCtaThreads, 1) loss_rows_kernel(const LossArg
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int n = A.batch * A.length, n_active = A.hdr->n_active;
   const int first = blockIdx.x / size, step = gridDim.x / size;
-
-  if (warp == kLossWarps) {
-    if (lane == 0) {
-      Ring r;
-      int filled = 0;  // slots in use at the start are none
-      int row = first < n_active ? A.list[first] : 0;
-      for (int i = first; i < n_active; i += step) {
-        const RowPart<T> p(A, row, rank, size);
-        if (i + step < n_active) row = A.list[i + step];
-        const int kept = min(p.chunks, kSlots);
-        const int total = PASS == kFused ? 2 * p.chunks - kept : p.chunks;
-        for (int c = 0; c < total; ++c) {
-          const int at = c < p.chunks ? c : c - p.chunks;
-          if (filled == kSlots)
-            wait_or_mark(&sh.empty[r.slot], r.phase ^ 1, sh);
-          else
-            ++filled;
-          if (*(volatile int*)&sh.gave_up) break;
-          const int nv = min(kChunkVecs, p.nv - at * kChunkVecs);
-          mbar_arrive_expect_tx(&sh.full[r.slot], nv * 16);
-          bulk_copy_g2s(slots + r.slot * kChunkVecs, p.body() + at * kChunkVecs, nv * 16, &sh.full[r.slot]);
-          r.next();
-        }
-        if (*(volatile int*)&sh.gave_up) break;
-      }
-      if (*(volatile int*)&sh.gave_up) {
-        // Copies still in flight end before the CTA's shared memory goes.
-        for (int i = 0; i < kSlots; ++i)
-          if (i < r.slot || filled == kSlots) mbar_wait_bounded(&sh.full[i], i < r.slot ? r.phase : r.phase ^ 1);
-      }
-    }
-    __syncwarp();
-  } else if (warp == kLossWarps + 1) {
-    if (KIND == kDistill) {
-      // The teacher's warp: q and its sums, a row or two ahead of the consumers.
-      int it = 0;
-      for (int i = first; i < n_active; i += step, ++it) {
-        const RowPart<T> p(A, A.list[i], rank, size);
-        TeacherRow& o = sh.teacher[it & 1];
-        if (it >= 2) wait_or_mark(&sh.teacher_empty[it & 1], ((it >> 1) & 1) ^ 1, sh);
-        constexpr int kPer = PKV_MAX_TOP / 32;
-        float v[kPer], x[kPer];
-        float top = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const int j = lane + 32 * e;
-          v[e] = -INFINITY, x[e] = 0.f;
-          if (j < A.k) {
-            int64_t id;
-            v[e] = teacher_logit(A, p.b, p.t, j, id);
-            const bool column = id >= 0 && id < A.vocab;
-            if (PASS != kBackward && v[e] != -INFINITY) x[e] = column ? as_float(p.x[id]) : NAN;
-            o.id[j] = column ? (int32_t)id : -1;
-            top = fmaxf(top, v[e]);
-          }
-        }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        // The norm in 64 bits: log q would lose digits to a rounded one.
-        double norm = 0.0;
-        if (A.tlse.p) {
-          norm = (double)A.tlse.at(p.b, p.t);
-        } else if (top > -INFINITY) {
-          double sum = 0.0;
-#pragma unroll
-          for (int e = 0; e < kPer; ++e)
-            if (v[e] != -INFINITY) sum += (double)expf((float)(((double)v[e] - (double)top) * A.inv_td));
-          norm = (double)top * A.inv_td + log(warp_sum_d(sum));
-        }
-        double qs = 0.0, qx = 0.0, ql = 0.0;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const int j = lane + 32 * e;
-          float q = 0.f;
-          if (v[e] != -INFINITY) {
-            const double lq = (double)v[e] * A.inv_td - norm;
-            q = expf((float)lq);
-            qs += (double)q;
-            if (q != 0.f || x[e] != x[e]) {
-              qx += (double)q * (double)x[e];
-              ql += (double)q * lq;
-            }
-          }
-          if (j < A.k) o.q[j] = q;
-        }
-        qs = warp_sum_d(qs), qx = warp_sum_d(qx), ql = warp_sum_d(ql);
-        if (lane == 0) o.norm = norm, o.q_sum = qs, o.qx = qx, o.qlogq = ql;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.teacher_full[it & 1]);
-      }
-    }
+  if (warp == S::kCopyWarp) {
+    if (lane == 0) copy_rows<T, PASS, S>(A, sh, slots, rank, size, first, step, n_active);
+  } else if (warp == S::kTeacherWarp) {
+    if (KIND == kDistill) teacher_rows<T, PASS, S>(A, sh, rank, size, first, step, n_active, lane);
+  } else if (warp == S::kTermsWarp) {
+    term_rows<T, KIND, ENT, PASS, S>(A, sh, rank, size, first, step, n_active, n, lane);
   } else {
-    const float up = A.upstream ? *A.upstream : 1.f;
-    const Scale2 ks = A.ks;
-    Ring r;
-    int it = 0;  // scored rows so far
-    int row_next = first < n ? A.list[first] : 0;
-    for (int i = first; i < n; i += step) {
-      const RowPart<T> p(A, row_next, rank, size);
-      if (i + step < n) row_next = A.list[i + step];
-      const int row = p.row, b = p.b, t = p.t;
-      // The columns outside the body are the first CTA's.
-      const int edge = rank == 0 ? A.vocab - p.nvec * VE : 0;
-      const int edge_col = tid < p.head ? tid : tid + p.nvec * VE;
-      const int kept = min(p.chunks, kSlots);
-      RowGrad o{0.f, 0.f, 0.f, 0.f, -1, i >= n_active};
-      float wt = 0.f;
-      const bool scored = i < n_active;
-      if (!scored) {
-        if (PASS != kBackward && tid == 0 && rank == 0) {
-          if (A.logprobs) A.logprobs[row] = 0.f;
-          if (A.kl_out) A.kl_out[row] = 0.f;
-          if (ENT && A.entropy) A.entropy[row] = 0.f;
-          A.row_val[row] = 0.0;
-        }
-        if (PASS == kForward) continue;
-      } else if (PASS == kBackward) {
-        const float4 rec = A.rec[row];
-        const float f = up * (A.seq_g ? A.seq_g[b] : 1.f);
-        o = RowGrad{rec.x, rec.y * f, rec.z * f, rec.w * f, -1, false};
-        if (KIND == kDistill) {
-          o.b = o.h = 0.f;
-          wt = rec.z * f;
-          o.zero = f == 0.f;
-          wait_or_mark(&sh.teacher_full[it & 1], (it >> 1) & 1, sh);
-        } else {
-          const int64_t tok = A.tokens.at(b, t);
-          o.tok = tok >= 0 && tok < A.vocab ? (int)tok : -1;
-          o.zero = o.a == 0.f && o.b == 0.f && o.h == 0.f;
-        }
-      } else {
-        // What the row's terms need is loaded now and used after the sums.
-        int64_t tok = 0;
-        float xt = 0.f;
-        if (KIND != kDistill) {
-          tok = A.tokens.at(b, t);
-          xt = tok >= 0 && tok < A.vocab ? as_float(p.x[tok]) : NAN;
-        }
-        RowSum a{-INFINITY, 0.f, 0.f};
-        for (int c = 0; c < p.chunks; ++c) {
-          wait_or_mark(&sh.full[r.slot], r.phase, sh);
-          const uint4* in = slots + r.slot * kChunkVecs;
-          const int nv = min(kChunkVecs, p.nv - c * kChunkVecs);
-          if (nv == kChunkVecs) {
-            float f[2 * VE];
-            float (&lo)[VE] = *reinterpret_cast<float (*)[VE]>(f);
-            float (&hi)[VE] = *reinterpret_cast<float (*)[VE]>(f + VE);
-            unpack<T>(in[tid], lo);
-            unpack<T>(in[tid + kLossThreads], hi);
-            fold<ENT>(a, f, ks);
-          } else {
-            for (int j = tid; j < nv; j += kLossThreads) {
-              float f[VE];
-              unpack<T>(in[j], f);
-              fold<ENT>(a, f, ks);
-            }
-          }
-          if (PASS == kForward || c < p.chunks - kept) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.empty[r.slot]);
-          }
-          r.next();
-        }
-        if (PASS == kFused) r.back(kept);
-        if (tid < edge) {
-          const float f[1] = {as_float(p.x[edge_col])};
-          fold<ENT>(a, f, ks);
-        }
-        // The CTA's sum: warps, then (every warp for itself) the warps' sums, then the cluster's.
-        a = warp_merge(a, 32, ks);
-        if (lane == 0) sh.part[it & 1][warp] = a;
-        consumers_sync();
-        a = warp_merge(sh.part[it & 1][lane & (kLossWarps - 1)], kLossWarps, ks);
-        if (size > 1) {
-          if (tid == 0) {
-            mbar_arrive_expect_tx(&sh.peers[it & 1], 16 * size);
-            for (int q = 0; q < size; ++q)
-              send_peer(&sh.peer[it & 1][rank], &sh.peers[it & 1], q, make_float4(a.m, a.s, a.w, 0.f));
-          }
-          wait_or_mark<true>(&sh.peers[it & 1], (it >> 1) & 1, sh);
-          const float4 v = sh.peer[it & 1][lane & (size - 1)];
-          a = warp_merge(RowSum{v.x, v.y, v.z}, size, ks);
-        }
-        const bool write = tid == 0 && rank == 0;
-        if (KIND == kPolicy) {
-          o = policy_tail<ENT>(A, row, b, t, a, xt, tok, write);
-        } else if (KIND == kPreference) {
-          const bool known = tok >= 0 && tok < A.vocab;
-          o = RowGrad{a.m, -1.f / a.s, 0.f, 1.f, 0, false};
-          if (write) A.row_val[row] = known ? (((double)xt - (double)a.m) * A.kd - log2_of(a.s)) * kLn2d : (double)NAN;
-        } else {
-          wait_or_mark(&sh.teacher_full[it & 1], (it >> 1) & 1, sh);
-          const TeacherRow& q = sh.teacher[it & 1];
-          // sum q (log q - log p), log p = ((x - m) k - log2 s) ln 2
-          const double w = (double)A.seq_w[b], tt = (double)A.temperature;
-          const double l = tt * tt * (q.qlogq - ((q.qx - q.q_sum * (double)a.m) * A.kd - q.q_sum * log2_of(a.s)) * kLn2d);
-          wt = (float)(w * tt);
-          o = RowGrad{a.m, l == l ? wt * (float)q.q_sum / a.s : NAN, 0.f, 0.f, -1, false};
-          if (write) {
-            A.kl_out[row] = (float)l;
-            A.row_val[row] = w * l;
-          }
-        }
-        if (PASS == kForward) {
-          if (write && A.rec)
-            A.rec[row] = KIND == kDistill ? make_float4(o.m, o.a, wt, 0.f) : make_float4(o.m, o.a, o.b, o.h);
-          if (KIND == kDistill) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.teacher_empty[it & 1]);
-          }
-          ++it;
-          continue;
-        }
-      }
-      T* g = (T*)A.g + b * A.gb + t * A.gr;
-      uint4* out = reinterpret_cast<uint4*>(g + p.head) + p.v0;
-      const bool vec = ((uintptr_t)out & 15) == 0;
-      auto store = [&](int j, const float (&f)[VE]) {
-        if (vec) {
-          __stcs(out + j, pack<T>(f));
-        } else {
-#pragma unroll
-          for (int q = 0; q < VE; ++q) put(g + p.head + (p.v0 + j) * VE + q, f[q]);
-        }
-      };
-      if (!scored) {
-        const float f[VE] = {};
-        for (int j = tid; j < p.nv; j += kLossThreads) store(j, f);
-      } else {
-        const int hot_vec = o.tok < 0 ? -1 : (o.tok - p.head >= 0 ? (o.tok - p.head) / VE - p.v0 : -1);
-        for (int c = 0; c < p.chunks; ++c) {
-          const int at = PASS == kBackward ? c : (c < kept ? p.chunks - kept + c : c - kept);
-          wait_or_mark(&sh.full[r.slot], r.phase, sh);
-          const uint4* in = slots + r.slot * kChunkVecs;
-          const int nv = min(kChunkVecs, p.nv - at * kChunkVecs);
-          for (int j = tid; j < nv; j += kLossThreads) {
-            float f[VE] = {};
-            if (!o.zero) {
-              unpack<T>(in[j], f);
-              grad_vec<ENT, T>(f, o, ks);
-              if (at * kChunkVecs + j == hot_vec) {
-                const int hot = o.tok - p.head - (p.v0 + at * kChunkVecs + j) * VE;
-#pragma unroll
-                for (int q = 0; q < VE; ++q)
-                  if (q == hot) f[q] += o.h;
-              }
-            }
-            store(at * kChunkVecs + j, f);
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.empty[r.slot]);
-          r.next();
-        }
-      }
-      if (tid < edge) {
-        float v = o.zero ? 0.f : grad_of<ENT>(as_float(p.x[edge_col]), o, ks);
-        if (!o.zero && edge_col == o.tok) v += o.h;
-        put(g + edge_col, v);
-      }
-      if (KIND == kDistill && scored) {
-        // The list's columns, over what their vectors wrote.  An id that comes twice is written once, with both shares.
-        consumers_sync();
-        const TeacherRow& q = sh.teacher[it & 1];
-        const int c0 = p.head + p.v0 * VE, c1 = c0 + p.nv * VE;
-        if (tid < A.k && !o.zero) {
-          const int id = q.id[tid];
-          if (id >= 0 && ((id >= c0 && id < c1) || (rank == 0 && (id < p.head || id >= p.head + p.nvec * VE)))) {
-            float sum = 0.f;
-            int firstly = tid;
-            for (int f = 0; f < A.k; ++f) {
-              if (q.id[f] != id) continue;
-              firstly = min(firstly, f);
-              sum += q.q[f];
-            }
-            if (firstly == tid) put(g + id, grad_of<false>(as_float(p.x[id]), o, ks) - wt * sum);
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.teacher_empty[it & 1]);
-      }
-      if (scored) ++it;
+    column_rows<T, KIND, ENT, PASS, S>(A, sh, slots, rank, size, first, step, n_active, n, tid);
+  }
+  __syncwarp();
+  __syncthreads();
+  if (size > 1) cluster_sync_all();  // no CTA leaves while its peers may still send to it
+  if (tid == 0 && *(volatile int*)&sh.gave_up) atomicExch(&A.hdr->error, 1);
+  if (PASS != kBackward && KIND != kPreference) {
+    // The last CTA adds the rows' losses, always in the same order.
+    if (tid == 0) {
+      __threadfence();
+      sh.last = atomicAdd(&A.hdr->ticket, 1) == (int)gridDim.x - 1;
     }
-    if (tid == 0 && *(volatile int*)&sh.gave_up) atomicExch(&A.hdr->error, 1);
-    if (PASS != kBackward && KIND != kPreference) {
-      // The last CTA adds the rows' losses, always in the same order.
-      consumers_sync();
+    __syncthreads();
+    if (sh.last) {
+      __threadfence();
+      double sum = 0.0;
+      for (int i = tid; i < n_active; i += S::kThreads) sum += __ldcg(A.row_val + A.list[i]);
+      sum = warp_sum_d(sum);
+      if (lane == 0) sh.sum[warp] = sum;
+      __syncthreads();
       if (tid == 0) {
-        __threadfence();
-        sh.last = atomicAdd(&A.hdr->ticket, 1) == (int)gridDim.x - 1;
-      }
-      consumers_sync();
-      if (sh.last) {
-        __threadfence();
-        double sum = 0.0;
-        for (int i = tid; i < n_active; i += kLossThreads) sum += __ldcg(A.row_val + A.list[i]);
-        sum = warp_sum_d(sum);
-        if (lane == 0) sh.sum[warp] = sum;
-        consumers_sync();
-        if (tid == 0) {
-          for (int i = 1; i < kLossWarps; ++i) sum += sh.sum[i];
-          *A.loss = __ldcg(&A.hdr->error) ? NAN : (float)sum;
-        }
+        for (int i = 1; i < S::kThreads / 32; ++i) sum += sh.sum[i];
+        *A.loss = __ldcg(&A.hdr->error) ? NAN : (float)sum;
       }
     }
   }
-  __syncwarp();
-  if (size > 1) cluster_sync_all();  // no CTA leaves while its peers may still send to it
 }
 
 // ---------------------------------------------------------------------------
@@ -796,9 +915,6 @@ Layout layout(int64_t batch, int64_t length) {
   return l;
 }
 
-constexpr int kDynBytes = kSlots * kChunkVecs * 16 + (int)sizeof(LossShared);
-static_assert(kDynBytes <= 232448, "a CTA's shared memory");
-
 int32_t sm_count(int* sms) {
   static int counts[64] = {};
   int dev = 0;
@@ -832,15 +948,18 @@ int32_t launch_after(K kernel, int grid, int threads, int cluster, int smem, con
   return cuda_status(what);
 }
 
-// CTAs that share a row: few rows are spread over the SMs by columns, as long as a CTA keeps at least a chunk.
-int row_cluster(int64_t rows, int64_t row_bytes, int sms) {
+// CTAs that share a row: few rows are spread over the SMs by columns, as long as a CTA keeps at least 16 KB.
+int row_cluster(int64_t rows, int64_t row_bytes, int ctas) {
   int c = 1;
-  while (c < kMaxCluster && rows * (2 * c) <= sms && row_bytes / (2 * c) >= kChunkVecs * 16) c *= 2;
+  while (c < kMaxCluster && rows * (2 * c) <= ctas && row_bytes / (2 * c) >= 16384) c *= 2;
   return c;
 }
 
 template <typename T, int KIND, bool ENT, int PASS>
 int32_t launch_typed(const LossArgs& a, cudaStream_t st) {
+  using S = ShapeOf<T, PASS>;
+  constexpr int kBytes = S::kRingBytes + (int)sizeof(LossShared<S>);
+  static_assert((kBytes + 1024) * S::kCtas <= 233472, "an SM's shared memory");
   int sms = 0;
   const int32_t e = sm_count(&sms);
   if (e != PKV_OK) return e;
@@ -849,14 +968,14 @@ int32_t launch_typed(const LossArgs& a, cudaStream_t st) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 64 || !ready[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDynBytes) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess)
       return cuda_status("loss rows shared memory");
     if (dev < 64) ready[dev] = true;
   }
   const int64_t rows = (int64_t)a.batch * a.length;
-  const int c = row_cluster(rows, (int64_t)a.vocab * sizeof(T), sms);
-  const int grid = (int)std::min<int64_t>(rows, sms / c) * c;
-  return launch_after(kernel, grid, kCtaThreads, c, kDynBytes, a, st, "loss rows launch");
+  const int c = row_cluster(rows, (int64_t)a.vocab * sizeof(T), sms * S::kCtas);
+  const int grid = (int)std::min<int64_t>(rows, sms * S::kCtas / c) * c;
+  return launch_after(kernel, grid, S::kThreads, c, kBytes, a, st, "loss rows launch");
 }
 
 template <int KIND, bool ENT, int PASS>
@@ -876,8 +995,7 @@ LossArgs row_args(const pkv_loss_rows* r, const Layout& l, uint8_t* ws) {
   a.seq_w = reinterpret_cast<const float*>(ws + l.seq_w);
   a.row_val = reinterpret_cast<double*>(ws + l.row_val);
   a.rec = reinterpret_cast<float4*>(ws + l.rec);
-  a.kd = kLog2ed / (double)r->temperature;
-  a.ks.hi = (float)a.kd, a.ks.lo = (float)(a.kd - (double)a.ks.hi);
+  a.ks = scale_for(r->temperature, &a.kd);
   a.inv_t = (float)(1.0 / (double)r->temperature), a.temperature = r->temperature;
   a.inv_td = 1.0 / (double)r->temperature;
   return a;

@@ -138,14 +138,15 @@ __global__ void __launch_bounds__(kTopThreads) top_logits_kernel(const TopArgs A
     for (int j = tid; j < sp.nvec; j += kTopThreads) {
       float v[VE];
       unpack<T>(body[j], v);
-      fold<false>(r, v, A.ks);
+      const uint4 raw[1] = {body[j]};
+      fold_vecs<false, T>(r, raw, A.ks);
 #pragma unroll
       for (int q = 0; q < VE; ++q) top = max(top, ordered(v[q]));
     }
     const int edge = A.vocab - sp.nvec * VE;
     if (tid < edge) {
       const float v[1] = {as_float(x[tid < sp.head ? tid : tid + sp.nvec * VE])};
-      fold<false>(r, v, A.ks);
+      fold<false>(r, v, v[0], A.ks);
       top = max(top, ordered(v[0]));
     }
     // The log-sum-exp, and the range of the threads' maxima.
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(kTopThreads) top_logits_kernel(const TopArgs A
         A.tokens[(int64_t)row * A.k + rank] = (int64_t)(0xffffffffu - (uint32_t)key);
       }
     }
-    if (tid == 0) A.lse[row] = (float)(((double)r.m * A.kd + log2_of(r.s)) * kLn2d);
+    if (tid == 0) A.lse[row] = (float)((log2_of(r.s) + (far_out(center(r.m, A.ks)) ? (double)r.m * A.kd : -(double)center(r.m, A.ks))) * kLn2d);
     __syncthreads();
   }
 }
@@ -250,8 +251,7 @@ extern "C" int32_t pkv_top_logits(const pkv_loss_rows* r, int32_t k, float* valu
   }
   TopArgs a{r->logits, r->batch_stride, r->row_stride, r->batch, r->length, r->vocab, k, {0.f, 0.f}, 0.0,
             values_out, tokens_out, lse_out};
-  a.kd = kLog2ed / (double)r->temperature;
-  a.ks.hi = (float)a.kd, a.ks.lo = (float)(a.kd - (double)a.ks.hi);
+  a.ks = scale_for(r->temperature, &a.kd);
   const int grid = (int)std::min<int64_t>(n, 4ll * sms);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (r->dtype == PKV_F32)
