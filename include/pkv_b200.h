@@ -775,7 +775,7 @@ int32_t pkv_distillation_loss_backward(const pkv_loss_rows* rows, const pkv_dist
 /* The k largest logits of each row, largest first, equal ones by their column
  * (NaN counts as the largest, -0 as 0): values float and columns int64
  * [batch][length][k], lse_out float [batch][length] the log-sum-exp of logits
- * / temperature.  1 <= k <= min(vocab, PKV_MAX_TOP); the mask and grad of
+ * / temperature (NaN for a row with NaN or +inf).  1 <= k <= min(vocab, PKV_MAX_TOP); the mask and grad of
  * `rows` are not used. */
 int32_t pkv_top_logits(const pkv_loss_rows* rows, int32_t k, float* values_out, int64_t* tokens_out, float* lse_out,
                        void* stream);

@@ -9,14 +9,20 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <string>
 #include <type_traits>
 
 #include "pkv_b200.h"
+#include "pkv_device.cuh"
+#include "pkv_error.h"
 
 namespace pkv {
 
 // PKV_OK, or the status and error message for rows a call named `who` cannot take.
 int32_t check_vocab_rows(const pkv_loss_rows* r, const char* who);
+
+namespace {
 
 constexpr double kLn2d = 0.6931471805599453;
 constexpr double kLog2ed = 1.4426950408889634;
@@ -246,14 +252,192 @@ __device__ __forceinline__ void fold(RowSum& a, const float (&x)[N], float top, 
   }
 }
 
-// N vectors of a row's body.
+// N vectors of a row's body; their largest column.
 template <bool ENT, typename T, int N>
-__device__ __forceinline__ void fold_vecs(RowSum& a, const uint4 (&v)[N], Scale2 k) {
+__device__ __forceinline__ float fold_vecs(RowSum& a, const uint4 (&v)[N], Scale2 k) {
   constexpr int VE = 16 / sizeof(T);
   float f[N * VE];
 #pragma unroll
   for (int i = 0; i < N; ++i) unpack<T>(v[i], *reinterpret_cast<float (*)[VE]>(f + i * VE));
-  fold<ENT>(a, f, top_of<T>(v), k);
+  const float top = top_of<T>(v);
+  fold<ENT>(a, f, top, k);
+  return top;
 }
 
+// ---------------------------------------------------------------------------
+// Rows through a shared-memory ring, by a CTA or a cluster.
+
+constexpr int kMaxCluster = 8;
+
+// Shape of a launch: threads that work on the columns, 16-byte vectors of a ring slot each takes, ring slots, CTAs an SM.
+template <int THREADS, int VECS, int SLOTS, int CTAS>
+struct Shape {
+  static constexpr int kGroup = THREADS, kVecs = VECS, kSlots = SLOTS, kCtas = CTAS;
+  static constexpr int kChunk = VECS * THREADS;  // vectors of a slot
+  static constexpr int kWarps = THREADS / 32;
+  static constexpr int kCopyWarp = kWarps, kTeacherWarp = kWarps + 1, kTermsWarp = kWarps + 2;
+  static constexpr int kThreads = THREADS + 96;
+  static constexpr int kRingBytes = SLOTS * kChunk * 16;
+};
+// mbar_try_wait that also sees what other CTAs of the cluster sent.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Waits are bounded.  One that gives up marks the CTA: every later wait of it passes at once, so that all roles run
+// to their ends (their barriers included) and the loss is made NaN.
+template <bool CLUSTER = false, typename Sh>
+__device__ __forceinline__ void wait_or_mark(uint64_t* bar, uint32_t parity, Sh& sh) {
+  auto passed = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+  if (passed()) return;
+  const long long start = clock64();
+  while (!passed()) {
+    if (*(volatile int*)&sh.gave_up) return;
+    if (clock64() - start > kWaitLimitCycles) {
+      *(volatile int*)&sh.gave_up = 1;
+      return;
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The same shared-memory object of CTA `rank` of the cluster.
+template <typename T>
+__device__ __forceinline__ const T* cluster_peer(const T* p, uint32_t rank) {
+  uint64_t q;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(q) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
+  return reinterpret_cast<const T*>(q);
+}
+
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+
+__device__ __forceinline__ RowSum warp_merge(RowSum a, int width, Scale2 k) {
+  for (int off = width / 2; off > 0; off >>= 1) {
+    RowSum b;
+    b.m = __shfl_xor_sync(0xffffffffu, a.m, off);
+    b.s = __shfl_xor_sync(0xffffffffu, a.s, off);
+    b.w = __shfl_xor_sync(0xffffffffu, a.w, off);
+    sum_merge(a, b, k);
+  }
+  return a;
+}
+
+// A row's place in memory and the part of it this CTA of its cluster has.
+template <typename T, int CHUNK>
+struct RowPart {
+  int row, b, t;
+  const T* x;
+  int head, nvec;      // the row's aligned body, in vectors
+  int v0, nv, chunks;  // this CTA's vectors
+  template <typename Args>
+  __device__ RowPart(const Args& A, int row_, int rank, int size) {
+    row = row_;
+    b = row / A.length, t = row - b * A.length;
+    x = (const T*)A.x + b * A.xb + t * A.xr;
+    const RowSplit<T> sp(x, A.vocab);
+    head = sp.head, nvec = sp.nvec;
+    const int per = (nvec + size - 1) / size;
+    v0 = min(nvec, rank * per);
+    nv = min(nvec, v0 + per) - v0;
+    chunks = (nv + CHUNK - 1) / CHUNK;
+  }
+  __device__ const uint4* body() const { return reinterpret_cast<const uint4*>(x + head) + v0; }
+};
+
+// A place in the ring.  Slots are filled, looked at and freed strictly in turn: a row's chunks 0 .. n-1, and, where
+// the row is needed twice, the last min(n, SLOTS) of them stay in their slots for the second time, which takes them
+// first; then, behind those, the others again (from L2).
+template <int SLOTS>
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == SLOTS) slot = 0, phase ^= 1;
+  }
+  __device__ __forceinline__ void back(int n) {  // n <= SLOTS
+    slot -= n;
+    if (slot < 0) slot += SLOTS, phase ^= 1;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Host.
+
+inline int32_t fail(int32_t status, const std::string& msg) {
+  pkv_set_error(msg);
+  return status;
+}
+
+inline int32_t cuda_status(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return PKV_OK;
+  return fail(PKV_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+inline int32_t sm_count(int* sms) {
+  static int counts[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status("device query");
+  if (dev < 64 && counts[dev]) {
+    *sms = counts[dev];
+    return PKV_OK;
+  }
+  if (cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return cuda_status("device query");
+  if (dev < 64) counts[dev] = *sms;
+  return PKV_OK;
+}
+
+// Launch `kernel` behind the kernel before it on the stream (it waits for that one itself).
+template <typename K, typename Args>
+int32_t launch_after(K kernel, int grid, int threads, int cluster, int smem, const Args& a, cudaStream_t st,
+                     const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kernel, a);
+  return cuda_status(what);
+}
+
+// CTAs that share a row: few rows are spread over the SMs by columns, as long as a CTA keeps at least 16 KB.
+inline int row_cluster(int64_t rows, int64_t row_bytes, int ctas) {
+  int c = 1;
+  while (c < kMaxCluster && rows * (2 * c) <= ctas && row_bytes / (2 * c) >= 16384) c *= 2;
+  return c;
+}
+
+}  // namespace
 }  // namespace pkv

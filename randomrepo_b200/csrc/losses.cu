@@ -30,7 +30,6 @@
 namespace pkv {
 namespace {
 
-constexpr int kMaxCluster = 8;
 constexpr float kLn2 = 0.6931471805599453f;
 
 enum Kind { kPolicy = 0, kPreference = 1, kDistill = 2 };
@@ -260,16 +259,6 @@ struct TeacherRow {
   float q[PKV_MAX_TOP];
 };
 
-// Shape of a launch: threads that work on the columns, 16-byte vectors of a ring slot each takes, ring slots, CTAs an SM.
-template <int THREADS, int VECS, int SLOTS, int CTAS>
-struct Shape {
-  static constexpr int kGroup = THREADS, kVecs = VECS, kSlots = SLOTS, kCtas = CTAS;
-  static constexpr int kChunk = VECS * THREADS;  // vectors of a slot
-  static constexpr int kWarps = THREADS / 32;
-  static constexpr int kCopyWarp = kWarps, kTeacherWarp = kWarps + 1, kTermsWarp = kWarps + 2;
-  static constexpr int kThreads = THREADS + 96;
-  static constexpr int kRingBytes = SLOTS * kChunk * 16;
-};
 // Measured on rows of 151 936 columns.  Sums or gradient alone: four CTAs of 128 threads that take 8 vectors at a time
 // (16-bit sums of 4 096 rows 227 us; 256 threads x 2 CTAs 238, 512 threads x 4 vectors x 1 CTA 275).  Both in one
 // launch: two CTAs an SM hide each other's turns between the passes, and a larger chunk its waits (499 us; one CTA of
@@ -292,49 +281,6 @@ struct alignas(128) LossShared {
   TeacherRow teacher[2];
 };
 
-// mbar_try_wait that also sees what other CTAs of the cluster sent.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// Waits are bounded.  One that gives up marks the CTA: every later wait of it passes at once, so that all roles run
-// to their ends (their barriers included) and the loss is made NaN.
-template <bool CLUSTER = false, typename Sh>
-__device__ __forceinline__ void wait_or_mark(uint64_t* bar, uint32_t parity, Sh& sh) {
-  auto passed = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
-  if (passed()) return;
-  const long long start = clock64();
-  while (!passed()) {
-    if (*(volatile int*)&sh.gave_up) return;
-    if (clock64() - start > kWaitLimitCycles) {
-      *(volatile int*)&sh.gave_up = 1;
-      return;
-    }
-  }
-}
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // 16 bytes into the same shared-memory place of CTA `rank` of the cluster, counted on its barrier.
 __device__ __forceinline__ void send_peer(void* dst, uint64_t* bar, uint32_t rank, float4 v) {
   uint32_t d, b;
@@ -344,60 +290,6 @@ __device__ __forceinline__ void send_peer(void* dst, uint64_t* bar, uint32_t ran
                "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(b)
                : "memory");
 }
-
-__device__ __forceinline__ double warp_sum_d(double v) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  return v;
-}
-
-__device__ __forceinline__ RowSum warp_merge(RowSum a, int width, Scale2 k) {
-  for (int off = width / 2; off > 0; off >>= 1) {
-    RowSum b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, off);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, off);
-    b.w = __shfl_xor_sync(0xffffffffu, a.w, off);
-    sum_merge(a, b, k);
-  }
-  return a;
-}
-
-// A row's place in memory and the part of it this CTA of its cluster has.
-template <typename T, int CHUNK>
-struct RowPart {
-  int row, b, t;
-  const T* x;
-  int head, nvec;      // the row's aligned body, in vectors
-  int v0, nv, chunks;  // this CTA's vectors
-  __device__ RowPart(const LossArgs& A, int row_, int rank, int size) {
-    row = row_;
-    b = row / A.length, t = row - b * A.length;
-    x = (const T*)A.x + b * A.xb + t * A.xr;
-    const RowSplit<T> sp(x, A.vocab);
-    head = sp.head, nvec = sp.nvec;
-    const int per = (nvec + size - 1) / size;
-    v0 = min(nvec, rank * per);
-    nv = min(nvec, v0 + per) - v0;
-    chunks = (nv + CHUNK - 1) / CHUNK;
-  }
-  __device__ const uint4* body() const { return reinterpret_cast<const uint4*>(x + head) + v0; }
-};
-
-// A place in the ring.  Slots are filled, looked at and freed strictly in turn: a row's chunks 0 .. n-1 for its sums,
-// the last min(n, kSlots) of which stay in their slots for its gradient, which takes them first; then, behind those,
-// the others again (from L2).
-template <int SLOTS>
-struct Ring {
-  int slot = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void next() {
-    if (++slot == SLOTS) slot = 0, phase ^= 1;
-  }
-  __device__ __forceinline__ void back(int n) {  // n <= SLOTS
-    slot -= n;
-    if (slot < 0) slot += SLOTS, phase ^= 1;
-  }
-};
 
 // The copying warp (one lane of it).
 template <typename T, int PASS, typename S, typename Sh>
@@ -883,17 +775,6 @@ __global__ void __launch_bounds__(1024) loss_pair_kernel(const PairArgs A) {
 // ---------------------------------------------------------------------------
 // Host.
 
-int32_t fail(int32_t status, const std::string& msg) {
-  pkv_set_error(msg);
-  return status;
-}
-
-int32_t cuda_status(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return PKV_OK;
-  return fail(PKV_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
-}
-
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Layout {
@@ -913,46 +794,6 @@ Layout layout(int64_t batch, int64_t length) {
   l.seq_g = at, at += up256(4 * batch);
   l.total = at;
   return l;
-}
-
-int32_t sm_count(int* sms) {
-  static int counts[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status("device query");
-  if (dev < 64 && counts[dev]) {
-    *sms = counts[dev];
-    return PKV_OK;
-  }
-  if (cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return cuda_status("device query");
-  if (dev < 64) counts[dev] = *sms;
-  return PKV_OK;
-}
-
-// Launch `kernel` behind the kernel before it on the stream (it waits for that one itself).
-template <typename K, typename Args>
-int32_t launch_after(K kernel, int grid, int threads, int cluster, int smem, const Args& a, cudaStream_t st,
-                     const char* what) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = cluster, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  cudaLaunchKernelEx(&cfg, kernel, a);
-  return cuda_status(what);
-}
-
-// CTAs that share a row: few rows are spread over the SMs by columns, as long as a CTA keeps at least 16 KB.
-int row_cluster(int64_t rows, int64_t row_bytes, int ctas) {
-  int c = 1;
-  while (c < kMaxCluster && rows * (2 * c) <= ctas && row_bytes / (2 * c) >= 16384) c *= 2;
-  return c;
 }
 
 template <typename T, int KIND, bool ENT, int PASS>

@@ -26,11 +26,11 @@ logits' device, never synchronise, and can be captured in a CUDA graph.  There i
 
 from __future__ import annotations
 
+import math
 import struct
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import lib
@@ -48,6 +48,7 @@ _ROWS = struct.Struct("@PqqPqqPqqiiiif")
 _POLICY = struct.Struct("@PqqPqqPqqPqqffffif")
 _PREFERENCE = struct.Struct("@PqqPffif")
 _DISTILLATION = struct.Struct("@PqqPqqiPqqif")
+_NONE = (0, 0, 0)
 
 
 class PolicyLoss(NamedTuple):
@@ -83,27 +84,31 @@ def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
         raise ValueError(f"{what}: logits must be float32, float16 or bfloat16")
     if logits.dim() not in (2, 3) or logits.shape[-1] < 1:
         raise ValueError(f"{what}: logits must be [batch, length, vocab] or [length, vocab]")
-    if logits.shape[-1] > 1 and logits.stride(-1) != 1:
+    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
         raise ValueError(f"{what}: logits must have a contiguous vocabulary dim")
+    if logits.requires_grad:
+        logits = logits.detach()
     return logits.unsqueeze(0) if logits.dim() == 2 else logits
 
 
 def _rows_like(t: torch.Tensor, x: torch.Tensor, dtype: torch.dtype, what: str, name: str,
                broadcast: bool = False) -> torch.Tensor:
     """A per-row input as [B, T] of ``dtype`` on the logits' device (``broadcast``: [B] or [B, 1] too)."""
-    b, n = x.shape[0], x.shape[1]
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{what}: {name} must be a tensor")
     if t.device != x.device:
         raise ValueError(f"{what}: {name} must be on the logits' device")
-    if broadcast and t.dim() == 1 and t.shape[0] == b and not (b == 1 and n != 1 and t.shape[0] == n):
-        t = t.unsqueeze(1)
-    if t.dim() == 1 and b == 1 and t.shape[0] == n:
-        t = t.unsqueeze(0)
-    if tuple(t.shape) != (b, n):
-        if not (broadcast and tuple(t.shape) == (b, 1)):
-            raise ValueError(f"{what}: {name} must have one value per logits row, got {tuple(t.shape)}")
-        t = t.expand(b, n)
+    rows = x.shape[:2]
+    if t.shape != rows:
+        b, n = rows
+        if broadcast and t.dim() == 1 and t.shape[0] == b and (b != 1 or n == 1):
+            t = t.unsqueeze(1)
+        elif t.dim() == 1 and b == 1 and t.shape[0] in ((n, 1) if broadcast else (n,)):
+            t = t.unsqueeze(0)
+        if t.shape != rows:
+            if not (broadcast and t.shape == (b, 1)):
+                raise ValueError(f"{what}: {name} must have one value per logits row, got {tuple(t.shape)}")
+            t = t.expand(b, n)
     if t.dtype != dtype:
         if dtype == torch.int64 and (t.is_floating_point() or t.dtype == torch.bool):
             raise ValueError(f"{what}: {name} must be integers")
@@ -117,12 +122,15 @@ def _mask(mask: torch.Tensor | None, x: torch.Tensor, what: str) -> torch.Tensor
         return None
     if isinstance(mask, torch.Tensor) and mask.dtype not in (torch.bool, torch.uint8):
         mask = mask != 0
-    m = _rows_like(mask, x, mask.dtype if isinstance(mask, torch.Tensor) else torch.bool, what, "mask")
-    return m.view(torch.uint8) if m.dtype == torch.bool else m
+    # (a byte each, read as such)
+    return _rows_like(mask, x, mask.dtype if isinstance(mask, torch.Tensor) else torch.bool, what, "mask")
 
 
 def _array(t: torch.Tensor | None) -> tuple[int, int, int]:
-    return (0, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+    if t is None:
+        return _NONE
+    sb, st = t.stride()[:2]
+    return t.data_ptr(), sb, st
 
 
 def _reduction(name: str, what: str) -> int:
@@ -151,43 +159,41 @@ def _grad_like(x: torch.Tensor) -> torch.Tensor:
 class _Call:
     """One loss call: the packed rows and terms, its tensors, and the workspace a backward pass reads."""
 
-    __slots__ = ("x", "mask", "temperature", "terms", "keep", "ws", "backward")
+    __slots__ = ("x", "mask", "temperature", "terms", "keep", "ws", "nbytes", "backward")
+
+    def __init__(self, x, mask, temperature, terms, keep, backward, what):
+        temperature = float(temperature)
+        if not 0.0 < temperature < math.inf:
+            raise ValueError(f"{what}: the temperature must be positive and finite")
+        self.x, self.mask, self.temperature = x, mask, temperature
+        self.terms, self.keep, self.backward = terms, keep, backward
+        b, n, _ = x.shape
+        self.nbytes = lib.pkv_loss_workspace_bytes(b, n)
+        if self.nbytes < 0:
+            raise ValueError(f"{what}: too many rows")
+        self.ws = torch.empty(self.nbytes, dtype=torch.uint8, device=x.device)
 
     def rows(self, grad: torch.Tensor | None) -> bytes:
         x = self.x
-        return _ROWS.pack(x.data_ptr(), x.stride(0), x.stride(1), *_array(grad), *_array(self.mask), x.shape[0],
-                          x.shape[1], x.shape[2], _DTYPES[x.dtype], self.temperature)
+        return _ROWS.pack(*_array(x), *_array(grad), *_array(self.mask), *x.shape, _DTYPES[x.dtype], self.temperature)
 
 
-def _call(x: torch.Tensor, mask, temperature: float, terms: bytes, keep: tuple, backward, what: str) -> _Call:
-    temperature = float(temperature)
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"{what}: the temperature must be positive and finite")
-    c = _Call()
-    c.x, c.mask, c.temperature, c.terms, c.keep, c.backward = x, mask, temperature, terms, keep, backward
-    nbytes = lib.pkv_loss_workspace_bytes(x.shape[0], x.shape[1])
-    if nbytes < 0:
-        raise ValueError(f"{what}: too many rows")
-    c.ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    return c
-
-
-def _stream(x: torch.Tensor) -> int:
-    return torch.cuda.current_stream(x.device).cuda_stream
+def _on_device(x: torch.Tensor, fn, *args) -> None:
+    """``fn(*args, stream)`` with the current stream of ``x``'s device, which is the current device meanwhile."""
+    index = x.device.index
+    if index == torch._C._cuda_getDevice():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if st:
+        _lib.raise_for_status(st)
 
 
 def _launch(fn, c: _Call, grad, outputs: tuple) -> None:
     """``fn(rows, terms, *outputs, workspace)`` on the logits' device and its current stream."""
-    x = c.x
-    args = (c.rows(grad), c.terms, *[t if t is None else t.data_ptr() for t in outputs], c.ws.data_ptr(),
-            c.ws.numel(), _stream(x))
-    if x.device.index == torch.cuda.current_device():
-        st = fn(*args)
-    else:
-        with torch.cuda.device(x.device):
-            st = fn(*args)
-    if st:
-        _lib.raise_for_status(st)
+    _on_device(c.x, fn, c.rows(grad), c.terms, *[None if t is None else t.data_ptr() for t in outputs],
+               c.ws.data_ptr(), c.nbytes)
 
 
 class _RowLoss(torch.autograd.Function):
@@ -195,16 +201,16 @@ class _RowLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, x, call, fn, outputs):
-        with torch.no_grad():
-            _launch(fn, call, None, outputs)
+        _launch(fn, call, None, outputs)
         ctx.call = call
         ctx.save_for_backward(logits, call.ws, *[t for t in call.keep if t is not None])
         ctx.mark_non_differentiable(*[t for t in outputs[1:] if t is not None])
         return outputs[:1] + tuple(t for t in outputs[1:] if t is not None)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_loss, *_):
+        if torch.is_grad_enabled():  # (create_graph=True)
+            raise RuntimeError("the vocabulary-row losses are differentiable once")
         logits = ctx.saved_tensors[0]  # (also checks that nothing was changed in place since)
         c = ctx.call
         grad = _grad_like(c.x)
@@ -215,7 +221,7 @@ class _RowLoss(torch.autograd.Function):
 
 def _run(fn, c: _Call, logits: torch.Tensor, outputs: tuple):
     """The outputs of a differentiable call."""
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         got = iter(_RowLoss.apply(logits, c.x, c, fn, outputs))
         return tuple(None if t is None else next(got) for t in outputs)
     _launch(fn, c, None, outputs)
@@ -231,7 +237,7 @@ def _run_with_grad(fn, c: _Call, logits: torch.Tensor, outputs: tuple) -> torch.
 def _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef, entropy_coef,
             temperature, reduction, scale):
     what = "policy_loss"
-    x = _logits(logits.detach() if isinstance(logits, torch.Tensor) else logits, what)
+    x = _logits(logits, what)
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError(f"{what}: clip_low and clip_high must be >= 0")
     tok = _rows_like(tokens, x, torch.int64, what, "tokens")
@@ -241,11 +247,12 @@ def _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_l
     m = _mask(mask, x, what)
     terms = _POLICY.pack(*_array(tok), *_array(adv), *_array(old), *_array(ref), clip_low, clip_high, kl_coef,
                          entropy_coef, _reduction(reduction, what), scale)
-    c = _call(x, m, temperature, terms, (tok, adv, old, ref, m), lib.pkv_policy_loss_backward, what)
+    c = _Call(x, m, temperature, terms, (tok, adv, old, ref, m), lib.pkv_policy_loss_backward, what)
     shape = logits.shape[:-1]
-    new = lambda: torch.empty(shape, dtype=torch.float32, device=x.device)  # noqa: E731
-    outputs = (torch.empty((), dtype=torch.float32, device=x.device), new(), None if ref is None else new(),
-               new() if entropy_coef else None)
+    dev = x.device
+    outputs = (torch.empty((), dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.float32, device=dev),
+               None if ref is None else torch.empty(shape, dtype=torch.float32, device=dev),
+               torch.empty(shape, dtype=torch.float32, device=dev) if entropy_coef else None)
     return c, outputs
 
 
@@ -283,7 +290,7 @@ def policy_loss_and_grad(logits: torch.Tensor, tokens: torch.Tensor, advantages:
 
 def _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, length_normalised, scale):
     what = "preference_loss"
-    x = _logits(logits.detach() if isinstance(logits, torch.Tensor) else logits, what)
+    x = _logits(logits, what)
     if logits.dim() != 3 or x.shape[0] % 2:
         raise ValueError(f"{what}: logits must be [2 * pairs, length, vocab], the chosen answers first")
     if not 0.0 <= label_smoothing <= 1.0:
@@ -297,7 +304,7 @@ def _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, lengt
         ref = ref.to(torch.float32).contiguous()
     terms = _PREFERENCE.pack(*_array(tok), 0 if ref is None else ref.data_ptr(), beta, label_smoothing,
                              int(bool(length_normalised)), scale)
-    c = _call(x, m, 1.0, terms, (tok, ref, m), lib.pkv_preference_loss_backward, what)
+    c = _Call(x, m, 1.0, terms, (tok, ref, m), lib.pkv_preference_loss_backward, what)
     new = lambda *s: torch.empty(s, dtype=torch.float32, device=x.device)  # noqa: E731
     return c, (new(), new(x.shape[0]), new(x.shape[0] // 2))
 
@@ -329,29 +336,34 @@ def preference_loss_and_grad(logits: torch.Tensor, tokens: torch.Tensor, mask: t
     return PreferenceLoss(*outputs), grad
 
 
-def _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale):
-    what = "distillation_loss"
-    x = _logits(logits.detach() if isinstance(logits, torch.Tensor) else logits, what)
-    lists = []
-    for t, name, dtype in ((teacher_ids, "teacher_ids", torch.int64), (teacher_logits, "teacher_logits", torch.float32)):
-        if not isinstance(t, torch.Tensor) or t.device != x.device:
-            raise ValueError(f"{what}: {name} must be on the logits' device")
-        if t.dim() != logits.dim() or t.shape[:-1] != logits.shape[:-1] or not 1 <= t.shape[-1] <= _MAX_TOP:
-            raise ValueError(f"{what}: {name} must be {list(logits.shape[:-1])} + [k], k from 1 to {_MAX_TOP}, got "
-                             f"{tuple(t.shape)}")
+def _teacher_list(t: torch.Tensor, logits: torch.Tensor, dtype: torch.dtype, what: str, name: str) -> torch.Tensor:
+    """A teacher's list as [B, T, k] of ``dtype`` with contiguous entries."""
+    if not isinstance(t, torch.Tensor) or t.device != logits.device:
+        raise ValueError(f"{what}: {name} must be on the logits' device")
+    shape = t.shape
+    if len(shape) != logits.dim() or shape[:-1] != logits.shape[:-1] or not 1 <= shape[-1] <= _MAX_TOP:
+        raise ValueError(f"{what}: {name} must be {list(logits.shape[:-1])} + [k], k from 1 to {_MAX_TOP}, got "
+                         f"{tuple(shape)}")
+    if t.dtype != dtype:
         if dtype == torch.int64 and (t.is_floating_point() or t.dtype == torch.bool):
             raise ValueError(f"{what}: {name} must be integers")
-        t = t.unsqueeze(0) if t.dim() == 2 else t
         t = t.to(dtype)
-        lists.append(t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous())
-    ids, tl = lists
+    if t.stride(-1) != 1 and shape[-1] > 1:
+        t = t.contiguous()
+    return t.unsqueeze(0) if len(shape) == 2 else t
+
+
+def _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale):
+    what = "distillation_loss"
+    x = _logits(logits, what)
+    ids = _teacher_list(teacher_ids, logits, torch.int64, what, "teacher_ids")
+    tl = _teacher_list(teacher_logits, logits, torch.float32, what, "teacher_logits")
     if ids.shape != tl.shape:
         raise ValueError(f"{what}: teacher_ids and teacher_logits must have the same shape")
     lse = None if teacher_lse is None else _rows_like(teacher_lse, x, torch.float32, what, "teacher_lse")
     m = _mask(mask, x, what)
-    terms = _DISTILLATION.pack(ids.data_ptr(), ids.stride(0), ids.stride(1), tl.data_ptr(), tl.stride(0), tl.stride(1),
-                               ids.shape[-1], *_array(lse), _reduction(reduction, what), scale)
-    c = _call(x, m, temperature, terms, (ids, tl, lse, m), lib.pkv_distillation_loss_backward, what)
+    terms = _DISTILLATION.pack(*_array(ids), *_array(tl), ids.shape[-1], *_array(lse), _reduction(reduction, what), scale)
+    c = _Call(x, m, temperature, terms, (ids, tl, lse, m), lib.pkv_distillation_loss_backward, what)
     return c, (torch.empty((), dtype=torch.float32, device=x.device),
                torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device))
 
@@ -388,22 +400,20 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, 
 def top_logits(logits: torch.Tensor, k: int, *,
                temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The k largest logits of each row (k <= 256): (values float32 [..., k], tokens int64 [..., k], the log-sum-exp
-    of logits / temperature [...]), largest first, equal ones by their column.  NaN counts as the largest value."""
+    of logits / temperature [...]), largest first, equal ones by their column.  NaN counts as the
+    largest value; a row with NaN or +inf has a NaN log-sum-exp."""
     what = "top_logits"
-    x = _logits(logits.detach() if isinstance(logits, torch.Tensor) else logits, what)
+    x = _logits(logits, what)
     k = int(k)
     if not 1 <= k <= min(_MAX_TOP, x.shape[-1]):
         raise ValueError(f"{what}: k must be from 1 to {min(_MAX_TOP, x.shape[-1])}")
     temperature = float(temperature)
-    if not 0.0 < temperature < float("inf"):
+    if not 0.0 < temperature < math.inf:
         raise ValueError(f"{what}: the temperature must be positive and finite")
     shape = logits.shape[:-1]
     values = torch.empty((*shape, k), dtype=torch.float32, device=x.device)
     tokens = torch.empty((*shape, k), dtype=torch.int64, device=x.device)
     lse = torch.empty(shape, dtype=torch.float32, device=x.device)
-    rows = _ROWS.pack(x.data_ptr(), x.stride(0), x.stride(1), 0, 0, 0, 0, 0, 0, x.shape[0], x.shape[1], x.shape[2],
-                      _DTYPES[x.dtype], temperature)
-    with torch.cuda.device(x.device):
-        _lib.raise_for_status(lib.pkv_top_logits(rows, k, values.data_ptr(), tokens.data_ptr(), lse.data_ptr(),
-                                                 _stream(x)))
+    rows = _ROWS.pack(*_array(x), *_NONE, *_NONE, *x.shape, _DTYPES[x.dtype], temperature)
+    _on_device(x, lib.pkv_top_logits, rows, k, values.data_ptr(), tokens.data_ptr(), lse.data_ptr())
     return values, tokens, lse
