@@ -16,6 +16,7 @@
 // value is found exactly, by its digits.  Few rows are spread over clusters;
 // a cluster's first CTA merges the parts' lists.
 #include <cuda_runtime.h>
+#include <float.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -29,12 +30,16 @@
 namespace pkv {
 namespace {
 
-// Three CTAs an SM of 128 threads with a 48 KB ring (as the losses' sums; a third CTA's lists fit no fourth).
-using TopShape = Shape<128, 8, 3, 3>;
+// Two CTAs an SM: 256 threads read the columns, 128 pick the row before.  (One group doing both: 391 us against
+// 341 us for 4 096 rows of 151 936 16-bit columns and k = 64, since the columns waited for each row's picking.)
+using TopShape = Shape<256, 4, 4, 2>;
 constexpr int kTopThreads = TopShape::kGroup;
 constexpr int kTopWarps = TopShape::kWarps;
+constexpr int kPickThreads = 128;
+constexpr int kPickWarps = kPickThreads / 32;
+constexpr int kTopCta = kTopThreads + kPickThreads + 32;
 constexpr int kTopCap = 1024;   // candidates a row may have
-constexpr int kTopGroups = 24;  // groups a thread notes
+constexpr int kTopGroups = 12;  // groups a thread notes
 
 struct TopArgs {
   const void* x;
@@ -59,45 +64,76 @@ __device__ __forceinline__ float unordered(uint32_t o) {
 }
 
 struct alignas(128) TopShared {
-  uint64_t full[TopShape::kSlots], empty[TopShape::kSlots];
-  uint64_t keys[kTopCap];
-  uint64_t best[PKV_MAX_TOP];             // this CTA's list, largest first
-  float tops[kTopGroups][kTopThreads];    // a group's largest value
-  RowSum sum[kTopWarps], all;
-  int part[2][kTopWarps];
+  uint64_t full[TopShape::kSlots], empty[TopShape::kSlots], row_full[2], row_empty[2];
+  alignas(16) uint64_t keys[kTopCap];
+  uint64_t best[PKV_MAX_TOP];                 // this CTA's list, largest first
+  alignas(16) float tops[2][kTopGroups][kTopThreads];  // a group's largest value
+  RowSum sum[2][kTopWarps], all;
+  uint16_t hits[kTopCap];                     // groups that reach the threshold
+  float4 range[kPickWarps];
+  uint32_t part[kPickWarps];
   int hist[256];
-  int count, best_n, gave_up;
+  int count, n_hits, best_n, gave_up;
 };
 
-__device__ __forceinline__ void top_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kTopThreads) : "memory"); }
+// The threads that pick; `pick_id` is a thread's place among them.
+__device__ __forceinline__ void pick_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPickThreads) : "memory"); }
+__device__ __forceinline__ int pick_id() { return (int)threadIdx.x - kTopThreads; }
 
-// The sum of v over the threads; `flip` alternates from call to call.
-__device__ __forceinline__ int top_sum(int v, int& flip, TopShared& sh) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  flip ^= 1;
-  if ((threadIdx.x & 31) == 0) sh.part[flip][threadIdx.x >> 5] = v;
-  top_sync();
-  v = 0;
-  for (int i = 0; i < kTopWarps; ++i) v += sh.part[flip][i];
-  return v;
+// The least lo, the largest hi and the sum of n over them.
+__device__ __forceinline__ void pick_range(float& lo, float& hi, int& n, TopShared& sh) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+  }
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) sh.range[pick_id() >> 5] = make_float4(lo, hi, __int_as_float(n), 0.f);
+  pick_sync();
+  n = 0;
+  for (int i = 0; i < kPickWarps; ++i) {
+    const float4 v = sh.range[i];
+    lo = fminf(lo, v.x), hi = fmaxf(hi, v.y), n += __float_as_int(v.z);
+  }
 }
 
 template <typename T>
 using TopPart = RowPart<T, TopShape::kChunk>;
 
-// f(column, value) for this thread's vector j of the CTA's part, and for its edge column.
-template <typename T, typename F>
-__device__ __forceinline__ void vector_columns(const TopPart<T>& p, int j, F f) {
-  constexpr int VE = RowSplit<T>::VE;
-  float v[VE];
-  unpack<T>(p.body()[j], v);
+// A part of less than a chunk: its vectors go round the threads, so that there are more groups.
+template <typename T>
+__device__ __forceinline__ bool lone_chunk(const TopPart<T>& p) { return p.nv < TopShape::kChunk; }
+
+// f(column, value) for the columns of vector at(i) (< 0: none) of the CTA's part, i = pick_id(), + kPickThreads, ...
+// below n, where the vector's largest value is not below `from` (NaN: all of them).  Four vectors are on their way at once (f's writes would keep a loop's loads apart).
+template <typename T, typename At, typename F>
+__device__ __forceinline__ void vectors(const TopPart<T>& p, int n, At at, float from, F f) {
+  constexpr int VE = RowSplit<T>::VE, kBatch = 4;
+  for (int i0 = pick_id(); i0 < n; i0 += kBatch * kPickThreads) {
+    uint4 v[kBatch];
+    int j[kBatch];
 #pragma unroll
-  for (int q = 0; q < VE; ++q) f(p.head + (p.v0 + j) * VE + q, v[q]);
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * kPickThreads;
+      j[u] = i < n ? at(i) : -1;
+      if (j[u] >= 0) v[u] = p.body()[j[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (j[u] < 0) continue;
+      const uint4 one[1] = {v[u]};
+      if (top_of<T>(one) < from) continue;
+      float x[VE];
+      unpack<T>(v[u], x);
+#pragma unroll
+      for (int q = 0; q < VE; ++q) f(p.head + (p.v0 + j[u]) * VE + q, x[q]);
+    }
+  }
 }
 template <typename T, typename F>
 __device__ __forceinline__ void edge_column(const TopPart<T>& p, int edge, F f) {
-  if ((int)threadIdx.x < edge) {
-    const int c = (int)threadIdx.x < p.head ? threadIdx.x : threadIdx.x + p.nvec * RowSplit<T>::VE;
+  if (pick_id() < edge) {
+    const int c = pick_id() < p.head ? pick_id() : pick_id() + p.nvec * RowSplit<T>::VE;
     f(c, as_float(p.x[c]));
   }
 }
@@ -105,7 +141,7 @@ __device__ __forceinline__ void edge_column(const TopPart<T>& p, int edge, F f) 
 // f(column, value) for every column of the CTA's part of the row, in no order.
 template <typename T, typename F>
 __device__ __forceinline__ void each_column(const TopPart<T>& p, int edge, F f) {
-  for (int j = threadIdx.x; j < p.nv; j += kTopThreads) vector_columns<T>(p, j, f);
+  vectors<T>(p, p.nv, [](int i) { return i; }, NAN, f);
   edge_column<T>(p, edge, f);
 }
 
@@ -119,24 +155,24 @@ __device__ __forceinline__ void take(int c, float v, uint32_t low, TopShared& sh
 
 // The columns whose key is at least `low` go into sh.keys (as many as fit); their number.
 template <typename T>
-__device__ int collect(const TopPart<T>& p, int edge, uint32_t low, TopShared& sh) {
-  top_sync();
-  if (threadIdx.x == 0) sh.count = 0;
-  top_sync();
+__device__ __noinline__ int collect(const TopPart<T>& p, int edge, uint32_t low, TopShared& sh) {
+  pick_sync();
+  if (pick_id() == 0) sh.count = 0;
+  pick_sync();
   each_column<T>(p, edge, [&](int c, float v) { take(c, v, low, sh); });
-  top_sync();
+  pick_sync();
   return sh.count;
 }
 
 // The k-th largest value's key, digit by digit (0 if there are fewer columns).
 template <typename T>
-__device__ uint32_t kth_key(const TopPart<T>& p, int edge, int k, TopShared& sh) {
+__device__ __noinline__ uint32_t kth_key(const TopPart<T>& p, int edge, int k, TopShared& sh) {
   uint32_t prefix = 0;
   int left = k;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    top_sync();
-    for (int i = threadIdx.x; i < 256; i += kTopThreads) sh.hist[i] = 0;
-    top_sync();
+    pick_sync();
+    for (int i = pick_id(); i < 256; i += kPickThreads) sh.hist[i] = 0;
+    pick_sync();
     const uint32_t fixed = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
     each_column<T>(p, edge, [&](int, float v) {
       const uint32_t o = ordered(v);
@@ -145,7 +181,7 @@ __device__ uint32_t kth_key(const TopPart<T>& p, int edge, int k, TopShared& sh)
       const uint32_t d = (o >> shift) & 255u, lanes = __match_any_sync(__activemask(), d);
       if ((threadIdx.x & 31) == __ffs(lanes) - 1) atomicAdd(&sh.hist[d], __popc(lanes));
     });
-    top_sync();
+    pick_sync();
     int d = 255;
     for (; d > 0 && sh.hist[d] < left; --d) left -= sh.hist[d];
     prefix |= (uint32_t)d << shift;
@@ -153,59 +189,121 @@ __device__ uint32_t kth_key(const TopPart<T>& p, int edge, int k, TopShared& sh)
   return prefix;
 }
 
-// This CTA's min(k, columns) best columns of its part into sh.best, largest first; their number.
+// This CTA's min(k, columns) best columns of its part into sh.best, largest first; their number.  `plain`: no column is
+// NaN or +inf.
 template <typename T>
-__device__ int part_list(const TopPart<T>& p, int edge, int k, const RowSum& a, TopShared& sh) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__device__ __forceinline__ int part_list(const TopPart<T>& p, int edge, int k, bool plain, int par, TopShared& sh) {
+  const int tid = pick_id(), lane = tid & 31, warp = tid >> 5;
   constexpr int VE = RowSplit<T>::VE;
   const int columns = p.nv * VE + edge;
   k = min(k, columns);
   if (k == 0) {
-    top_sync();
+    pick_sync();
     return 0;
   }
   const int per = (p.chunks + kTopGroups - 1) / kTopGroups;  // chunks a group spans
   const int groups = per ? (p.chunks + per - 1) / per : 0;
-  int flip = 0;
   uint32_t low = 0;
   int m = kTopCap + 1;
-  const bool plain = top_sum(a.s == a.s ? 0 : 1, flip, sh) == 0;  // no NaN (of a NaN or infinite column)
   if (plain) {
-    // A threshold that k to k + k / 4 + 8 groups reach, if there is one (ties may leave more).  Invariant: at least k
-    // groups (or, for -inf, all columns) reach low, fewer than k reach high + 1.
-    auto reached = [&](uint32_t key) {
-      int c = 0;
-      for (int g = 0; g < groups; ++g) c += ordered(sh.tops[g][tid]) >= key;
-      return top_sum(c, flip, sh);
+    // The threshold is one that k to k + k / 2 + 16 groups reach, if ties allow it, from a histogram of the groups'
+    // values between `lo`, which at least k groups reach (the least of 128 or 512 maxima, each over some of a
+    // thread's groups), and the largest; the bin that holds the k-th is cut again while it is too full.
+    // (Every instruction of these few warps is waited for: the groups' values are read four at a time.)
+    constexpr int kReads = kTopGroups * kTopThreads / (4 * kPickThreads);
+    const float4* tops = reinterpret_cast<const float4*>(sh.tops[par]);
+    const int reads = (groups * kTopThreads / 4 - tid + kPickThreads - 1) / kPickThreads;
+    auto each_top = [&](auto f) {
+#pragma unroll 6
+      for (int r = 0; r < reads; ++r) {
+        const float4 v = tops[r * kPickThreads + tid];
+        f(v.x, 4 * (r * kPickThreads + tid)), f(v.y, 4 * (r * kPickThreads + tid) + 1);
+        f(v.z, 4 * (r * kPickThreads + tid) + 2), f(v.w, 4 * (r * kPickThreads + tid) + 3);
+      }
     };
-    uint32_t high = ordered(INFINITY);
-    low = ordered(-INFINITY);
-    if (reached(low + 1) >= k) {  // (a group notes -inf where it has no column)
-      ++low;
-      while (low < high) {
-        const uint32_t mid = low + (high - low + 1) / 2;
-        const int c = reached(mid);
-        if (c >= k) {
-          low = mid;
-          if (c <= k + k / 4 + 8) break;
-        } else {
-          high = mid - 1;
+    static_assert(kReads * 4 * kPickThreads == kTopGroups * kTopThreads, "whole reads");
+    const int subs = groups > 2 && k <= kPickThreads ? 1 : 4;  // (one value a thread, or four)
+    float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (also what a group notes where it has no column)
+    each_top([&](float t, int g) { best[g & 3] = fmaxf(best[g & 3], t); });
+    float hi = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+    if (subs == 1) best[0] = hi;
+    float lo = INFINITY;
+    int some = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < subs && best[q] > -INFINITY) lo = fminf(lo, best[q]), ++some;
+    pick_range(lo, hi, some, sh);
+    float from = -FLT_MAX;  // all above -inf
+    if (some >= k) {
+      from = lo;
+      for (int level = 0; level < 4 && hi > lo; ++level) {
+        const float scale = 255.f / (hi - lo);
+        for (int b = tid; b < 256; b += kPickThreads) sh.hist[b] = 0;
+        pick_sync();
+        each_top([&](float t, int) {
+          if (t >= lo) atomicAdd(&sh.hist[min(255, (int)((t - lo) * scale))], 1);
+        });
+        pick_sync();
+        // Every warp finds the last bin that k groups reach: a lane has 8 bins, and the sum of the lanes above it.
+        int mine = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mine += sh.hist[8 * lane + e];
+        int above = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const int o = __shfl_down_sync(0xffffffffu, above, off);
+          if (lane + off < 32) above += o;
         }
+        const int at_lane = 31 - __clz(__ballot_sync(0xffffffffu, above >= k));
+        int bin = 0, reached = 0;
+        if (lane == at_lane) {
+          reached = above - mine;
+          for (bin = 8 * lane + 7; bin > 8 * lane; --bin) {
+            if (reached + sh.hist[bin] >= k) break;
+            reached += sh.hist[bin];
+          }
+          reached += sh.hist[bin];
+        }
+        bin = __shfl_sync(0xffffffffu, bin, at_lane);
+        reached = __shfl_sync(0xffffffffu, reached, at_lane);
+        // The bin's lower end, and a little below for the roundings of a value's bin: no value of the bin is lost.
+        const float width = 1.f / scale, slack = 4e-6f * (hi - lo) + 4e-7f * fmaxf(fabsf(lo), fabsf(hi));
+        const float end = lo + (float)bin * width;
+        from = bin ? fmaxf(lo, end - slack) : lo;
+        if (reached <= k + k / 2 + 16 || width < 4.f * slack) break;
+        hi = fminf(hi, end + width);
+        lo = from;
       }
-      if (tid == 0) sh.count = 0;
-      top_sync();
-      auto look = [&](int c, float v) { take(c, v, low, sh); };
-      for (int g = 0; g < groups; ++g) {
-        if (ordered(sh.tops[g][tid]) < low) continue;
-        const int j1 = min(p.nv, (g + 1) * per * TopShape::kChunk);
-        for (int j = g * per * TopShape::kChunk + tid; j < j1; j += kTopThreads) vector_columns<T>(p, j, look);
-      }
-      edge_column<T>(p, edge, look);
-      top_sync();
+    }
+    if (tid == 0) sh.count = sh.n_hits = 0;
+    pick_sync();
+    low = ordered(from);
+    each_top([&](float t, int g) {
+      if (t < from) return;
+      const int at = atomicAdd(&sh.n_hits, 1);
+      if (at < kTopCap) sh.hits[at] = (uint16_t)g;
+    });
+    auto look = [&](int c, float v) { take(c, v, low, sh); };
+    edge_column<T>(p, edge, look);
+    pick_sync();
+    // All threads share the hit groups' vectors.
+    const int hits = sh.n_hits, vecs = per * TopShape::kVecs;
+    const bool lone = lone_chunk<T>(p);
+    if (hits <= kTopCap) {
+      vectors<T>(p, hits * vecs, [&](int i) {
+        const int hit = i / vecs, u = i - hit * vecs, group = sh.hits[hit];
+        const int j = lone ? group + u * kTopThreads
+                           : (group / kTopThreads * per + u / TopShape::kVecs) * TopShape::kChunk +
+                                 group % kTopThreads * TopShape::kVecs + u % TopShape::kVecs;
+        return j < p.nv ? j : -1;
+      }, from, look);
+      pick_sync();
       m = sh.count;
     }
-    // Too many, or fewer groups than k with a column above -inf: the columns above, then the ties.
-    if (m > kTopCap) m = collect<T>(p, edge, low + 1, sh);
+    if (m > kTopCap)
+      m = collect<T>(p, edge, low + 1, sh);  // the columns above, then the ties
+    else if (m < k)
+      low = ordered(-INFINITY);  // all there is above it
   }
   if (m > kTopCap) {
     low = kth_key<T>(p, edge, k, sh);
@@ -215,36 +313,43 @@ __device__ int part_list(const TopPart<T>& p, int edge, int k, const RowSum& a, 
     // Columns equal to low, the lowest first: the part's body, with the row's edges (all in one CTA) around it.
     const int c0 = edge ? 0 : p.head + p.v0 * VE, c1 = p.head + (p.v0 + p.nv) * VE;
     const int tail = p.head + p.nvec * VE, end = edge ? c1 + (edge - p.head) : c1;
-    for (int at0 = c0; at0 < end && m < k; at0 += kTopThreads) {
+    for (int at0 = c0; at0 < end && m < k; at0 += kPickThreads) {
       const int c = at0 + tid < c1 ? at0 + tid : tail + (at0 + tid - c1);
       const bool tie = at0 + tid < end && ordered(as_float(p.x[c])) == low;
       const uint32_t vote = __ballot_sync(0xffffffffu, tie);
-      top_sync();
-      if (lane == 0) sh.part[0][warp] = __popc(vote);
-      top_sync();
+      pick_sync();
+      if (lane == 0) sh.part[warp] = __popc(vote);
+      pick_sync();
       int at = m + __popc(vote & ((1u << lane) - 1u));
-      for (int i = 0; i < kTopWarps; ++i) {
-        if (i < warp) at += sh.part[0][i];
-        m += sh.part[0][i];
+      for (int i = 0; i < kPickWarps; ++i) {
+        if (i < warp) at += (int)sh.part[i];
+        m += (int)sh.part[i];
       }
       if (tie && at < k) sh.keys[at] = (uint64_t)low << 32 | (0xffffffffu - (uint32_t)c);
     }
     m = min(m, k);
-    top_sync();
+    pick_sync();
   }
-  for (int i = tid; i < m; i += kTopThreads) {
+  if (tid == 0 && (m & 1)) sh.keys[m] = 0;  // (no column's key)
+  pick_sync();
+  const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(sh.keys);
+  for (int i = tid; i < m; i += kPickThreads) {
     const uint64_t key = sh.keys[i];
     int rank = 0;
-    for (int j = 0; j < m; ++j) rank += sh.keys[j] > key;
+#pragma unroll 4
+    for (int j = 0; j < (m + 1) / 2; ++j) {
+      const ulonglong2 two = pairs[j];
+      rank += (two.x > key) + (two.y > key);
+    }
     if (rank < k) sh.best[rank] = key;
   }
-  top_sync();
+  pick_sync();
   return k;
 }
 
 // Bound by HBM: the row is read once (16-bit columns: and by the exponentials of its log-sum-exp).
 template <typename T>
-__global__ void __launch_bounds__(kTopThreads + 32, TopShape::kCtas) top_logits_kernel(const TopArgs A) {
+__global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(const TopArgs A) {
   extern __shared__ __align__(128) uint8_t dyn[];
   uint4* slots = reinterpret_cast<uint4*>(dyn);
   TopShared& sh = *reinterpret_cast<TopShared*>(dyn + TopShape::kRingBytes);
@@ -253,6 +358,7 @@ __global__ void __launch_bounds__(kTopThreads + 32, TopShape::kCtas) top_logits_
   const int rank = cluster_rank(), size = cluster_size();
   if (tid == 0) {
     for (int i = 0; i < TopShape::kSlots; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], kTopWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.row_full[i], kTopWarps), mbar_init(&sh.row_empty[i], kPickWarps);
     sh.gave_up = 0;
     fence_barrier_init();
   }
@@ -268,11 +374,10 @@ __global__ void __launch_bounds__(kTopThreads + 32, TopShape::kCtas) top_logits_
       A.lse[row] = bad ? NAN : (float)((log2_of(a.s) + (far_out(c) ? (double)a.m * A.kd : -(double)c)) * kLn2d);
     }
   };
-  if (warp == kTopWarps) {
+  if (warp == kTopWarps + kPickWarps) {
     if (lane == 0) {
       Ring<TopShape::kSlots> r;
       int filled = 0;
-      const uint64_t policy = l2_evict_first_policy();
       for (int row = first; row < n; row += step) {
         const TopPart<T> p(A, row, rank, size);
         for (int c = 0; c < p.chunks; ++c) {
@@ -283,8 +388,7 @@ __global__ void __launch_bounds__(kTopThreads + 32, TopShape::kCtas) top_logits_
           if (*(volatile int*)&sh.gave_up) break;
           const int nv = min(TopShape::kChunk, p.nv - c * TopShape::kChunk);
           mbar_arrive_expect_tx(&sh.full[r.slot], nv * 16);
-          bulk_copy_g2s_hint(slots + r.slot * TopShape::kChunk, p.body() + c * TopShape::kChunk, nv * 16, &sh.full[r.slot],
-                             policy);
+          bulk_copy_g2s(slots + r.slot * TopShape::kChunk, p.body() + c * TopShape::kChunk, nv * 16, &sh.full[r.slot]);
           r.next();
         }
       }
@@ -292,28 +396,33 @@ __global__ void __launch_bounds__(kTopThreads + 32, TopShape::kCtas) top_logits_
         for (int k = 0; k < TopShape::kSlots; ++k)
           if (k < r.slot || filled == TopShape::kSlots) mbar_wait_bounded(&sh.full[k], k < r.slot ? r.phase : r.phase ^ 1);
     }
-  } else {
+  } else if (warp < kTopWarps) {
     Ring<TopShape::kSlots> r;
-    for (int row = first; row < n; row += step) {
+    for (int row = first, it = 0; row < n; row += step, ++it) {
       const TopPart<T> p(A, row, rank, size);
       const int edge = rank == 0 ? A.vocab - p.nvec * VE : 0;
-      const int per = (p.chunks + kTopGroups - 1) / kTopGroups;
+      const int per = (p.chunks + kTopGroups - 1) / kTopGroups, par = it & 1;
+      if (it >= 2) wait_or_mark(&sh.row_empty[par], ((it >> 1) & 1) ^ 1, sh);
       RowSum a{-INFINITY, 0.f, 0.f};
       float top = -INFINITY;
-      for (int c = 0; c < p.chunks; ++c) {
+      for (int c = 0, in_group = 0, group = 0; c < p.chunks; ++c) {
         wait_or_mark(&sh.full[r.slot], r.phase, sh);
         const uint4* in = slots + r.slot * TopShape::kChunk;
         const int nv = min(TopShape::kChunk, p.nv - c * TopShape::kChunk);
+        // A thread's vectors lie together, so that a group is 64 bytes of a chunk; each pair of threads starts at
+        // another of them, which keeps the reads off each other's banks.
+        static_assert(TopShape::kVecs == 4, "the turn below");
+        const int at = tid * 4, turn = tid >> 1;
         if (nv == TopShape::kChunk) {
+          uint4 v[4];
 #pragma unroll
-          for (int h = 0; h < TopShape::kVecs; h += 4) {
-            uint4 v[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = in[tid + (h + u) * kTopThreads];
-            top = fmaxf(top, fold_vecs<false, T>(a, v, A.ks));
-          }
+          for (int u = 0; u < 4; ++u) v[u] = in[at + ((u + turn) & 3)];
+          top = fmaxf(top, fold_vecs<false, T>(a, v, A.ks));
         } else {
-          for (int j = tid; j < nv; j += kTopThreads) {
+          const bool lone = lone_chunk<T>(p);
+          for (int u = 0; u < 4; ++u) {
+            const int j = lone ? tid + u * kTopThreads : at + u;
+            if (j >= nv) break;
             const uint4 v[1] = {in[j]};
             top = fmaxf(top, fold_vecs<false, T>(a, v, A.ks));
           }
@@ -321,27 +430,38 @@ __global__ void __launch_bounds__(kTopThreads + 32, TopShape::kCtas) top_logits_
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.empty[r.slot]);
         r.next();
-        if ((c + 1) % per == 0 || c + 1 == p.chunks) {
-          sh.tops[c / per][tid] = top;
+        if (++in_group == per || c + 1 == p.chunks) {
+          sh.tops[par][group++][tid] = top;
           top = -INFINITY;
+          in_group = 0;
         }
       }
       if (tid < edge) {
         const float f[1] = {as_float(p.x[tid < p.head ? tid : tid + p.nvec * VE])};
         fold<false>(a, f, f[0], A.ks);
       }
-      const RowSum w = warp_merge(a, 32, A.ks);
-      if (lane == 0) sh.sum[warp] = w;
-      const int m = part_list<T>(p, edge, A.k, a, sh);
-      RowSum all = sh.sum[0];
-      for (int i = 1; i < kTopWarps; ++i) sum_merge(all, sh.sum[i], A.ks);
+      a = warp_merge(a, 32, A.ks);
+      if (lane == 0) sh.sum[par][warp] = a;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.row_full[par]);
+    }
+  } else {
+    for (int row = first, it = 0; row < n; row += step, ++it) {
+      const TopPart<T> p(A, row, rank, size);
+      const int edge = rank == 0 ? A.vocab - p.nvec * VE : 0, par = it & 1;
+      wait_or_mark(&sh.row_full[par], (it >> 1) & 1, sh);
+      RowSum all = sh.sum[par][0];
+      for (int i = 1; i < kTopWarps; ++i) sum_merge(all, sh.sum[par][i], A.ks);
+      const int m = part_list<T>(p, edge, A.k, all.s == all.s, par, sh);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.row_empty[par]);
       if (size == 1) {
-        for (int i = tid; i < A.k; i += kTopThreads) write(row, all, sh.best[i], i);
-      } else if (tid == 0) {
+        for (int i = pick_id(); i < A.k; i += kPickThreads) write(row, all, sh.best[i], i);
+      } else if (pick_id() == 0) {
         sh.all = all;
         sh.best_n = m;
       }
-      top_sync();  // (sh.sum and sh.best are read before the next row's)
+      pick_sync();  // (sh.best is read before the next row's)
     }
   }
   if (size == 1) return;
@@ -357,11 +477,11 @@ __global__ void __launch_bounds__(kTopThreads + 32, TopShape::kCtas) top_logits_
       const TopShared* peer = cluster_peer(&sh, q);
       if (q > 0) sum_merge(all, peer->all, A.ks);
       if (tid == 0) s_n[q] = peer->best_n;
-      for (int i = tid; i < peer->best_n; i += kTopThreads + 32) lists[q * PKV_MAX_TOP + i] = peer->best[i];
+      for (int i = tid; i < peer->best_n; i += kTopCta) lists[q * PKV_MAX_TOP + i] = peer->best[i];
       if (tid == 0 && peer->gave_up) sh.gave_up = 1;
     }
     __syncthreads();
-    for (int i = tid; i < size * A.k; i += kTopThreads + 32) {
+    for (int i = tid; i < size * A.k; i += kTopCta) {
       const int q = i / A.k, at = i - q * A.k;
       if (at >= s_n[q]) continue;
       const uint64_t key = lists[q * PKV_MAX_TOP + at];
@@ -420,7 +540,7 @@ extern "C" int32_t pkv_top_logits(const pkv_loss_rows* r, int32_t k, float* valu
   auto launch = [&](auto* kernel) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess)
       return cuda_status("top_logits shared memory");
-    return launch_after(kernel, grid, kTopThreads + 32, c, kBytes, a, s, "top_logits launch");
+    return launch_after(kernel, grid, kTopCta, c, kBytes, a, s, "top_logits launch");
   };
   if (r->dtype == PKV_F32) return launch(top_logits_kernel<float>);
   if (r->dtype == PKV_F16) return launch(top_logits_kernel<__half>);
