@@ -699,7 +699,7 @@ typedef struct pkv_loss_rows {
   int64_t mask_batch_stride, mask_row_stride;
   int32_t batch, length, vocab;
   int32_t dtype;              /* enum pkv_dtype */
-  float temperature;          /* rows are logits / temperature */
+  float temperature;          /* rows are logits / temperature, in [1e-6, 1e6] */
 } pkv_loss_rows;
 
 /* One value a row: [batch][length] with element strides (0 broadcasts); data NULL: absent. */

@@ -34,19 +34,18 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// k = log2(e) / T, as a pair of floats where one is off by more than 2e-8 of
-// it (at T = 1 it is not): a sum over many columns shows the scale's error as
-// that much of log p, which is up to about 20.
+// k = log2(e) / T as a pair of floats: one float's error (up to 6e-8 of k) shows in log p as that much of it, and adds
+// up in a sequence's sum.  lo > 0, so that a column of -inf stays -inf in x hi + x lo.
 struct Scale2 {
   float hi, lo;
 };
 inline Scale2 scale_for(float temperature, double* kd) {
   const double k = kLog2ed / (double)temperature;
-  Scale2 s{(float)k, 0.f};
-  if ((double)s.hi > k) s.hi = nextafterf(s.hi, 0.f);  // lo >= 0: a column of -inf stays -inf in x hi + x lo
-  if (k - (double)s.hi > 2e-8 * k) s.lo = (float)(k - (double)s.hi);
-  *kd = (double)s.hi + (double)s.lo;
-  return s;
+  float hi = (float)k;
+  if ((double)hi >= k) hi = nextafterf(hi, 0.f);
+  const float lo = (float)(k - (double)hi);
+  *kd = (double)hi + (double)lo;
+  return Scale2{hi, lo};
 }
 
 __device__ __forceinline__ float ex2(float y) {
@@ -199,13 +198,11 @@ __device__ __forceinline__ float top_of(const uint4 (&v)[N]) {
   }
 }
 
-// Add columns whose largest is `top` to the running sums.  LO: the scale has a second float.
-template <bool ENT, bool LO, int N>
+// Add columns whose largest is `top` to the running sums.
+template <bool ENT, int N>
 __device__ __forceinline__ void fold_near(RowSum& a, const float (&x)[N], float c, Scale2 k) {
   if constexpr (N == 1) {
-    float y = fmaf(x[0], k.hi, c);
-    if (LO) y = fmaf(x[0], k.lo, y);
-    const float e = ex2(y);
+    const float y = fmaf(x[0], k.lo, fmaf(x[0], k.hi, c)), e = ex2(y);
     a.s += e;
     if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
   } else {
@@ -215,9 +212,7 @@ __device__ __forceinline__ void fold_near(RowSum& a, const float (&x)[N], float 
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
       const f32x2 xx = pair(x[i], x[i + 1]);
-      f32x2 y2 = fma2(xx, hi, cc);
-      if (LO) y2 = fma2(xx, lo, y2);
-      const float2 y = unpair(y2);
+      const float2 y = unpair(fma2(xx, lo, fma2(xx, hi, cc)));
       const f32x2 e = pair(ex2(y.x), ex2(y.y));
       s[(i / 2) & 1] = add2(s[(i / 2) & 1], e);
       if (ENT) w = fma2(e, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), w);
@@ -245,10 +240,8 @@ __device__ __forceinline__ void fold(RowSum& a, const float (&x)[N], float top, 
       a.s += e;
       if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
     }
-  } else if (k.lo == 0.f) {
-    fold_near<ENT, false>(a, x, c, k);
   } else {
-    fold_near<ENT, true>(a, x, c, k);
+    fold_near<ENT>(a, x, c, k);
   }
 }
 

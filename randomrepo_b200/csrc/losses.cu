@@ -234,7 +234,7 @@ __device__ __forceinline__ void grad_columns(float (&x)[N], const RowGrad& o, Sc
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     float y = fmaf(x[i], k.hi, c);
-    if (sizeof(T) == 4 && k.lo != 0.f) y = fmaf(x[i], k.lo, y);  // (half a step of 16 bits hides it)
+    if (sizeof(T) == 4) y = fmaf(x[i], k.lo, y);  // (half a step of 16 bits hides it)
     x[i] = ex2(y) * (ENT ? fmaf(o.b, fmaxf(y, -1e30f), o.a) : o.a);
   }
 }
@@ -874,8 +874,8 @@ int32_t check_vocab_rows(const pkv_loss_rows* r, const char* who) {
   if (r->vocab > (1 << 30)) return fail(PKV_ERR_UNSUPPORTED, w + ": more than 2^30 columns");
   if (r->dtype != PKV_F32 && r->dtype != PKV_F16 && r->dtype != PKV_BF16)
     return fail(PKV_ERR_ARG, w + ": unknown dtype");
-  if (!(r->temperature > 0.f) || !std::isfinite(r->temperature))
-    return fail(PKV_ERR_ARG, w + ": the temperature must be positive and finite");
+  if (!(r->temperature >= 1e-6f && r->temperature <= 1e6f))
+    return fail(PKV_ERR_ARG, w + ": the temperature must lie in [1e-6, 1e6]");
   const int64_t size = r->dtype == PKV_F32 ? 4 : 2;
   if ((int64_t)r->batch * r->length > 0) {
     if (!r->logits || (uintptr_t)r->logits % size) return fail(PKV_ERR_ARG, w + ": logits pointer");

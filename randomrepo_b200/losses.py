@@ -26,7 +26,6 @@ logits' device, never synchronise, and can be captured in a CUDA graph.  There i
 
 from __future__ import annotations
 
-import math
 import struct
 from typing import NamedTuple
 
@@ -91,14 +90,13 @@ def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
     return logits.unsqueeze(0) if logits.dim() == 2 else logits
 
 
-def _rows_like(t: torch.Tensor, x: torch.Tensor, dtype: torch.dtype, what: str, name: str,
+def _rows_like(t: torch.Tensor, rows: torch.Size, dev: torch.device, dtype: torch.dtype, what: str, name: str,
                broadcast: bool = False) -> torch.Tensor:
-    """A per-row input as [B, T] of ``dtype`` on the logits' device (``broadcast``: [B] or [B, 1] too)."""
+    """A per-row input as [B, T] (``rows``) of ``dtype`` on ``dev`` (``broadcast``: [B] or [B, 1] too)."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{what}: {name} must be a tensor")
-    if t.device != x.device:
+    if t.device != dev:
         raise ValueError(f"{what}: {name} must be on the logits' device")
-    rows = x.shape[:2]
     if t.shape != rows:
         b, n = rows
         if broadcast and t.dim() == 1 and t.shape[0] == b and (b != 1 or n == 1):
@@ -116,14 +114,14 @@ def _rows_like(t: torch.Tensor, x: torch.Tensor, dtype: torch.dtype, what: str, 
     return t
 
 
-def _mask(mask: torch.Tensor | None, x: torch.Tensor, what: str) -> torch.Tensor | None:
+def _mask(mask: torch.Tensor | None, rows: torch.Size, dev: torch.device, what: str) -> torch.Tensor | None:
     """The mask as bytes [B, T] (anything but 0 is scored)."""
     if mask is None:
         return None
     if isinstance(mask, torch.Tensor) and mask.dtype not in (torch.bool, torch.uint8):
         mask = mask != 0
     # (a byte each, read as such)
-    return _rows_like(mask, x, mask.dtype if isinstance(mask, torch.Tensor) else torch.bool, what, "mask")
+    return _rows_like(mask, rows, dev, mask.dtype if isinstance(mask, torch.Tensor) else torch.bool, what, "mask")
 
 
 def _array(t: torch.Tensor | None) -> tuple[int, int, int]:
@@ -163,8 +161,8 @@ class _Call:
 
     def __init__(self, x, mask, temperature, terms, keep, backward, what):
         temperature = float(temperature)
-        if not 0.0 < temperature < math.inf:
-            raise ValueError(f"{what}: the temperature must be positive and finite")
+        if not 1e-6 <= temperature <= 1e6:
+            raise ValueError(f"{what}: the temperature must lie in [1e-6, 1e6]")
         self.x, self.mask, self.temperature = x, mask, temperature
         self.terms, self.keep, self.backward = terms, keep, backward
         b, n, _ = x.shape
@@ -200,30 +198,29 @@ class _RowLoss(torch.autograd.Function):
     """Forward: the loss call without a gradient.  Backward: the rows again, times the upstream gradient."""
 
     @staticmethod
-    def forward(ctx, logits, x, call, fn, outputs):
+    def forward(ctx, logits, call, fn, outputs):
         _launch(fn, call, None, outputs)
         ctx.call = call
         ctx.save_for_backward(logits, call.ws, *[t for t in call.keep if t is not None])
-        ctx.mark_non_differentiable(*[t for t in outputs[1:] if t is not None])
-        return outputs[:1] + tuple(t for t in outputs[1:] if t is not None)
+        return outputs[0]
 
     @staticmethod
-    def backward(ctx, grad_loss, *_):
+    def backward(ctx, grad_loss):
         if torch.is_grad_enabled():  # (create_graph=True)
             raise RuntimeError("the vocabulary-row losses are differentiable once")
         logits = ctx.saved_tensors[0]  # (also checks that nothing was changed in place since)
         c = ctx.call
         grad = _grad_like(c.x)
-        up = grad_loss.to(dtype=torch.float32, device=c.x.device)
-        _launch(c.backward, c, grad, (up,))
-        return grad.view(logits.shape) if grad.shape != logits.shape else grad, None, None, None, None
+        if grad_loss.dtype != torch.float32 or grad_loss.device != c.x.device:
+            grad_loss = grad_loss.to(dtype=torch.float32, device=c.x.device)
+        _launch(c.backward, c, grad, (grad_loss,))
+        return grad.view(logits.shape) if grad.dim() != logits.dim() else grad, None, None, None
 
 
 def _run(fn, c: _Call, logits: torch.Tensor, outputs: tuple):
-    """The outputs of a differentiable call."""
+    """The outputs of a differentiable call: the loss, and per-row values without a gradient."""
     if logits.requires_grad and torch.is_grad_enabled():
-        got = iter(_RowLoss.apply(logits, c.x, c, fn, outputs))
-        return tuple(None if t is None else next(got) for t in outputs)
+        return (_RowLoss.apply(logits, c, fn, outputs), *outputs[1:])
     _launch(fn, c, None, outputs)
     return outputs
 
@@ -231,7 +228,7 @@ def _run(fn, c: _Call, logits: torch.Tensor, outputs: tuple):
 def _run_with_grad(fn, c: _Call, logits: torch.Tensor, outputs: tuple) -> torch.Tensor:
     grad = _grad_like(c.x)
     _launch(fn, c, grad, outputs)
-    return grad if grad.shape == logits.shape else grad.squeeze(0)
+    return grad if grad.dim() == logits.dim() else grad.squeeze(0)
 
 
 def _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef, entropy_coef,
@@ -240,16 +237,16 @@ def _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_l
     x = _logits(logits, what)
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError(f"{what}: clip_low and clip_high must be >= 0")
-    tok = _rows_like(tokens, x, torch.int64, what, "tokens")
-    adv = _rows_like(advantages, x, torch.float32, what, "advantages", broadcast=True)
-    old = None if old_logprobs is None else _rows_like(old_logprobs, x, torch.float32, what, "old_logprobs")
-    ref = None if ref_logprobs is None else _rows_like(ref_logprobs, x, torch.float32, what, "ref_logprobs")
-    m = _mask(mask, x, what)
+    rows, dev = x.shape[:2], x.device
+    tok = _rows_like(tokens, rows, dev, torch.int64, what, "tokens")
+    adv = _rows_like(advantages, rows, dev, torch.float32, what, "advantages", broadcast=True)
+    old = None if old_logprobs is None else _rows_like(old_logprobs, rows, dev, torch.float32, what, "old_logprobs")
+    ref = None if ref_logprobs is None else _rows_like(ref_logprobs, rows, dev, torch.float32, what, "ref_logprobs")
+    m = _mask(mask, rows, dev, what)
     terms = _POLICY.pack(*_array(tok), *_array(adv), *_array(old), *_array(ref), clip_low, clip_high, kl_coef,
                          entropy_coef, _reduction(reduction, what), scale)
     c = _Call(x, m, temperature, terms, (tok, adv, old, ref, m), lib.pkv_policy_loss_backward, what)
     shape = logits.shape[:-1]
-    dev = x.device
     outputs = (torch.empty((), dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.float32, device=dev),
                None if ref is None else torch.empty(shape, dtype=torch.float32, device=dev),
                torch.empty(shape, dtype=torch.float32, device=dev) if entropy_coef else None)
@@ -295,8 +292,9 @@ def _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, lengt
         raise ValueError(f"{what}: logits must be [2 * pairs, length, vocab], the chosen answers first")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"{what}: label_smoothing must lie in [0, 1]")
-    tok = _rows_like(tokens, x, torch.int64, what, "tokens")
-    m = _mask(mask, x, what)
+    rows, dev = x.shape[:2], x.device
+    tok = _rows_like(tokens, rows, dev, torch.int64, what, "tokens")
+    m = _mask(mask, rows, dev, what)
     ref = ref_logprobs
     if ref is not None:
         if not isinstance(ref, torch.Tensor) or ref.device != x.device or tuple(ref.shape) != (x.shape[0],):
@@ -360,9 +358,11 @@ def _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temper
     tl = _teacher_list(teacher_logits, logits, torch.float32, what, "teacher_logits")
     if ids.shape != tl.shape:
         raise ValueError(f"{what}: teacher_ids and teacher_logits must have the same shape")
-    lse = None if teacher_lse is None else _rows_like(teacher_lse, x, torch.float32, what, "teacher_lse")
-    m = _mask(mask, x, what)
-    terms = _DISTILLATION.pack(*_array(ids), *_array(tl), ids.shape[-1], *_array(lse), _reduction(reduction, what), scale)
+    rows, dev = x.shape[:2], x.device
+    lse = None if teacher_lse is None else _rows_like(teacher_lse, rows, dev, torch.float32, what, "teacher_lse")
+    m = _mask(mask, rows, dev, what)
+    terms = _DISTILLATION.pack(*_array(ids), *_array(tl), ids.shape[-1], *_array(lse), _reduction(reduction, what),
+                               scale)
     c = _Call(x, m, temperature, terms, (ids, tl, lse, m), lib.pkv_distillation_loss_backward, what)
     return c, (torch.empty((), dtype=torch.float32, device=x.device),
                torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device))
@@ -408,8 +408,8 @@ def top_logits(logits: torch.Tensor, k: int, *,
     if not 1 <= k <= min(_MAX_TOP, x.shape[-1]):
         raise ValueError(f"{what}: k must be from 1 to {min(_MAX_TOP, x.shape[-1])}")
     temperature = float(temperature)
-    if not 0.0 < temperature < math.inf:
-        raise ValueError(f"{what}: the temperature must be positive and finite")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"{what}: the temperature must lie in [1e-6, 1e6]")
     shape = logits.shape[:-1]
     values = torch.empty((*shape, k), dtype=torch.float32, device=x.device)
     tokens = torch.empty((*shape, k), dtype=torch.int64, device=x.device)

@@ -29,6 +29,11 @@ head_dim, dtype code]`` (the ``pkv_pool_geom`` of the C ABI).
   (a verify step) over a ``pkv_verify_plan``, on the kernel that puts keys on
   the tensor-core rows (``PagedKVCacheStore.prefill_step`` picks it when the
   chunks fit).
+* ``policy_loss(...)``, ``preference_loss(...)``, ``distillation_loss(...)``
+  ``-> (loss, per-row outputs, dlogits)``: the vocabulary-row losses with
+  their gradients (``randomrepo_b200.losses.*_loss_and_grad``; outputs a call
+  does not have are empty), and ``top_logits(logits, k, temperature) ->
+  (values, tokens, lse)``.
 """
 
 from __future__ import annotations
@@ -37,7 +42,7 @@ import ctypes
 
 import torch
 
-from . import _lib
+from . import _lib, losses
 from ._lib import lib
 
 __all__ = ["pool_geom"]
@@ -203,3 +208,76 @@ def verify_attention(pool: torch.Tensor, geom: list[int], layer: int, q: torch.T
 def _(pool, geom, layer, q, block_tables, work_items, n_items, n_ctas, n_combine, n_slots, scale, error_word,
       workspace):
     return torch.empty_like(q)
+
+
+def _none_like(t: torch.Tensor | None, logits: torch.Tensor) -> torch.Tensor:
+    return logits.new_empty(0, dtype=torch.float32) if t is None else t
+
+
+@torch.library.custom_op("pkv::policy_loss", mutates_args=(), device_types="cuda")
+def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Tensor,
+                old_logprobs: torch.Tensor | None, mask: torch.Tensor | None, ref_logprobs: torch.Tensor | None,
+                clip_low: float, clip_high: float, kl_coef: float, entropy_coef: float, temperature: float,
+                reduction: str, scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                                                       torch.Tensor]:
+    """``losses.policy_loss_and_grad``: (loss, logprobs, kl, entropy, dlogits); kl is empty without a
+    reference, entropy with an entropy_coef of 0."""
+    r, grad = losses.policy_loss_and_grad(logits, tokens, advantages, old_logprobs, mask, ref_logprobs=ref_logprobs,
+                                          clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef,
+                                          entropy_coef=entropy_coef, temperature=temperature, reduction=reduction,
+                                          scale=scale)
+    return r.loss, r.logprobs, _none_like(r.kl, logits), _none_like(r.entropy, logits), grad.contiguous()
+
+
+@policy_loss.register_fake
+def _(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef, entropy_coef,
+      temperature, reduction, scale):
+    row = lambda there: logits.new_empty(logits.shape[:-1] if there else (0,), dtype=torch.float32)  # noqa: E731
+    return (logits.new_empty((), dtype=torch.float32), row(True), row(ref_logprobs is not None),
+            row(entropy_coef != 0), logits.new_empty(logits.shape))
+
+
+@torch.library.custom_op("pkv::preference_loss", mutates_args=(), device_types="cuda")
+def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | None,
+                    ref_logprobs: torch.Tensor | None, beta: float, label_smoothing: float, length_normalised: bool,
+                    scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``losses.preference_loss_and_grad``: (loss, logprobs, margins, dlogits)."""
+    r, grad = losses.preference_loss_and_grad(logits, tokens, mask, ref_logprobs, beta=beta,
+                                              label_smoothing=label_smoothing, length_normalised=length_normalised,
+                                              scale=scale)
+    return r.loss, r.logprobs, r.margins, grad.contiguous()
+
+
+@preference_loss.register_fake
+def _(logits, tokens, mask, ref_logprobs, beta, label_smoothing, length_normalised, scale):
+    f32 = lambda *s: logits.new_empty(s, dtype=torch.float32)  # noqa: E731
+    return f32(), f32(logits.shape[0]), f32(logits.shape[0] // 2), logits.new_empty(logits.shape)
+
+
+@torch.library.custom_op("pkv::distillation_loss", mutates_args=(), device_types="cuda")
+def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                      mask: torch.Tensor | None, teacher_lse: torch.Tensor | None, temperature: float, reduction: str,
+                      scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``losses.distillation_loss_and_grad``: (loss, kl, dlogits)."""
+    r, grad = losses.distillation_loss_and_grad(logits, teacher_ids, teacher_logits, mask, teacher_lse=teacher_lse,
+                                                temperature=temperature, reduction=reduction, scale=scale)
+    return r.loss, r.kl, grad.contiguous()
+
+
+@distillation_loss.register_fake
+def _(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale):
+    return (logits.new_empty((), dtype=torch.float32), logits.new_empty(logits.shape[:-1], dtype=torch.float32),
+            logits.new_empty(logits.shape))
+
+
+@torch.library.custom_op("pkv::top_logits", mutates_args=(), device_types="cuda")
+def top_logits(logits: torch.Tensor, k: int, temperature: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``losses.top_logits``: (values, tokens, lse)."""
+    return losses.top_logits(logits, k, temperature=temperature)
+
+
+@top_logits.register_fake
+def _(logits, k, temperature):
+    shape = logits.shape[:-1]
+    return (logits.new_empty((*shape, k), dtype=torch.float32), logits.new_empty((*shape, k), dtype=torch.int64),
+            logits.new_empty(shape, dtype=torch.float32))

@@ -567,3 +567,91 @@ def test_a_rollouts_training_step(cuda_device):
         (step,) = torch.autograd.grad(out.loss, student)
         student = (student - step).detach().requires_grad_()
     assert step.isfinite().all() and out.loss.isfinite()
+
+
+def test_operators_equal_the_functions(cuda_device):
+    """``torch.ops.pkv`` losses are the same calls."""
+    import randomrepo_b200.ops  # noqa: F401 - registers the operators
+    from randomrepo_b200 import losses
+
+    logits, ids, teacher, g = _distill_case(4, 6, 1001, 9, BF16, cuda_device)
+    tokens = torch.randint(0, 1001, (4, 6), generator=g).to(cuda_device)
+    mask = _mask("some", 4, 6, g, cuda_device)
+    adv = torch.randn(4, generator=g).to(cuda_device)
+    ref = -7 + torch.randn(4, 6, generator=g).to(cuda_device)
+    want, grad = losses.policy_loss_and_grad(logits, tokens, adv, None, mask, ref_logprobs=ref, kl_coef=0.1)
+    got = torch.ops.pkv.policy_loss(logits, tokens, adv, None, mask, ref, 0.2, 0.2, 0.1, 0.0, 1.0, "token_mean", 1.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, (*want[:3], torch.empty(0, device=cuda_device), grad)))
+    want, grad = losses.preference_loss_and_grad(logits, tokens, mask, None, beta=0.3)
+    got = torch.ops.pkv.preference_loss(logits, tokens, mask, None, 0.3, 0.0, False, 1.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, (*want, grad)))
+    want, grad = losses.distillation_loss_and_grad(logits, ids, teacher, mask, temperature=2.0)
+    got = torch.ops.pkv.distillation_loss(logits, ids, teacher, mask, None, 2.0, "token_mean", 1.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, (*want, grad)))
+    got = torch.ops.pkv.top_logits(logits, 5, 1.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, losses.top_logits(logits, 5)))
+
+
+def test_refusals_on_the_device(cuda_device):
+    """What the host can see is refused before a launch; a second derivative and a changed input are errors."""
+    from randomrepo_b200 import losses
+
+    logits, g = _logits(2, 3, 33, F32, cuda_device)
+    tokens = torch.randint(0, 33, (2, 3), generator=g).to(cuda_device)
+    adv = torch.ones(2, device=cuda_device)
+    with pytest.raises(ValueError):
+        losses.policy_loss(logits, tokens.cpu(), adv)
+    with pytest.raises(ValueError):
+        losses.policy_loss(logits, tokens, adv, mask=torch.ones(2, 3))  # on the host
+    with pytest.raises(ValueError):
+        losses.top_logits(logits, 34)
+    leaf = logits.detach().requires_grad_()
+    out = losses.policy_loss(leaf, tokens, adv)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out.loss, leaf, create_graph=True)
+    out = losses.policy_loss(leaf, tokens, adv)
+    tokens.add_(0)
+    with pytest.raises(RuntimeError, match="modified"):
+        out.loss.backward()
+
+
+def test_int_masks_and_types_are_taken(cuda_device):
+    """HF attention masks (int64), uint8 and float masks, int32 tokens, float64 inputs and [T, V] rows."""
+    from randomrepo_b200 import losses
+
+    logits, tokens, adv, old, ref, mask = _policy_case(3, 7, 301, F32, cuda_device, "some")
+    want, grad = losses.policy_loss_and_grad(logits, tokens, adv, old, mask, ref_logprobs=ref, kl_coef=0.1)
+    for m in (mask.long(), mask.byte() * 255, mask.float() * 0.5):
+        got, g2 = losses.policy_loss_and_grad(logits, tokens.int(), adv.double(), old.double(), m, ref_logprobs=ref,
+                                              kl_coef=0.1)
+        assert torch.equal(got.loss, want.loss) and torch.equal(grad, g2)
+    one, g1 = losses.policy_loss_and_grad(logits[0], tokens[0], adv[0], old[0], mask[0], reduction="sum")
+    two, g2 = losses.policy_loss_and_grad(logits[:1], tokens[:1], adv[:1], old[:1], mask[:1], reduction="sum")
+    assert one.logprobs.shape == (7,) and g1.shape == (7, 301)
+    assert torch.equal(one.loss, two.loss) and torch.equal(g1, g2[0])
+    leaf = logits[0].detach().requires_grad_()
+    losses.policy_loss(leaf, tokens[0], adv[0], old[0], mask[0], reduction="sum").loss.backward()
+    torch.testing.assert_close(leaf.grad, g1, atol=1e-6, rtol=1e-5)
+
+
+def test_rows_past_32_bits(cuda_device):
+    """A tensor whose last rows start past 2^32 bytes and 2^31 elements."""
+    from randomrepo_b200 import losses
+
+    v = 151936
+    flat = torch.zeros(16384, v, dtype=BF16, device=cuda_device)  # 2.5 G elements
+    g = torch.Generator().manual_seed(3)
+    small = (torch.randn(3, v, generator=g) * 3).to(BF16).to(cuda_device)
+    flat[-3:] = small
+    mask = torch.zeros(1, 16384, dtype=torch.bool, device=cuda_device)
+    mask[0, -3:] = True
+    tokens = torch.randint(0, v, (1, 16384), generator=g).to(cuda_device)
+    adv = torch.ones(1, device=cuda_device)
+    got, grad = losses.policy_loss_and_grad(flat.unsqueeze(0), tokens, adv, None, mask)
+    want, wgrad = losses.policy_loss_and_grad(small.unsqueeze(0), tokens[:, -3:], adv)
+    torch.testing.assert_close(got.logprobs[0, -3:], want.logprobs[0], atol=LP, rtol=0)
+    torch.testing.assert_close(grad[0, -3:].float(), wgrad[0].float(), atol=1e-6, rtol=2.0**-7)
+    assert not grad[0, :-3].any()
+    del grad, wgrad
+    values, ids, _ = losses.top_logits(flat, 4)
+    assert torch.equal(ids[-3:], _top_definition(small, 4)[1]) and torch.equal(ids[0].cpu(), torch.arange(4))

@@ -188,3 +188,31 @@ def test_gradients_are_laid_out_like_the_logits_rows():
         assert last <= g.untyped_storage().nbytes() // 2
     wide = torch.zeros(1, 1, 17).expand(3, 4, 17)
     assert losses._grad_like(wide).is_contiguous()
+
+
+def test_operators_have_fake_shapes():
+    """``torch.ops.pkv`` losses trace with fake tensors: shapes and types without running a kernel."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import randomrepo_b200.ops  # noqa: F401 - registers the operators
+
+    with FakeTensorMode():
+        dev = torch.device("cuda", 0)
+        for shape in ((4, 9, 1001), (9, 1001)):
+            x = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+            rows = shape[:-1]
+            tok = torch.empty(rows, dtype=torch.int64, device=dev)
+            f = torch.empty(rows, device=dev)
+            loss, lp, kl, ent, grad = torch.ops.pkv.policy_loss(x, tok, f, f, None, f, 0.2, 0.2, 0.1, 0.0, 1.0, "sum", 1.0)
+            assert loss.shape == () and lp.shape == rows and kl.shape == rows and ent.shape == (0,)
+            assert grad.shape == shape and grad.dtype == torch.bfloat16 and lp.dtype == torch.float32
+            ids = torch.empty((*rows, 5), dtype=torch.int64, device=dev)
+            loss, kl, grad = torch.ops.pkv.distillation_loss(x, ids, torch.empty((*rows, 5), device=dev), None, None,
+                                                             2.0, "token_mean", 1.0)
+            assert loss.shape == () and kl.shape == rows and grad.shape == shape
+            v, t, lse = torch.ops.pkv.top_logits(x, 7, 1.0)
+            assert v.shape == (*rows, 7) and t.dtype == torch.int64 and lse.shape == rows
+        x = torch.empty((4, 9, 1001), device=dev)
+        loss, s, m, grad = torch.ops.pkv.preference_loss(x, torch.empty((4, 9), dtype=torch.int64, device=dev), None,
+                                                         None, 0.1, 0.0, False, 1.0)
+        assert loss.shape == () and s.shape == (4,) and m.shape == (2,) and grad.shape == x.shape
