@@ -198,64 +198,77 @@ __device__ __forceinline__ float top_of(const uint4 (&v)[N]) {
   }
 }
 
-// Add columns whose largest is `top` to the running sums.
-template <bool ENT, int N>
-__device__ __forceinline__ void fold_near(RowSum& a, const float (&x)[N], float c, Scale2 k) {
-  if constexpr (N == 1) {
-    const float y = fmaf(x[0], k.lo, fmaf(x[0], k.hi, c)), e = ex2(y);
-    a.s += e;
-    if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
-  } else {
-    static_assert(N % 2 == 0, "columns go in pairs");
-    const f32x2 cc = pair(c, c), hi = pair(k.hi, k.hi), lo = pair(k.lo, k.lo);
-    f32x2 s[2] = {pair(a.s, 0.f), 0ull}, w = pair(a.w, 0.f);
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const f32x2 xx = pair(x[i], x[i + 1]);
-      const float2 y = unpair(fma2(xx, lo, fma2(xx, hi, cc)));
-      const f32x2 e = pair(ex2(y.x), ex2(y.y));
-      s[(i / 2) & 1] = add2(s[(i / 2) & 1], e);
-      if (ENT) w = fma2(e, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), w);
-    }
-    const float2 t = unpair(add2(s[0], s[1])), u = unpair(w);
-    a.s = t.x + t.y;
-    if (ENT) a.w = u.x + u.y;
-  }
-}
+// The running sums of a thread.  m is a column near the largest so far: as long as no column's 2^y passes 2^20 it
+// stays, so that the sums are rarely rescaled.  c is its center, +inf where there is none (no column yet, or far out).
+template <bool ENT>
+struct Fold {
+  float m = -INFINITY, c = INFINITY;
+  f32x2 s0 = 0ull, s1 = 0ull, w = 0ull;
 
-template <bool ENT, int N>
-__device__ __forceinline__ void fold(RowSum& a, const float (&x)[N], float top, Scale2 k) {
-  if (!(top > -INFINITY)) {  // nothing but -inf, or NaN
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (x[i] != x[i]) a.s = NAN;
-    return;
+  __device__ __forceinline__ RowSum sum() const {
+    const float2 t = unpair(add2(s0, s1)), u = unpair(w);
+    return RowSum{m, t.x + t.y, ENT ? u.x + u.y : 0.f};
   }
-  if (top > a.m) sum_rescale(a, top, k);
-  const float c = center(a.m, k);
-  if (far_out(c)) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float y = (x[i] - a.m) * k.hi, e = ex2(y);
-      a.s += e;
-      if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
-    }
-  } else {
-    fold_near<ENT>(a, x, c, k);
-  }
-}
 
-// N vectors of a row's body; their largest column.
-template <bool ENT, typename T, int N>
-__device__ __forceinline__ float fold_vecs(RowSum& a, const uint4 (&v)[N], Scale2 k) {
-  constexpr int VE = 16 / sizeof(T);
-  float f[N * VE];
+  // Add columns whose largest is `top`.
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], float top, Scale2 k) {
+    if (!(fmaf(top, k.hi, c) <= 20.f)) {
+      RowSum a = sum();
+      if (!(top > -INFINITY)) {  // nothing but -inf, or NaN
 #pragma unroll
-  for (int i = 0; i < N; ++i) unpack<T>(v[i], *reinterpret_cast<float (*)[VE]>(f + i * VE));
-  const float top = top_of<T>(v);
-  fold<ENT>(a, f, top, k);
-  return top;
-}
+        for (int i = 0; i < N; ++i)
+          if (x[i] != x[i]) a.s = NAN;
+      } else {
+        if (top > m) sum_rescale(a, top, k);
+        m = a.m;
+        const float at = center(m, k);
+        c = far_out(at) ? INFINITY : at;
+        if (far_out(at)) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float y = (x[i] - m) * k.hi, e = ex2(y);
+            a.s += e;
+            if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
+          }
+        }
+      }
+      s0 = pair(a.s, 0.f), s1 = 0ull, w = pair(a.w, 0.f);
+      if (c == INFINITY) return;
+    }
+    if constexpr (N == 1) {
+      const float y = fmaf(x[0], k.lo, fmaf(x[0], k.hi, c)), e = ex2(y);
+      s0 = add2(s0, pair(e, 0.f));
+      if (ENT) w = add2(w, pair(e * fmaxf(y, -1e30f), 0.f));
+    } else {
+      static_assert(N % 4 == 0, "columns go in pairs, to two sums");
+      const f32x2 cc = pair(c, c), hi = pair(k.hi, k.hi), lo = pair(k.lo, k.lo);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const f32x2 xx = pair(x[i], x[i + 1]);
+        const float2 y = unpair(fma2(xx, lo, fma2(xx, hi, cc)));
+        const f32x2 e = pair(ex2(y.x), ex2(y.y));
+        if (i & 2)
+          s1 = add2(s1, e);
+        else
+          s0 = add2(s0, e);
+        if (ENT) w = fma2(e, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), w);
+      }
+    }
+  }
+
+  // Add N vectors of a row's body; their largest column.
+  template <typename T, int N>
+  __device__ __forceinline__ float add_vecs(const uint4 (&v)[N], Scale2 k) {
+    constexpr int VE = 16 / sizeof(T);
+    float f[N * VE];
+#pragma unroll
+    for (int i = 0; i < N; ++i) unpack<T>(v[i], *reinterpret_cast<float (*)[VE]>(f + i * VE));
+    const float top = top_of<T>(v);
+    add(f, top, k);
+    return top;
+  }
+};
 
 // ---------------------------------------------------------------------------
 // Rows through a shared-memory ring, by a CTA or a cluster.

@@ -515,7 +515,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
     const uint32_t phase = (it >> 1) & 1;
     const int again = PASS == kFused ? p.chunks - min(p.chunks, S::kSlots) : 0;
     if (PASS != kBackward && i < n_active) {
-      RowSum a{-INFINITY, 0.f, 0.f};
+      Fold<ENT> fold;
       for (int c = 0; c < p.chunks; ++c) {
         wait_or_mark(&sh.full[r.slot], r.phase, sh);
         const uint4* in = slots + r.slot * S::kChunk;
@@ -528,12 +528,12 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
             uint4 v[kAtOnce];
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) v[u] = in[tid + (h + u) * S::kGroup];
-            fold_vecs<ENT, T>(a, v, ks);
+            fold.template add_vecs<T>(v, ks);
           }
         } else {
           for (int j = tid; j < nv; j += S::kGroup) {
             const uint4 v[1] = {in[j]};
-            fold_vecs<ENT, T>(a, v, ks);
+            fold.template add_vecs<T>(v, ks);
           }
         }
         if (PASS == kForward || c < again) {
@@ -545,9 +545,9 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
       if (PASS == kFused) r.back(p.chunks - again);
       if (tid < edge) {
         const float f[1] = {as_float(p.x[edge_col])};
-        fold<ENT>(a, f, f[0], ks);
+        fold.add(f, f[0], ks);
       }
-      a = warp_merge(a, 32, ks);
+      const RowSum a = warp_merge(fold.sum(), 32, ks);
       if (it >= 2) wait_or_mark(&sh.part_empty[par], phase ^ 1, sh);
       if (lane == 0) {
         sh.part[par][warp] = a;

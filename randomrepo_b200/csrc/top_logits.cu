@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
       const int edge = rank == 0 ? A.vocab - p.nvec * VE : 0;
       const int per = (p.chunks + kTopGroups - 1) / kTopGroups, par = it & 1;
       if (it >= 2) wait_or_mark(&sh.row_empty[par], ((it >> 1) & 1) ^ 1, sh);
-      RowSum a{-INFINITY, 0.f, 0.f};
+      Fold<false> fold;
       float top = -INFINITY;
       for (int c = 0, in_group = 0, group = 0; c < p.chunks; ++c) {
         wait_or_mark(&sh.full[r.slot], r.phase, sh);
@@ -417,14 +417,14 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
           uint4 v[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) v[u] = in[at + ((u + turn) & 3)];
-          top = fmaxf(top, fold_vecs<false, T>(a, v, A.ks));
+          top = fmaxf(top, fold.template add_vecs<T>(v, A.ks));
         } else {
           const bool lone = lone_chunk<T>(p);
           for (int u = 0; u < 4; ++u) {
             const int j = lone ? tid + u * kTopThreads : at + u;
             if (j >= nv) break;
             const uint4 v[1] = {in[j]};
-            top = fmaxf(top, fold_vecs<false, T>(a, v, A.ks));
+            top = fmaxf(top, fold.template add_vecs<T>(v, A.ks));
           }
         }
         __syncwarp();
@@ -438,9 +438,9 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
       }
       if (tid < edge) {
         const float f[1] = {as_float(p.x[tid < p.head ? tid : tid + p.nvec * VE])};
-        fold<false>(a, f, f[0], A.ks);
+        fold.add(f, f[0], A.ks);
       }
-      a = warp_merge(a, 32, A.ks);
+      const RowSum a = warp_merge(fold.sum(), 32, A.ks);
       if (lane == 0) sh.sum[par][warp] = a;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.row_full[par]);
