@@ -260,13 +260,16 @@ struct TeacherRow {
 };
 
 // Measured on rows of 151 936 columns.  Sums or gradient alone: four CTAs of 128 threads that take 8 vectors at a time
-// (16-bit sums of 4 096 rows 227 us; 256 threads x 2 CTAs 238, 512 threads x 4 vectors x 1 CTA 275).  Both in one
-// launch: two CTAs an SM hide each other's turns between the passes, and a larger chunk its waits (499 us; one CTA of
-// 768 threads 494, of 512 threads with 2 vectors 580) -- but for float32, whose rows in flight would then overflow L2
-// before they are read again, one CTA (8 192 rows 1.85 ms against 2.23 ms).
+// (16-bit sums of 4 096 rows 213 us; before the sums' last change 227, where 256 threads x 2 CTAs took 238 and 512
+// threads x 4 vectors x 1 CTA 275).  Both in one launch, 16 bits: two CTAs an SM hide each other's turns between the
+// passes, and a larger chunk its waits (490 us; one CTA of 768 threads 494, 512 threads with 2 vectors 580); bound by
+// the two exponentials and their conversions a column as much as by HBM.  float32, half the exponentials a byte: one
+// CTA an SM, whose rows in flight stay in L2 until their second pass, a row to a pair of CTAs where even they would
+// not (8 192 rows 1.58 ms; without pairs 1.84, 512 threads in pairs 1.61, two CTAs an SM 2.23, four CTAs a row 3.56).
 template <typename T, int PASS> struct ShapeOf : Shape<128, 8, 3, 4> {};
 template <typename T> struct ShapeOf<T, kFused> : Shape<384, 4, 4, 2> {};
-template <> struct ShapeOf<float, kFused> : Shape<512, 4, 6, 1> {};
+template <> struct ShapeOf<float, kFused> : Shape<384, 4, 8, 1> {};
+constexpr int64_t kRowsInL2 = 64 << 20;  // bytes of rows in flight that come back from L2
 
 template <typename S>
 struct alignas(128) LossShared {
@@ -814,7 +817,9 @@ int32_t launch_typed(const LossArgs& a, cudaStream_t st) {
     if (dev < 64) ready[dev] = true;
   }
   const int64_t rows = (int64_t)a.batch * a.length;
-  const int c = row_cluster(rows, (int64_t)a.vocab * sizeof(T), sms * S::kCtas);
+  const int64_t row_bytes = (int64_t)a.vocab * sizeof(T);
+  int c = row_cluster(rows, row_bytes, sms * S::kCtas);
+  if (PASS == kFused && S::kCtas == 1 && c == 1 && rows > sms && sms * row_bytes > kRowsInL2) c = 2;
   const int grid = (int)std::min<int64_t>(rows, sms * S::kCtas / c) * c;
   return launch_after(kernel, grid, S::kThreads, c, kBytes, a, st, "loss rows launch");
 }
