@@ -231,11 +231,17 @@ __device__ __forceinline__ void grad_columns(float (&x)[N], const RowGrad& o, Sc
     }
     return;
   }
+  const f32x2 cc = pair(c, c), hi = pair(k.hi, k.hi), lo = pair(k.lo, k.lo), a = pair(o.a, o.a), b = pair(o.b, o.b);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float y = fmaf(x[i], k.hi, c);
-    if (sizeof(T) == 4) y = fmaf(x[i], k.lo, y);  // (half a step of 16 bits hides it)
-    x[i] = ex2(y) * (ENT ? fmaf(o.b, fmaxf(y, -1e30f), o.a) : o.a);
+  for (int i = 0; i < N; i += 2) {
+    const f32x2 xx = pair(x[i], i + 1 < N ? x[i + 1] : 0.f);
+    f32x2 y2 = fma2(xx, hi, cc);
+    if (sizeof(T) == 4) y2 = fma2(xx, lo, y2);  // (half a step of 16 bits hides it)
+    const float2 y = unpair(y2);
+    const f32x2 e = pair(ex2(y.x), ex2(y.y));
+    const float2 v = unpair(mul2(e, ENT ? fma2(b, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), a) : a));
+    x[i] = v.x;
+    if (i + 1 < N) x[i + 1] = v.y;
   }
 }
 
