@@ -65,32 +65,25 @@ struct RowSum {
   float m, s, w;
 };
 
-__device__ __forceinline__ void sum_rescale(RowSum& a, float m_new, Scale2 k) {
+// d: the exponent that takes sums from a reference m to another.
+__device__ __forceinline__ float rescale_exponent(float m, float m_new, Scale2 k) {
   const float c = center(m_new, k);
-  const float d = far_out(c) ? (a.m - m_new) * k.hi : c - center(a.m, k), f = ex2(d);
+  return far_out(c) ? (m - m_new) * k.hi : c - center(m, k);
+}
+
+__device__ __forceinline__ void sum_rescale(RowSum& a, float m_new, float d, float f) {
   a.w = f > 0.f ? f * fmaf(d, a.s, a.w) : 0.f;  // (a NaN stays in s)
   a.s *= f;
   a.m = m_new;
 }
 
-__device__ __forceinline__ void sum_merge(RowSum& a, RowSum b, Scale2 k) {
-  const float mn = fmaxf(a.m, b.m);
-  if (mn == -INFINITY) {
-    a.s += b.s;  // 0, or the NaN of a NaN column
-    return;
-  }
-  // (the larger one's factor is 2^0: exact)
-  sum_rescale(a, mn, k);
-  sum_rescale(b, mn, k);
-  a.s += b.s;
-  a.w += b.w;
-}
-
-// log2 of a positive float to about 1e-7 absolute: the exponent apart, so that a large sum costs no digits.
-__device__ __forceinline__ double log2_of(float s) {
+// log2 of a row's sum to about 1e-8: the exponent apart, so that a large sum costs no digits.  The approximate 2^y
+// behind the sum is 5e-8 of itself low on average (measured for y from -42 to -1/2; exact at y = 0, at least one
+// column's), which would add up in a sequence's log-probability: its share is put back.
+__device__ __forceinline__ double log2_sum(float s) {
   int e;
   const float f = frexpf(s, &e);
-  return (double)e + (double)log2f(f);
+  return (double)e + (double)log2f(f) + (double)(7.2e-8f * (1.f - 1.f / s));
 }
 
 // Columns [0, head) and [head + VE nvec, vocab) of a row are outside its 16-byte-aligned body.
@@ -200,6 +193,7 @@ __device__ __forceinline__ float top_of(const uint4 (&v)[N]) {
 
 // The running sums of a thread.  m is a column near the largest so far: as long as no column's 2^y passes 2^20 it
 // stays, so that the sums are rarely rescaled.  c is its center, +inf where there is none (no column yet, or far out).
+// The lanes of a warp that add whole chunks share their m: their sums then merge without the approximate 2^d.
 template <bool ENT>
 struct Fold {
   float m = -INFINITY, c = INFINITY;
@@ -210,17 +204,26 @@ struct Fold {
     return RowSum{m, t.x + t.y, ENT ? u.x + u.y : 0.f};
   }
 
-  // Add columns whose largest is `top`.
-  template <int N>
+  // Add columns whose largest is `top`.  WHOLE: all lanes of the warp do.
+  template <bool WHOLE, int N>
   __device__ __forceinline__ void add(const float (&x)[N], float top, Scale2 k) {
-    if (!(fmaf(top, k.hi, c) <= 20.f)) {
+    const bool passed = !(fmaf(top, k.hi, c) <= 20.f);
+    if (WHOLE ? __any_sync(0xffffffffu, passed) : passed) {
       RowSum a = sum();
+      if (WHOLE) {
+        top = fmaxf(top, m);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      }
       if (!(top > -INFINITY)) {  // nothing but -inf, or NaN
 #pragma unroll
         for (int i = 0; i < N; ++i)
           if (x[i] != x[i]) a.s = NAN;
       } else {
-        if (top > m) sum_rescale(a, top, k);
+        if (top > m) {
+          const float d = rescale_exponent(m, top, k);
+          sum_rescale(a, top, d, ex2(d));
+        }
         m = a.m;
         const float at = center(m, k);
         c = far_out(at) ? INFINITY : at;
@@ -258,14 +261,14 @@ struct Fold {
   }
 
   // Add N vectors of a row's body; their largest column.
-  template <typename T, int N>
+  template <bool WHOLE, typename T, int N>
   __device__ __forceinline__ float add_vecs(const uint4 (&v)[N], Scale2 k) {
     constexpr int VE = 16 / sizeof(T);
     float f[N * VE];
 #pragma unroll
     for (int i = 0; i < N; ++i) unpack<T>(v[i], *reinterpret_cast<float (*)[VE]>(f + i * VE));
     const float top = top_of<T>(v);
-    add(f, top, k);
+    add<WHOLE>(f, top, k);
     return top;
   }
 };
@@ -342,13 +345,18 @@ __device__ __forceinline__ double warp_sum_d(double v) {
   return v;
 }
 
+// The sums of `width` lanes (a power of two), on a common reference.  The factors are exact ones: the approximate 2^d is
+// 5e-8 low on average, and a row's sum passes here up to three times.
 __device__ __forceinline__ RowSum warp_merge(RowSum a, int width, Scale2 k) {
+  float m = a.m;
+  for (int off = width / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  if (a.m != m) {  // (no column anywhere: s is 0, or the NaN of a NaN column)
+    const float d = rescale_exponent(a.m, m, k);
+    sum_rescale(a, m, d, (float)exp2((double)d));
+  }
   for (int off = width / 2; off > 0; off >>= 1) {
-    RowSum b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, off);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, off);
-    b.w = __shfl_xor_sync(0xffffffffu, a.w, off);
-    sum_merge(a, b, k);
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, off);
+    a.w += __shfl_xor_sync(0xffffffffu, a.w, off);
   }
   return a;
 }

@@ -87,7 +87,7 @@ struct RowGrad {
 // log2 of a column's probability, in 64 bits.
 __device__ __forceinline__ double log2_prob(const LossArgs& A, const RowSum& r, float x) {
   const float c = center(r.m, A.ks);
-  return (far_out(c) ? ((double)x - (double)r.m) * A.kd : (double)x * A.kd + (double)c) - log2_of(r.s);
+  return (far_out(c) ? ((double)x - (double)r.m) * A.kd : (double)x * A.kd + (double)c) - log2_sum(r.s);
 }
 
 // A scored row's own inputs, loaded before its sums are made.
@@ -100,7 +100,7 @@ template <bool ENT>
 __device__ __forceinline__ RowGrad policy_tail(const LossArgs& A, int row, RowSum r, const RowTerms& q, bool write) {
   const int64_t tok = q.tok;
   const bool known = tok >= 0 && tok < A.vocab;
-  const double log2s = log2_of(r.s);
+  const double log2s = log2_sum(r.s);
   const double lp = known ? log2_prob(A, r, q.x_tok) * kLn2d : (double)NAN;
   const float w = q.w, adv = q.adv;
   const float ratio = A.old.p ? expf((float)(lp - (double)q.old)) : (lp == lp ? 1.f : NAN);
@@ -461,7 +461,7 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
         // sum q (log q - log p), log p = (x k + c - log2 s) ln 2
         const double w = (double)q.w, tt = (double)A.temperature;
         const float c = center(a.m, ks);
-        double qp = te.qx * A.kd + te.q_sum * ((double)c - log2_of(a.s));  // sum q log2 p
+        double qp = te.qx * A.kd + te.q_sum * ((double)c - log2_sum(a.s));  // sum q log2 p
         if (far_out(c) && qp == qp) {
           qp = 0.0;
           for (int f = 0; f < A.k; ++f)
@@ -537,12 +537,12 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
             uint4 v[kAtOnce];
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) v[u] = in[tid + (h + u) * S::kGroup];
-            fold.template add_vecs<T>(v, ks);
+            fold.template add_vecs<true, T>(v, ks);
           }
         } else {
           for (int j = tid; j < nv; j += S::kGroup) {
             const uint4 v[1] = {in[j]};
-            fold.template add_vecs<T>(v, ks);
+            fold.template add_vecs<false, T>(v, ks);
           }
         }
         if (PASS == kForward || c < again) {
@@ -554,7 +554,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
       if (PASS == kFused) r.back(p.chunks - again);
       if (tid < edge) {
         const float f[1] = {as_float(p.x[edge_col])};
-        fold.add(f, f[0], ks);
+        fold.template add<false>(f, f[0], ks);
       }
       const RowSum a = warp_merge(fold.sum(), 32, ks);
       if (it >= 2) wait_or_mark(&sh.part_empty[par], phase ^ 1, sh);

@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
     A.tokens[(int64_t)row * A.k + at] = bad ? -1 : (int64_t)(0xffffffffu - (uint32_t)key);
     if (at == 0) {
       const float c = center(a.m, A.ks);
-      A.lse[row] = bad ? NAN : (float)((log2_of(a.s) + (far_out(c) ? (double)a.m * A.kd : -(double)c)) * kLn2d);
+      A.lse[row] = bad ? NAN : (float)((log2_sum(a.s) + (far_out(c) ? (double)a.m * A.kd : -(double)c)) * kLn2d);
     }
   };
   if (warp == kTopWarps + kPickWarps) {
@@ -417,14 +417,14 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
           uint4 v[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) v[u] = in[at + ((u + turn) & 3)];
-          top = fmaxf(top, fold.template add_vecs<T>(v, A.ks));
+          top = fmaxf(top, fold.template add_vecs<true, T>(v, A.ks));
         } else {
           const bool lone = lone_chunk<T>(p);
           for (int u = 0; u < 4; ++u) {
             const int j = lone ? tid + u * kTopThreads : at + u;
             if (j >= nv) break;
             const uint4 v[1] = {in[j]};
-            top = fmaxf(top, fold.template add_vecs<T>(v, A.ks));
+            top = fmaxf(top, fold.template add_vecs<false, T>(v, A.ks));
           }
         }
         __syncwarp();
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
       }
       if (tid < edge) {
         const float f[1] = {as_float(p.x[tid < p.head ? tid : tid + p.nvec * VE])};
-        fold.add(f, f[0], A.ks);
+        fold.template add<false>(f, f[0], A.ks);
       }
       const RowSum a = warp_merge(fold.sum(), 32, A.ks);
       if (lane == 0) sh.sum[par][warp] = a;
@@ -450,8 +450,7 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
       const TopPart<T> p(A, row, rank, size);
       const int edge = rank == 0 ? A.vocab - p.nvec * VE : 0, par = it & 1;
       wait_or_mark(&sh.row_full[par], (it >> 1) & 1, sh);
-      RowSum all = sh.sum[par][0];
-      for (int i = 1; i < kTopWarps; ++i) sum_merge(all, sh.sum[par][i], A.ks);
+      const RowSum all = warp_merge(lane < kTopWarps ? sh.sum[par][lane] : RowSum{-INFINITY, 0.f, 0.f}, 32, A.ks);
       const int m = part_list<T>(p, edge, A.k, all.s == all.s, par, sh);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.row_empty[par]);
@@ -472,10 +471,9 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
   if (rank == 0) {
     __shared__ int s_n[kMaxCluster];
     uint64_t* lists = reinterpret_cast<uint64_t*>(dyn);  // (the ring is done)
-    RowSum all = sh.all;
+    const RowSum all = warp_merge(lane < size ? cluster_peer(&sh, lane)->all : RowSum{-INFINITY, 0.f, 0.f}, 32, A.ks);
     for (int q = 0; q < size; ++q) {
       const TopShared* peer = cluster_peer(&sh, q);
-      if (q > 0) sum_merge(all, peer->all, A.ks);
       if (tid == 0) s_n[q] = peer->best_n;
       for (int i = tid; i < peer->best_n; i += kTopCta) lists[q * PKV_MAX_TOP + i] = peer->best[i];
       if (tid == 0 && peer->gave_up) sh.gave_up = 1;
