@@ -670,7 +670,8 @@ int32_t pkv_spec_accept(const float* target_logits, const float* draft_logits, i
  * element strides batch_stride / row_stride, columns contiguous.  A row whose
  * mask byte is 0 is not scored: it is never read, its outputs are 0 and its
  * gradient row is zeros.  With `grad` non-NULL the loss call writes the
- * gradient of `loss` too (the logits' dtype, rows that do not overlap), each
+ * gradient of `loss` too (the logits' dtype, rows that overlap neither each
+ * other nor the logits), each
  * logits row crossing HBM once; without it the call leaves what a later
  * *_backward call needs in the workspace (keep it, and the logits, until
  * then), which multiplies by the device scalar *upstream.  Gradients of rows

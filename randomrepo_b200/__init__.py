@@ -15,10 +15,13 @@ Public API (drop-in for ``agentrl.generation.paged_kv``):
   decode path);
 * ``assign_groups`` / ``StepGather`` (``randomrepo_b200.sharding``): GRPO
   groups per GPU and the per-step gather of sampled tokens and logprobs;
+* ``policy_loss`` / ``preference_loss`` / ``distillation_loss`` (and their
+  ``*_and_grad`` forms) and ``top_logits`` (``randomrepo_b200.losses``):
+  training on rollouts, from rows of logits;
 * ``randomrepo_b200.ops``: the kernels as PyTorch operators
   (``torch.ops.pkv.kv_append`` / ``kv_gather`` / ``copy_blocks`` /
-  ``decode_attention`` / ``prefill_attention``, with fake-tensor shapes),
-  registered when that module is imported.
+  ``decode_attention`` / ``prefill_attention`` and the losses, with
+  fake-tensor shapes), registered when that module is imported.
 
 All device work runs in ``libpkv_b200.so`` (hand-written sm_100a kernels),
 built in-tree by ``python -m randomrepo_b200.build``.  The library is loaded
@@ -38,6 +41,13 @@ _EXPORTS = {
     "SamplingConfig": "hf",
     "StepGather": "sharding",
     "assign_groups": "sharding",
+    "policy_loss": "losses",
+    "policy_loss_and_grad": "losses",
+    "preference_loss": "losses",
+    "preference_loss_and_grad": "losses",
+    "distillation_loss": "losses",
+    "distillation_loss_and_grad": "losses",
+    "top_logits": "losses",
 }
 
 __all__ = sorted(_EXPORTS)

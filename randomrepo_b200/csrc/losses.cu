@@ -154,27 +154,38 @@ struct PlanArgs {
   int32_t* seq_n;
 };
 
+// One CTA: each thread has a run of rows, whose mask it reads once (into bits, 64 rows at a time, eight reads on their
+// way; latency is all there is to this kernel).
 __global__ void __launch_bounds__(1024) loss_plan_kernel(const PlanArgs A) {
-  __shared__ int s_warp[33], s_full, s_total;
+  __shared__ int s_warp[32], s_full, s_total;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int n = A.batch * A.length;
-  auto scored = [&](int b, int t) { return A.mask == nullptr || A.mask[b * A.mb + t * A.mt] != 0; };
+  const int per = (n + 1023) / 1024, r0 = min(n, tid * per), r1 = min(n, r0 + per);
+  for (int b = tid; b < A.batch; b += 1024) A.seq_n[b] = 0;
   if (tid == 0) s_full = 0;
-  __syncthreads();
-  for (int b = warp; b < A.batch; b += 32) {
-    int c = 0;
-    for (int t = lane; t < A.length; t += 32) c += scored(b, t);
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0) {
-      A.seq_n[b] = c;
-      if (c > 0) atomicAdd(&s_full, 1);
+  // 64 rows from r, as bits; b and t of row r go on to the row behind them.
+  auto bits_of = [&](int r, int& b, int& t) {
+    const int m = min(64, r1 - r);
+    uint64_t bits = 0;
+#pragma unroll 8
+    for (int k = 0; k < m; ++k) {
+      if (A.mask == nullptr || A.mask[b * A.mb + t * A.mt] != 0) bits |= 1ull << k;
+      if (++t == A.length) t = 0, ++b;
+    }
+    return bits;
+  };
+  const int b0 = r0 < r1 ? r0 / A.length : 0, t0 = r0 < r1 ? r0 - b0 * A.length : 0;
+  uint64_t first = 0;  // (the only bits of a run of 64 rows)
+  int mine = 0;
+  {
+    int b = b0, t = t0;
+    for (int r = r0; r < r1; r += 64) {
+      const uint64_t bits = bits_of(r, b, t);
+      if (r == r0) first = bits;
+      mine += __popcll(bits);
     }
   }
-  // Each thread's run of rows: count, exclusive scan, then their places.
-  const int per = (n + 1023) / 1024, r0 = min(n, tid * per), r1 = min(n, r0 + per);
-  int mine = 0;
-  for (int r = r0; r < r1; ++r) mine += scored(r / A.length, r % A.length);
   int incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -196,18 +207,43 @@ __global__ void __launch_bounds__(1024) loss_plan_kernel(const PlanArgs A) {
   __syncthreads();
   const int total = s_total;
   int at = s_warp[warp] + incl - mine, rest = total + r0 - at;
-  for (int r = r0; r < r1; ++r) {
-    if (scored(r / A.length, r % A.length))
-      A.list[at++] = r;
-    else
-      A.list[rest++] = r;
+  int b = b0, t = t0, seq = b0, in_seq = 0;
+  int mb = b0, mt = t0;  // the mask's own place, where it is read again
+  auto count = [&]() {
+    if (in_seq) atomicAdd(A.seq_n + seq, in_seq);
+  };
+  for (int r = r0; r < r1; r += 64) {
+    const uint64_t bits = per <= 64 ? first : bits_of(r, mb, mt);
+    const int m = min(64, r1 - r);
+    for (int k = 0; k < m; ++k) {
+      if (b != seq) {
+        count();
+        seq = b, in_seq = 0;
+      }
+      if (bits >> k & 1) {
+        A.list[at++] = r + k;
+        ++in_seq;
+      } else {
+        A.list[rest++] = r + k;
+      }
+      if (++t == A.length) t = 0, ++b;
+    }
   }
-  for (int b = tid; b < A.batch; b += 1024) {
-    const int c = A.seq_n[b];
+  if (r0 < r1) count();
+  __threadfence_block();
+  __syncthreads();
+  if (A.reduction == PKV_SEQUENCE_MEAN) {
+    int full = 0;
+    for (int q = tid; q < A.batch; q += 1024) full += __ldcg(A.seq_n + q) > 0;
+    if (full) atomicAdd(&s_full, full);
+    __syncthreads();
+  }
+  for (int q = tid; q < A.batch; q += 1024) {
+    const int c = __ldcg(A.seq_n + q);
     float w = A.scale;
     if (A.reduction == PKV_TOKEN_MEAN) w = (float)((double)A.scale / max(total, 1));
     if (A.reduction == PKV_SEQUENCE_MEAN) w = (float)((double)A.scale / ((double)max(c, 1) * max(s_full, 1)));
-    A.seq_w[b] = w;
+    A.seq_w[q] = w;
   }
   if (tid == 0) {
     A.hdr->n_active = total;
@@ -440,7 +476,7 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
       RowSum a = warp_merge(lane < S::kWarps ? sh.part[par][lane] : RowSum{-INFINITY, 0.f, 0.f}, 32, ks);
       if (lane == 0) mbar_arrive(&sh.part_empty[par]);
       if (size > 1) {
-        if (lane == 0) {
+        if (lane == 0 && !*(volatile int*)&sh.gave_up) {  // (a CTA that gave up leaves its peers to do so)
           mbar_arrive_expect_tx(&sh.peers[par], 16 * size);
           for (int c = 0; c < size; ++c)
             send_peer(&sh.peer[par][rank], &sh.peers[par], c, make_float4(a.m, a.s, a.w, 0.f));
@@ -700,7 +736,13 @@ __global__ void __launch_bounds__(ShapeOf<T, PASS>::kThreads, ShapeOf<T, PASS>::
   __syncwarp();
   __syncthreads();
   if (size > 1) cluster_sync_all();  // no CTA leaves while its peers may still send to it
-  if (tid == 0 && *(volatile int*)&sh.gave_up) atomicExch(&A.hdr->error, 1);
+  if (tid == 0 && *(volatile int*)&sh.gave_up) {
+    atomicExch(&A.hdr->error, 1);
+    if (PASS != kForward && first < n) {  // (a gradient without a loss has no other sign)
+      const int row = A.list[first], b = row / A.length;
+      put((T*)A.g + b * A.gb + (row - b * A.length) * A.gr, NAN);
+    }
+  }
   if (PASS != kBackward && KIND != kPreference) {
     // The last CTA adds the rows' losses, always in the same order.
     if (tid == 0) {
@@ -899,6 +941,12 @@ int32_t check_vocab_rows(const pkv_loss_rows* r, const char* who) {
       const int64_t span = (r->length - 1) * rs + r->vocab;
       if (rs < r->vocab || (r->batch > 1 && r->grad_batch_stride < span))
         return fail(PKV_ERR_ARG, w + ": gradient rows overlap");
+      auto extent = [&](int64_t bs, int64_t rst) {
+        return ((r->batch - 1) * (r->batch > 1 ? bs : 0) + (r->length - 1) * (r->length > 1 ? rst : 0) + r->vocab) * size;
+      };
+      const uintptr_t x0 = (uintptr_t)r->logits, g0 = (uintptr_t)r->grad;
+      if (g0 < x0 + extent(r->batch_stride, r->row_stride) && x0 < g0 + extent(r->grad_batch_stride, r->grad_row_stride))
+        return fail(PKV_ERR_ARG, w + ": the gradient overlaps the logits");
     }
   }
   return PKV_OK;

@@ -462,6 +462,27 @@ def test_calls_repeat_bit_for_bit_and_leave_inputs_alone(cuda_device):
     assert torch.equal(logits, before)
 
 
+@pytest.mark.parametrize("b,t", [(1, 1), (3, 700), (2000, 3), (1, 70000), (70000, 1), (37, 1901)])
+def test_weights_of_many_rows(cuda_device, b, t):
+    """The plan of the scored rows: every row in its place and every sequence's weight, for runs of rows of all lengths."""
+    from randomrepo_b200 import losses
+
+    g = torch.Generator().manual_seed(b + t)
+    logits = torch.randn(b, t, 8, generator=g).to(cuda_device)
+    mask = (torch.rand(b, t, generator=g) < 0.4).to(cuda_device)
+    mask[0, 0] = True
+    tokens = torch.randint(0, 8, (b, t), generator=g).to(cuda_device)
+    adv = torch.randn(b, t, generator=g).to(cuda_device)
+    for reduction in ("token_mean", "sequence_mean"):
+        got, grad = losses.policy_loss_and_grad(logits, tokens, adv, None, mask, reduction=reduction, scale=float(b * t))
+        w = _weights(mask, b, t, reduction, float(b * t), cuda_device)
+        p = torch.softmax(logits.double(), -1)
+        p.scatter_add_(-1, tokens.unsqueeze(-1), -torch.ones(b, t, 1, dtype=torch.float64, device=cuda_device))
+        want = p * (w * adv.double()).unsqueeze(-1)
+        torch.testing.assert_close(grad.double(), want, atol=1e-6 * float(w.max()) * 4, rtol=1e-5)
+        assert abs(float(got.loss) + float((w * adv.double()).sum())) <= 1e-6 * float((w * adv.double()).abs().sum())
+
+
 def test_capture_streams_and_two_calls_at_once(cuda_device):
     """A captured call replays on new inputs; two captured calls, and calls on two streams, do not share anything."""
     from randomrepo_b200 import losses

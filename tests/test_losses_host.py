@@ -73,8 +73,9 @@ def _rows(**kw):
 
 BAD_ROWS = [dict(batch=-1), dict(vocab=0), dict(dtype=7), dict(temperature=0.0), dict(temperature=math.inf),
             dict(temperature=math.nan), dict(logits=_Array(0, 5120, 512)), dict(logits=_Array(0x1002, 5120, 512)),
-            dict(logits=_Array(0x1000, -5120, 512)), dict(grad=_Array(0x2000, 5120, 511)),
-            dict(grad=_Array(0x2000, 5119, 512)), dict(grad=_Array(0x2001, 5120, 512))]
+            dict(logits=_Array(0x1000, -5120, 512)), dict(grad=_Array(0x20000, 5120, 511)), dict(grad=_Array(0x1000, 5120, 512)),
+            dict(grad=_Array(0x1000 + 2 * 5120 * 4 - 4, 5120, 512)),
+            dict(grad=_Array(0x20000, 5119, 512)), dict(grad=_Array(0x20001, 5120, 512))]
 
 
 @pytest.mark.parametrize("bad", BAD_ROWS)
