@@ -90,28 +90,35 @@ def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
     return logits.unsqueeze(0) if logits.dim() == 2 else logits
 
 
-def _rows_like(t: torch.Tensor, rows: torch.Size, dev: torch.device, dtype: torch.dtype, what: str, name: str,
-               broadcast: bool = False) -> torch.Tensor:
-    """A per-row input as [B, T] (``rows``) of ``dtype`` on ``dev`` (``broadcast``: [B] or [B, 1] too)."""
+def _rows_like(t: torch.Tensor, rows: torch.Size, dev: torch.device, dtype: torch.dtype, what: str,
+               name: str) -> torch.Tensor:
+    """A per-row input as [B, T] (``rows``) of ``dtype`` on ``dev`` ([T] for one sequence)."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{what}: {name} must be a tensor")
     if t.device != dev:
         raise ValueError(f"{what}: {name} must be on the logits' device")
     if t.shape != rows:
-        b, n = rows
-        if broadcast and t.dim() == 1 and t.shape[0] == b and (b != 1 or n == 1):
-            t = t.unsqueeze(1)
-        elif t.dim() == 1 and b == 1 and t.shape[0] in ((n, 1) if broadcast else (n,)):
+        if t.dim() == 1 and rows[0] == 1 and t.shape[0] == rows[1]:
             t = t.unsqueeze(0)
-        if t.shape != rows:
-            if not (broadcast and t.shape == (b, 1)):
-                raise ValueError(f"{what}: {name} must have one value per logits row, got {tuple(t.shape)}")
-            t = t.expand(b, n)
+        else:
+            raise ValueError(f"{what}: {name} must have one value per logits row, got {tuple(t.shape)}")
     if t.dtype != dtype:
         if dtype == torch.int64 and (t.is_floating_point() or t.dtype == torch.bool):
             raise ValueError(f"{what}: {name} must be integers")
         t = t.to(dtype)
     return t
+
+
+def _advantages(t: torch.Tensor, rows: torch.Size, dev: torch.device, what: str):
+    """Advantages [B, T], [B, 1] or [B] (one a sequence) as float32, and their pointer and strides."""
+    if isinstance(t, torch.Tensor) and t.shape != rows and t.device == dev and not (rows[0] == 1 and t.dim() == 1
+                                                                                and t.shape[0] == rows[1]):
+        if tuple(t.shape) not in ((rows[0],), (rows[0], 1)):
+            raise ValueError(f"{what}: advantages must be [batch, length] or [batch], got {tuple(t.shape)}")
+        t = t.to(torch.float32)
+        return t, (t.data_ptr(), t.stride(0), 0)
+    t = _rows_like(t, rows, dev, torch.float32, what, "advantages")
+    return t, _array(t)
 
 
 def _mask(mask: torch.Tensor | None, rows: torch.Size, dev: torch.device, what: str) -> torch.Tensor | None:
@@ -144,7 +151,7 @@ def _grad_like(x: torch.Tensor) -> torch.Tensor:
     b, n, v = x.shape
     dense = v * x.element_size() % 16 == 0 or (x.is_contiguous() and x.data_ptr() % 16 == 0)
     if dense or x.numel() == 0:
-        return torch.empty((b, n, v), dtype=x.dtype, device=x.device)
+        return torch.empty(b, n, v, dtype=x.dtype, device=x.device)  # (faster than a tuple of sizes)
     sb, sn = (x.stride(0) if b > 1 else 0), (x.stride(1) if n > 1 else 0)
     span = (n - 1) * sn + v
     if (n > 1 and sn < v) or (b > 1 and sb < span) or (b - 1) * sb + span > 2 * x.numel() + 64:
@@ -239,17 +246,16 @@ def _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_l
         raise ValueError(f"{what}: clip_low and clip_high must be >= 0")
     rows, dev = x.shape[:2], x.device
     tok = _rows_like(tokens, rows, dev, torch.int64, what, "tokens")
-    adv = _rows_like(advantages, rows, dev, torch.float32, what, "advantages", broadcast=True)
+    adv, adv_array = _advantages(advantages, rows, dev, what)
     old = None if old_logprobs is None else _rows_like(old_logprobs, rows, dev, torch.float32, what, "old_logprobs")
     ref = None if ref_logprobs is None else _rows_like(ref_logprobs, rows, dev, torch.float32, what, "ref_logprobs")
     m = _mask(mask, rows, dev, what)
-    terms = _POLICY.pack(*_array(tok), *_array(adv), *_array(old), *_array(ref), clip_low, clip_high, kl_coef,
+    terms = _POLICY.pack(*_array(tok), *adv_array, *_array(old), *_array(ref), clip_low, clip_high, kl_coef,
                          entropy_coef, _reduction(reduction, what), scale)
     c = _Call(x, m, temperature, terms, (tok, adv, old, ref, m), lib.pkv_policy_loss_backward, what)
-    shape = logits.shape[:-1]
-    outputs = (torch.empty((), dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.float32, device=dev),
-               None if ref is None else torch.empty(shape, dtype=torch.float32, device=dev),
-               torch.empty(shape, dtype=torch.float32, device=dev) if entropy_coef else None)
+    lp = torch.empty(*logits.shape[:-1], dtype=torch.float32, device=dev)
+    outputs = (lp.new_empty(()), lp, None if ref is None else torch.empty_like(lp),
+               torch.empty_like(lp) if entropy_coef else None)
     return c, outputs
 
 
@@ -303,8 +309,8 @@ def _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, lengt
     terms = _PREFERENCE.pack(*_array(tok), 0 if ref is None else ref.data_ptr(), beta, label_smoothing,
                              int(bool(length_normalised)), scale)
     c = _Call(x, m, 1.0, terms, (tok, ref, m), lib.pkv_preference_loss_backward, what)
-    new = lambda *s: torch.empty(s, dtype=torch.float32, device=x.device)  # noqa: E731
-    return c, (new(), new(x.shape[0]), new(x.shape[0] // 2))
+    sums = torch.empty(rows[0], dtype=torch.float32, device=dev)
+    return c, (sums.new_empty(()), sums, torch.empty(rows[0] // 2, dtype=torch.float32, device=dev))
 
 
 def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | None = None,
@@ -334,14 +340,14 @@ def preference_loss_and_grad(logits: torch.Tensor, tokens: torch.Tensor, mask: t
     return PreferenceLoss(*outputs), grad
 
 
-def _teacher_list(t: torch.Tensor, logits: torch.Tensor, dtype: torch.dtype, what: str, name: str) -> torch.Tensor:
-    """A teacher's list as [B, T, k] of ``dtype`` with contiguous entries."""
-    if not isinstance(t, torch.Tensor) or t.device != logits.device:
+def _teacher_list(t: torch.Tensor, lead: torch.Size, dev: torch.device, dtype: torch.dtype, what: str,
+                  name: str) -> torch.Tensor:
+    """A teacher's list [..., k] of the rows ``lead`` as [B, T, k] of ``dtype`` with contiguous entries."""
+    if not isinstance(t, torch.Tensor) or t.device != dev:
         raise ValueError(f"{what}: {name} must be on the logits' device")
     shape = t.shape
-    if len(shape) != logits.dim() or shape[:-1] != logits.shape[:-1] or not 1 <= shape[-1] <= _MAX_TOP:
-        raise ValueError(f"{what}: {name} must be {list(logits.shape[:-1])} + [k], k from 1 to {_MAX_TOP}, got "
-                         f"{tuple(shape)}")
+    if len(shape) != len(lead) + 1 or shape[:-1] != lead or not 1 <= shape[-1] <= _MAX_TOP:
+        raise ValueError(f"{what}: {name} must be {list(lead)} + [k], k from 1 to {_MAX_TOP}, got {tuple(shape)}")
     if t.dtype != dtype:
         if dtype == torch.int64 and (t.is_floating_point() or t.dtype == torch.bool):
             raise ValueError(f"{what}: {name} must be integers")
@@ -354,18 +360,18 @@ def _teacher_list(t: torch.Tensor, logits: torch.Tensor, dtype: torch.dtype, wha
 def _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale):
     what = "distillation_loss"
     x = _logits(logits, what)
-    ids = _teacher_list(teacher_ids, logits, torch.int64, what, "teacher_ids")
-    tl = _teacher_list(teacher_logits, logits, torch.float32, what, "teacher_logits")
+    lead, rows, dev = logits.shape[:-1], x.shape[:2], x.device
+    ids = _teacher_list(teacher_ids, lead, dev, torch.int64, what, "teacher_ids")
+    tl = _teacher_list(teacher_logits, lead, dev, torch.float32, what, "teacher_logits")
     if ids.shape != tl.shape:
         raise ValueError(f"{what}: teacher_ids and teacher_logits must have the same shape")
-    rows, dev = x.shape[:2], x.device
     lse = None if teacher_lse is None else _rows_like(teacher_lse, rows, dev, torch.float32, what, "teacher_lse")
     m = _mask(mask, rows, dev, what)
     terms = _DISTILLATION.pack(*_array(ids), *_array(tl), ids.shape[-1], *_array(lse), _reduction(reduction, what),
                                scale)
     c = _Call(x, m, temperature, terms, (ids, tl, lse, m), lib.pkv_distillation_loss_backward, what)
-    return c, (torch.empty((), dtype=torch.float32, device=x.device),
-               torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device))
+    kl = torch.empty(*lead, dtype=torch.float32, device=dev)
+    return c, (kl.new_empty(()), kl)
 
 
 def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
@@ -411,9 +417,9 @@ def top_logits(logits: torch.Tensor, k: int, *,
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError(f"{what}: the temperature must lie in [1e-6, 1e6]")
     shape = logits.shape[:-1]
-    values = torch.empty((*shape, k), dtype=torch.float32, device=x.device)
-    tokens = torch.empty((*shape, k), dtype=torch.int64, device=x.device)
-    lse = torch.empty(shape, dtype=torch.float32, device=x.device)
+    values = torch.empty(*shape, k, dtype=torch.float32, device=x.device)
+    tokens = torch.empty(*shape, k, dtype=torch.int64, device=x.device)
+    lse = torch.empty(*shape, dtype=torch.float32, device=x.device)
     rows = _ROWS.pack(*_array(x), *_NONE, *_NONE, *x.shape, _DTYPES[x.dtype], temperature)
     _on_device(x, lib.pkv_top_logits, rows, k, values.data_ptr(), tokens.data_ptr(), lse.data_ptr())
     return values, tokens, lse
