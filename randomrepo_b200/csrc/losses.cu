@@ -339,14 +339,14 @@ __device__ __forceinline__ void send_peer(void* dst, uint64_t* bar, uint32_t ran
 // The copying warp (one lane of it).
 template <typename T, int PASS, typename S, typename Sh>
 __device__ __forceinline__ void copy_rows(const LossArgs& A, Sh& sh, uint4* slots, int rank, int size, int first,
-                                          int step, int n_active) {
+                                          int step, int n_active, int row0) {
   Ring<S::kSlots> r;
   int filled = 0;
   // Chunks read twice are asked to stay in L2 until then; the others leave it first.
   uint64_t keep_policy;
   asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep_policy));
   const uint64_t once_policy = l2_evict_first_policy();
-  int row = first < n_active ? A.list[first] : 0;
+  int row = row0;
   for (int i = first; i < n_active; i += step) {
     const RowPart<T, S::kChunk> p(A, row, rank, size);
     if (i + step < n_active) row = A.list[i + step];
@@ -375,10 +375,10 @@ __device__ __forceinline__ void copy_rows(const LossArgs& A, Sh& sh, uint4* slot
 // The teacher's warp: q and its sums, a row or two ahead.
 template <typename T, int PASS, typename S, typename Sh>
 __device__ __forceinline__ void teacher_rows(const LossArgs& A, Sh& sh, int rank, int size, int first, int step,
-                                             int n_active, int lane) {
+                                             int n_active, int row0, int lane) {
   int it = 0;
   for (int i = first; i < n_active; i += step, ++it) {
-    const RowPart<T, S::kChunk> p(A, A.list[i], rank, size);
+    const RowPart<T, S::kChunk> p(A, it ? A.list[i] : row0, rank, size);
     TeacherRow& o = sh.teacher[it & 1];
     if (it >= 2) wait_or_mark(&sh.teacher_empty[it & 1], ((it >> 1) & 1) ^ 1, sh);
     constexpr int kPer = PKV_MAX_TOP / 32;
@@ -437,11 +437,11 @@ __device__ __forceinline__ void teacher_rows(const LossArgs& A, Sh& sh, int rank
 // coefficients (in the backward pass, those the forward pass left).
 template <typename T, int KIND, bool ENT, int PASS, typename S, typename Sh>
 __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, int size, int first, int step,
-                                          int n_active, int n, int lane) {
+                                          int n_active, int n, int row0, int lane) {
   const bool write = lane == 0 && rank == 0;
   const Scale2 ks = A.ks;
   const float up = A.upstream ? *A.upstream : 1.f;
-  int row_next = first < n_active ? A.list[first] : 0;
+  int row_next = row0;
   int64_t tok_next = 0;
   if (KIND != kDistill && first < n_active) tok_next = A.tokens.at(row_next / A.length, row_next % A.length);
   for (int i = first, it = 0; i < n_active; i += step, ++it) {
@@ -543,13 +543,13 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
 // The warps that work on the columns: a row's sums, then its gradient.
 template <typename T, int KIND, bool ENT, int PASS, typename S, typename Sh>
 __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uint4* slots, int rank, int size,
-                                            int first, int step, int n_active, int n, int tid) {
+                                            int first, int step, int n_active, int n, int row0, int tid) {
   constexpr int VE = 16 / sizeof(T);
   const int lane = tid & 31, warp = tid >> 5;
   const Scale2 ks = A.ks;
   Ring<S::kSlots> r;
   const int end = PASS == kForward ? n_active : n;
-  int row = first < end ? A.list[first] : 0;
+  int row = row0;
   for (int i = first, it = 0; i < end; i += step) {
     const RowPart<T, S::kChunk> p(A, row, rank, size);
     if (i + step < end) row = A.list[i + step];
@@ -722,16 +722,18 @@ __global__ void __launch_bounds__(ShapeOf<T, PASS>::kThreads, ShapeOf<T, PASS>::
   __syncthreads();
   if (size > 1) cluster_sync_all();
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int n = A.batch * A.length, n_active = A.hdr->n_active;
-  const int first = blockIdx.x / size, step = gridDim.x / size;
+  if (PASS != kBackward) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int n = A.batch * A.length, first = blockIdx.x / size, step = gridDim.x / size;
+  const int row0 = first < n ? A.list[first] : 0;  // (on its way beside the count)
+  const int n_active = A.hdr->n_active;
   if (warp == S::kCopyWarp) {
-    if (lane == 0) copy_rows<T, PASS, S>(A, sh, slots, rank, size, first, step, n_active);
+    if (lane == 0) copy_rows<T, PASS, S>(A, sh, slots, rank, size, first, step, n_active, row0);
   } else if (warp == S::kTeacherWarp) {
-    if (KIND == kDistill) teacher_rows<T, PASS, S>(A, sh, rank, size, first, step, n_active, lane);
+    if (KIND == kDistill) teacher_rows<T, PASS, S>(A, sh, rank, size, first, step, n_active, row0, lane);
   } else if (warp == S::kTermsWarp) {
-    term_rows<T, KIND, ENT, PASS, S>(A, sh, rank, size, first, step, n_active, n, lane);
+    term_rows<T, KIND, ENT, PASS, S>(A, sh, rank, size, first, step, n_active, n, row0, lane);
   } else {
-    column_rows<T, KIND, ENT, PASS, S>(A, sh, slots, rank, size, first, step, n_active, n, tid);
+    column_rows<T, KIND, ENT, PASS, S>(A, sh, slots, rank, size, first, step, n_active, n, row0, tid);
   }
   __syncwarp();
   __syncthreads();
@@ -753,7 +755,7 @@ __global__ void __launch_bounds__(ShapeOf<T, PASS>::kThreads, ShapeOf<T, PASS>::
     if (sh.last) {
       __threadfence();
       double sum = 0.0;
-      for (int i = tid; i < n_active; i += S::kThreads) sum += __ldcg(A.row_val + A.list[i]);
+      for (int i = tid; i < n; i += S::kThreads) sum += __ldcg(A.row_val + i);  // (0 where a row is not scored)
       sum = warp_sum_d(sum);
       if (lane == 0) sh.sum[warp] = sum;
       __syncthreads();
@@ -783,6 +785,8 @@ struct PairArgs {
 __global__ void __launch_bounds__(1024) loss_pair_kernel(const PairArgs A) {
   __shared__ double s_d[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int b = warp; b < A.batch; b += 32) {
     double sum = 0.0;
     for (int t = lane; t < A.length; t += 32)
@@ -1021,8 +1025,7 @@ extern "C" int32_t pkv_preference_loss(const pkv_loss_rows* r, const pkv_prefere
              p->ref_logprobs, p->beta, p->label_smoothing, p->scale,
              reinterpret_cast<const double*>(ws + l.row_val), reinterpret_cast<const int32_t*>(ws + l.seq_n),
              reinterpret_cast<double*>(ws + l.seq_sum), reinterpret_cast<float*>(ws + l.seq_g), logprobs, margins, loss};
-  loss_pair_kernel<<<1, 1024, 0, s>>>(q);
-  if ((st = cuda_status("preference pairs launch")) != PKV_OK) return st;
+  if ((st = launch_after(loss_pair_kernel, 1, 1024, 1, 0, q, s, "preference pairs launch")) != PKV_OK) return st;
   if (!r->grad || empty_rows(r)) return PKV_OK;
   a.seq_g = q.seq_g;
   return launch_rows<kPreference, false, kBackward>(a, r->dtype, s);
