@@ -100,33 +100,42 @@ __device__ __forceinline__ void pick_range(float& lo, float& hi, int& n, TopShar
 template <typename T>
 using TopPart = RowPart<T, TopShape::kChunk>;
 
+// log2 of the chunks that a group of the part spans.
+template <typename T>
+__device__ __forceinline__ int group_shift(const TopPart<T>& p) {
+  const int per = (p.chunks + kTopGroups - 1) / kTopGroups;
+  return per > 1 ? 32 - __clz(per - 1) : 0;
+}
+
 // A part of less than a chunk: its vectors go round the threads, so that there are more groups.
 template <typename T>
 __device__ __forceinline__ bool lone_chunk(const TopPart<T>& p) { return p.nv < TopShape::kChunk; }
 
 // f(column, value) for the columns of vector at(i) (< 0: none) of the CTA's part, i = pick_id(), + kPickThreads, ...
-// below n, where the vector's largest value is not below `from` (NaN: all of them).  Four vectors are on their way at once (f's writes would keep a loop's loads apart).
-template <typename T, typename At, typename F>
+// below n, where the vector's largest value is not below `from` (NaN: all of them).  BATCH vectors are on their way at
+// once (f's writes would keep a loop's loads apart).
+template <typename T, int BATCH, typename At, typename F>
 __device__ __forceinline__ void vectors(const TopPart<T>& p, int n, At at, float from, F f) {
-  constexpr int VE = RowSplit<T>::VE, kBatch = 4;
-  for (int i0 = pick_id(); i0 < n; i0 += kBatch * kPickThreads) {
-    uint4 v[kBatch];
-    int j[kBatch];
+  constexpr int VE = RowSplit<T>::VE;
+  for (int i0 = pick_id(); i0 < n; i0 += BATCH * kPickThreads) {
+    uint4 v[BATCH];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * kPickThreads;
-      j[u] = i < n ? at(i) : -1;
-      if (j[u] >= 0) v[u] = p.body()[j[u]];
+    for (int u = 0; u < BATCH; ++u) {
+      const int i = i0 + u * kPickThreads, j = i < n ? at(i) : -1;
+      v[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (j >= 0) v[u] = p.body()[j];
     }
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      if (j[u] < 0) continue;
+    for (int u = 0; u < BATCH; ++u) {
       const uint4 one[1] = {v[u]};
-      if (top_of<T>(one) < from) continue;
+      const int i = i0 + u * kPickThreads;
+      if (i >= n || top_of<T>(one) < from) continue;
+      const int j = at(i);
+      if (j < 0) continue;
       float x[VE];
       unpack<T>(v[u], x);
 #pragma unroll
-      for (int q = 0; q < VE; ++q) f(p.head + (p.v0 + j[u]) * VE + q, x[q]);
+      for (int q = 0; q < VE; ++q) f(p.head + (p.v0 + j) * VE + q, x[q]);
     }
   }
 }
@@ -141,7 +150,7 @@ __device__ __forceinline__ void edge_column(const TopPart<T>& p, int edge, F f) 
 // f(column, value) for every column of the CTA's part of the row, in no order.
 template <typename T, typename F>
 __device__ __forceinline__ void each_column(const TopPart<T>& p, int edge, F f) {
-  vectors<T>(p, p.nv, [](int i) { return i; }, NAN, f);
+  vectors<T, 4>(p, p.nv, [](int i) { return i; }, NAN, f);
   edge_column<T>(p, edge, f);
 }
 
@@ -201,8 +210,7 @@ __device__ __forceinline__ int part_list(const TopPart<T>& p, int edge, int k, b
     pick_sync();
     return 0;
   }
-  const int per = (p.chunks + kTopGroups - 1) / kTopGroups;  // chunks a group spans
-  const int groups = per ? (p.chunks + per - 1) / per : 0;
+  const int shift = group_shift<T>(p), groups = (p.chunks + (1 << shift) - 1) >> shift;
   uint32_t low = 0;
   int m = kTopCap + 1;
   if (plain) {
@@ -222,7 +230,7 @@ __device__ __forceinline__ int part_list(const TopPart<T>& p, int edge, int k, b
       }
     };
     static_assert(kReads * 4 * kPickThreads == kTopGroups * kTopThreads, "whole reads");
-    const int subs = groups > 2 && k <= kPickThreads ? 1 : 4;  // (one value a thread, or four)
+    const int subs = groups * kTopThreads / 4 >= kPickThreads && k <= kPickThreads ? 1 : 4;  // (values a thread)
     float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (also what a group notes where it has no column)
     each_top([&](float t, int g) { best[g & 3] = fmaxf(best[g & 3], t); });
     float hi = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
@@ -278,23 +286,38 @@ __device__ __forceinline__ int part_list(const TopPart<T>& p, int edge, int k, b
     if (tid == 0) sh.count = sh.n_hits = 0;
     pick_sync();
     low = ordered(from);
-    each_top([&](float t, int g) {
-      if (t < from) return;
-      const int at = atomicAdd(&sh.n_hits, 1);
-      if (at < kTopCap) sh.hits[at] = (uint16_t)g;
-    });
+    // The groups that reach it: their number first, so that a warp takes its places at once.
+    int n_mine = 0;
+    each_top([&](float t, int) { n_mine += t >= from; });
+    int place = n_mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, place, off);
+      if (lane >= off) place += o;
+    }
+    int base = 0;
+    if (lane == 31) base = atomicAdd(&sh.n_hits, place);
+    place += __shfl_sync(0xffffffffu, base, 31) - n_mine;
+    if (n_mine)
+      each_top([&](float t, int g) {
+        if (t < from) return;
+        if (place < kTopCap) sh.hits[place] = (uint16_t)g;
+        ++place;
+      });
     auto look = [&](int c, float v) { take(c, v, low, sh); };
     edge_column<T>(p, edge, look);
     pick_sync();
     // All threads share the hit groups' vectors.
-    const int hits = sh.n_hits, vecs = per * TopShape::kVecs;
+    constexpr int kLogVecs = 2;
+    static_assert(TopShape::kVecs == 1 << kLogVecs, "a thread's vectors");
+    const int hits = sh.n_hits, log_vecs = shift + kLogVecs;
     const bool lone = lone_chunk<T>(p);
     if (hits <= kTopCap) {
-      vectors<T>(p, hits * vecs, [&](int i) {
-        const int hit = i / vecs, u = i - hit * vecs, group = sh.hits[hit];
-        const int j = lone ? group + u * kTopThreads
-                           : (group / kTopThreads * per + u / TopShape::kVecs) * TopShape::kChunk +
-                                 group % kTopThreads * TopShape::kVecs + u % TopShape::kVecs;
+      vectors<T, 8>(p, hits << log_vecs, [&](int i) {
+        const int group = sh.hits[i >> log_vecs], u = i & ((1 << log_vecs) - 1);
+        const int chunk = (group / kTopThreads << shift) + (u >> kLogVecs), t = group % kTopThreads;
+        const int j = lone ? t + u * kTopThreads
+                           : chunk * TopShape::kChunk + t * TopShape::kVecs + (u & (TopShape::kVecs - 1));
         return j < p.nv ? j : -1;
       }, from, look);
       pick_sync();
@@ -401,7 +424,7 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
     for (int row = first, it = 0; row < n; row += step, ++it) {
       const TopPart<T> p(A, row, rank, size);
       const int edge = rank == 0 ? A.vocab - p.nvec * VE : 0;
-      const int per = (p.chunks + kTopGroups - 1) / kTopGroups, par = it & 1;
+      const int per = 1 << group_shift<T>(p), par = it & 1;
       if (it >= 2) wait_or_mark(&sh.row_empty[par], ((it >> 1) & 1) ^ 1, sh);
       Fold<false> fold;
       float top = -INFINITY;
@@ -411,16 +434,16 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
         const int nv = min(TopShape::kChunk, p.nv - c * TopShape::kChunk);
         // A thread's vectors lie together, so that a group is 64 bytes of a chunk; each pair of threads starts at
         // another of them, which keeps the reads off each other's banks.
-        static_assert(TopShape::kVecs == 4, "the turn below");
-        const int at = tid * 4, turn = tid >> 1;
+        constexpr int kVecs = TopShape::kVecs;
+        const int at = tid * kVecs, turn = tid >> 1;
         if (nv == TopShape::kChunk) {
-          uint4 v[4];
+          uint4 v[kVecs];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) v[u] = in[at + ((u + turn) & 3)];
+          for (int u = 0; u < kVecs; ++u) v[u] = in[at + ((u + turn) & (kVecs - 1))];
           top = fmaxf(top, fold.template add_vecs<true, T>(v, A.ks));
         } else {
           const bool lone = lone_chunk<T>(p);
-          for (int u = 0; u < 4; ++u) {
+          for (int u = 0; u < kVecs; ++u) {
             const int j = lone ? tid + u * kTopThreads : at + u;
             if (j >= nv) break;
             const uint4 v[1] = {in[j]};
