@@ -294,12 +294,15 @@ __device__ __forceinline__ float teacher_logit(const LossArgs& A, int b, int t, 
   return id < 0 ? -INFINITY : v;  // an absent entry
 }
 
-// A row's teacher list as its warp leaves it for the others.
+// A row's teacher list as its warp leaves it for the others (X: with the columns' logits).
+template <bool X>
 struct TeacherRow {
   double q_sum, qx, qlogq; // sums over the list of q, q x[id] and q log q (a NaN: an id past the vocabulary)
-  int32_t id[PKV_MAX_TOP]; // -1: not a column
-  float q[PKV_MAX_TOP];
+  int32_t id[PKV_MAX_TOP]; // -1: not a column, or one that an entry before has
+  float q[PKV_MAX_TOP];    // the column's share, of all its entries
+  float x[X ? PKV_MAX_TOP : 1];
 };
+constexpr int kIdTable = 2 * PKV_MAX_TOP;
 
 // Measured on rows of 151 936 columns.  Sums or gradient alone: four CTAs of 128 threads that take 8 vectors at a time
 // (16-bit sums of 4 096 rows 213 us; before the sums' last change 227, where 256 threads x 2 CTAs took 238 and 512
@@ -309,11 +312,11 @@ struct TeacherRow {
 // CTA an SM, whose rows in flight stay in L2 until their second pass, a row to a pair of CTAs where even they would
 // not (8 192 rows 1.58 ms; without pairs 1.84, 512 threads in pairs 1.61, two CTAs an SM 2.23, four CTAs a row 3.56).
 template <typename T, int PASS> struct ShapeOf : Shape<128, 8, 3, 4> {};
-template <typename T> struct ShapeOf<T, kFused> : Shape<384, 4, 4, 2> {};
-template <> struct ShapeOf<float, kFused> : Shape<384, 4, 8, 1> {};
+template <typename T> struct ShapeOf<T, kFused> : Shape<640, 4, 5, 1> {};
+template <> struct ShapeOf<float, kFused> : Shape<512, 4, 6, 1> {};
 constexpr int64_t kRowsInL2 = 64 << 20;  // bytes of rows in flight that come back from L2
 
-template <typename S>
+template <typename S, bool X>
 struct alignas(128) LossShared {
   uint64_t full[S::kSlots], empty[S::kSlots];
   uint64_t part_full[2], part_empty[2], grad_full[2], grad_empty[2], teacher_full[2], teacher_empty[2], peers[2];
@@ -323,7 +326,8 @@ struct alignas(128) LossShared {
   float grad_wt[2];
   double sum[32];
   int last, gave_up;
-  TeacherRow teacher[2];
+  TeacherRow<X> teacher[2];
+  int32_t ids[kIdTable];  // the ids of a list, by their hash
 };
 
 // 16 bytes into the same shared-memory place of CTA `rank` of the cluster, counted on its barrier.
@@ -336,6 +340,17 @@ __device__ __forceinline__ void send_peer(void* dst, uint64_t* bar, uint32_t ran
                : "memory");
 }
 
+// The order of copies, which the column warps follow.  Sums or gradient alone: a row's chunks in turn.  Both: a row's
+// chunks for its sums, then the first chunk of the row behind it (whose sums begin while this row's coefficients are
+// made), then the chunks that did not stay in the ring, again, for its gradient.  The last kSlots - 1 chunks stay; a
+// slot's next copy waits for that slot alone, so chunks are freed in any order.
+
+// How many chunks of a row are copied twice.
+template <int PASS, typename S>
+__device__ __forceinline__ int chunks_again(int chunks) {
+  return PASS == kFused ? chunks - min(chunks, S::kSlots - 1) : 0;
+}
+
 // The copying warp (one lane of it).
 template <typename T, int PASS, typename S, typename Sh>
 __device__ __forceinline__ void copy_rows(const LossArgs& A, Sh& sh, uint4* slots, int rank, int size, int first,
@@ -346,29 +361,39 @@ __device__ __forceinline__ void copy_rows(const LossArgs& A, Sh& sh, uint4* slot
   uint64_t keep_policy;
   asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep_policy));
   const uint64_t once_policy = l2_evict_first_policy();
+  // False: a wait gave up.
+  auto copy = [&](const RowPart<T, S::kChunk>& p, int at, bool keep) {
+    if (filled == S::kSlots)
+      wait_or_mark(&sh.empty[r.slot], r.phase ^ 1, sh);
+    else
+      ++filled;
+    if (*(volatile int*)&sh.gave_up) {
+      // Copies still in flight end before the CTA's shared memory goes.
+      for (int k = 0; k < S::kSlots; ++k)
+        if (k < r.slot || filled == S::kSlots) mbar_wait_bounded(&sh.full[k], k < r.slot ? r.phase : r.phase ^ 1);
+      return false;
+    }
+    const int nv = min(S::kChunk, p.nv - at * S::kChunk);
+    mbar_arrive_expect_tx(&sh.full[r.slot], nv * 16);
+    bulk_copy_g2s_hint(slots + r.slot * S::kChunk, p.body() + at * S::kChunk, nv * 16, &sh.full[r.slot],
+                       keep ? keep_policy : once_policy);
+    r.next();
+    return true;
+  };
   int row = row0;
   for (int i = first; i < n_active; i += step) {
     const RowPart<T, S::kChunk> p(A, row, rank, size);
     if (i + step < n_active) row = A.list[i + step];
-    const int again = PASS == kFused ? p.chunks - min(p.chunks, S::kSlots) : 0;
-    for (int c = 0; c < p.chunks + again; ++c) {
-      const int at = c < p.chunks ? c : c - p.chunks;
-      if (filled == S::kSlots)
-        wait_or_mark(&sh.empty[r.slot], r.phase ^ 1, sh);
-      else
-        ++filled;
-      if (*(volatile int*)&sh.gave_up) {
-        // Copies still in flight end before the CTA's shared memory goes.
-        for (int k = 0; k < S::kSlots; ++k)
-          if (k < r.slot || filled == S::kSlots) mbar_wait_bounded(&sh.full[k], k < r.slot ? r.phase : r.phase ^ 1);
-        return;
-      }
-      const int nv = min(S::kChunk, p.nv - at * S::kChunk);
-      mbar_arrive_expect_tx(&sh.full[r.slot], nv * 16);
-      bulk_copy_g2s_hint(slots + r.slot * S::kChunk, p.body() + at * S::kChunk, nv * 16, &sh.full[r.slot],
-                         c < again ? keep_policy : once_policy);
-      r.next();
+    const int again = chunks_again<PASS, S>(p.chunks);
+    for (int c = PASS == kFused && i != first ? 1 : 0; c < p.chunks; ++c)
+      if (!copy(p, c, c < again)) return;
+    if (PASS != kFused) continue;
+    if (i + step < n_active) {
+      const RowPart<T, S::kChunk> next(A, row, rank, size);
+      if (next.chunks && !copy(next, 0, chunks_again<PASS, S>(next.chunks) > 0)) return;
     }
+    for (int c = 0; c < again; ++c)
+      if (!copy(p, c, false)) return;
   }
 }
 
@@ -379,24 +404,43 @@ __device__ __forceinline__ void teacher_rows(const LossArgs& A, Sh& sh, int rank
   int it = 0;
   for (int i = first; i < n_active; i += step, ++it) {
     const RowPart<T, S::kChunk> p(A, it ? A.list[i] : row0, rank, size);
-    TeacherRow& o = sh.teacher[it & 1];
+    auto& o = sh.teacher[it & 1];
     if (it >= 2) wait_or_mark(&sh.teacher_empty[it & 1], ((it >> 1) & 1) ^ 1, sh);
     constexpr int kPer = PKV_MAX_TOP / 32;
     float v[kPer], x[kPer];
+    int ids[kPer];
     float top = -INFINITY;
+    for (int j = lane; j < kIdTable; j += 32) sh.ids[j] = -1;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       const int j = lane + 32 * e;
-      v[e] = -INFINITY, x[e] = 0.f;
+      v[e] = -INFINITY, x[e] = 0.f, ids[e] = -1;
       if (j < A.k) {
         int64_t id;
         v[e] = teacher_logit(A, p.b, p.t, j, id);
-        const bool column = id >= 0 && id < A.vocab;
-        if (PASS != kBackward && v[e] != -INFINITY) x[e] = column ? as_float(p.x[id]) : NAN;
-        o.id[j] = column ? (int32_t)id : -1;
+        if (id >= 0 && id < A.vocab)
+          ids[e] = (int)id, x[e] = PASS == kBackward ? 0.f : as_float(p.x[id]);
+        else if (v[e] != -INFINITY)
+          x[e] = NAN;
         top = fmaxf(top, v[e]);
       }
     }
+    // Does an id come twice?  (A column is written once, with all its shares; lists hardly ever need that.)
+    __syncwarp();
+    bool twice = false;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (32 * e >= A.k || ids[e] < 0) continue;
+      for (int at = ids[e] & (kIdTable - 1);; at = (at + 1) & (kIdTable - 1)) {
+        const int there = atomicCAS(&sh.ids[at], -1, ids[e]);
+        if (there == -1) break;
+        if (there == ids[e]) {
+          twice = true;
+          break;
+        }
+      }
+    }
+    twice = __any_sync(0xffffffffu, twice);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     // The norm in 64 bits: log q would lose digits to a rounded one.
@@ -424,7 +468,29 @@ __device__ __forceinline__ void teacher_rows(const LossArgs& A, Sh& sh, int rank
           ql += (double)q * lq;
         }
       }
-      if (j < A.k) o.q[j] = q;
+      if (j < A.k) {
+        o.q[j] = q, o.id[j] = ids[e];
+        if (PASS == kFused) o.x[j] = x[e];
+      }
+    }
+    if (twice) {
+      __syncwarp();
+      float all[kPer];
+      bool later[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int j = lane + 32 * e;
+        all[e] = 0.f, later[e] = false;
+        if (j >= A.k) continue;
+        for (int f = 0; f < A.k; ++f)
+          if (o.id[f] == ids[e]) all[e] += o.q[f], later[e] |= f < j;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int j = lane + 32 * e;
+        if (j < A.k) o.q[j] = all[e], o.id[j] = later[e] ? -1 : ids[e];
+      }
     }
     qs = warp_sum_d(qs), qx = warp_sum_d(qx), ql = warp_sum_d(ql);
     if (lane == 0) o.q_sum = qs, o.qx = qx, o.qlogq = ql;
@@ -493,7 +559,7 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
         if (write) A.row_val[row] = known ? log2_prob(A, a, q.x_tok) * kLn2d : (double)NAN;
       } else {
         wait_or_mark(&sh.teacher_full[par], phase, sh);
-        const TeacherRow& te = sh.teacher[par];
+        const auto& te = sh.teacher[par];
         // sum q (log q - log p), log p = (x k + c - log2 s) ln 2
         const double w = (double)q.w, tt = (double)A.temperature;
         const float c = center(a.m, ks);
@@ -547,8 +613,37 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
   constexpr int VE = 16 / sizeof(T);
   const int lane = tid & 31, warp = tid >> 5;
   const Scale2 ks = A.ks;
-  Ring<S::kSlots> r;
+  Ring<S::kSlots> r, zero;  // the next copy; the row's first chunk
   const int end = PASS == kForward ? n_active : n;
+  // Chunk c of a row, at r, into its sums.
+  auto sum_chunk = [&](Fold<ENT>& fold, const RowPart<T, S::kChunk>& p, int c, bool done) {
+    wait_or_mark(&sh.full[r.slot], r.phase, sh);
+    const uint4* in = slots + r.slot * S::kChunk;
+    const int nv = min(S::kChunk, p.nv - c * S::kChunk);
+    if (nv == S::kChunk) {
+      constexpr int kAtOnce = 4;
+      static_assert(S::kVecs % kAtOnce == 0, "vectors are taken four at a time");
+#pragma unroll
+      for (int h = 0; h < S::kVecs; h += kAtOnce) {
+        uint4 v[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) v[u] = in[tid + (h + u) * S::kGroup];
+        fold.template add_vecs<true, T>(v, ks);
+      }
+    } else {
+      for (int j = tid; j < nv; j += S::kGroup) {
+        const uint4 v[1] = {in[j]};
+        fold.template add_vecs<false, T>(v, ks);
+      }
+    }
+    if (done) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.empty[r.slot]);
+    }
+    r.next();
+  };
+  Fold<ENT> fold;
+  int begun = 0;  // chunks of the row that are in its sums already (0 or 1)
   int row = row0;
   for (int i = first, it = 0; i < end; i += step) {
     const RowPart<T, S::kChunk> p(A, row, rank, size);
@@ -558,36 +653,14 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
     const int edge_col = tid < p.head ? tid : tid + p.nvec * VE;
     const int par = it & 1;
     const uint32_t phase = (it >> 1) & 1;
-    const int again = PASS == kFused ? p.chunks - min(p.chunks, S::kSlots) : 0;
+    const int again = chunks_again<PASS, S>(p.chunks);
+    Ring<S::kSlots> at_zero = zero;
     if (PASS != kBackward && i < n_active) {
-      Fold<ENT> fold;
-      for (int c = 0; c < p.chunks; ++c) {
-        wait_or_mark(&sh.full[r.slot], r.phase, sh);
-        const uint4* in = slots + r.slot * S::kChunk;
-        const int nv = min(S::kChunk, p.nv - c * S::kChunk);
-        if (nv == S::kChunk) {
-          constexpr int kAtOnce = 4;
-          static_assert(S::kVecs % kAtOnce == 0, "vectors are taken four at a time");
-#pragma unroll
-          for (int h = 0; h < S::kVecs; h += kAtOnce) {
-            uint4 v[kAtOnce];
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u) v[u] = in[tid + (h + u) * S::kGroup];
-            fold.template add_vecs<true, T>(v, ks);
-          }
-        } else {
-          for (int j = tid; j < nv; j += S::kGroup) {
-            const uint4 v[1] = {in[j]};
-            fold.template add_vecs<false, T>(v, ks);
-          }
-        }
-        if (PASS == kForward || c < again) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.empty[r.slot]);
-        }
-        r.next();
+      if (!begun) {
+        fold = Fold<ENT>();
+        at_zero = r;
       }
-      if (PASS == kFused) r.back(p.chunks - again);
+      for (int c = begun; c < p.chunks; ++c) sum_chunk(fold, p, c, PASS == kForward || c < again);
       if (tid < edge) {
         const float f[1] = {as_float(p.x[edge_col])};
         fold.template add<false>(f, f[0], ks);
@@ -597,6 +670,16 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
       if (lane == 0) {
         sh.part[par][warp] = a;
         mbar_arrive(&sh.part_full[par]);
+      }
+      begun = 0;
+      if (PASS == kFused && i + step < n_active) {
+        const RowPart<T, S::kChunk> next(A, row, rank, size);
+        if (next.chunks) {
+          fold = Fold<ENT>();
+          zero = r;
+          sum_chunk(fold, next, 0, chunks_again<PASS, S>(next.chunks) > 0);
+          begun = 1;
+        }
       }
     }
     if (PASS == kForward) {
@@ -626,10 +709,24 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
     const RowGrad o = sh.grad[par];
     const float wt = KIND == kDistill ? sh.grad_wt[par] : 0.f;
     const int hot_vec = o.tok < p.head ? -1 : (o.tok - p.head) / VE - p.v0;
+    // Both passes: the chunks that stayed, which lie before the next row's first one (a row that stayed whole: its
+    // first chunk where it was begun), then the others behind it.
+    const int stayed = p.chunks - again;
+    Ring<S::kSlots> from = r;
+    if (PASS == kFused) {
+      if (again)
+        from.back(begun + stayed);
+      else
+        from = at_zero;
+    }
     for (int c = 0; c < p.chunks; ++c) {
       const int at = c + again < p.chunks ? c + again : c + again - p.chunks;
-      wait_or_mark(&sh.full[r.slot], r.phase, sh);
-      const uint4* in = slots + r.slot * S::kChunk;
+      if (PASS == kFused && c == (again ? stayed : 1)) {
+        from = r;
+        if (!again) from.back(begun + stayed - 1);
+      }
+      wait_or_mark(&sh.full[from.slot], from.phase, sh);
+      const uint4* in = slots + from.slot * S::kChunk;
       const int j0 = at * S::kChunk, nv = min(S::kChunk, p.nv - j0);
       const bool hot_here = (unsigned)(hot_vec - j0) < (unsigned)nv;
       if (vec && !o.zero && nv == S::kChunk && !hot_here) {
@@ -657,31 +754,25 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.empty[r.slot]);
-      r.next();
+      if (lane == 0) mbar_arrive(&sh.empty[from.slot]);
+      from.next();
     }
+    if (PASS == kBackward || again) r = from;
     if (tid < edge) {
       float v = o.zero ? 0.f : grad_of<ENT, T>(as_float(p.x[edge_col]), o, ks);
       if (!o.zero && edge_col == o.tok) v += o.h;
       put(g + edge_col, v);
     }
     if (KIND == kDistill) {
-      // The list's columns, over what their vectors wrote.  An id that comes twice is written once, with both shares.
+      // The list's columns, over what their vectors wrote.
       if (PASS == kBackward) wait_or_mark(&sh.teacher_full[par], phase, sh);
       asm volatile("bar.sync 1, %0;" ::"n"(S::kGroup) : "memory");
-      const TeacherRow& q = sh.teacher[par];
+      const auto& q = sh.teacher[par];
       const int c0 = p.head + p.v0 * VE, c1 = c0 + p.nv * VE;
       for (int e = tid; e < A.k && !o.zero; e += S::kGroup) {
         const int id = q.id[e];
-        if (id < 0 || !((id >= c0 && id < c1) || (rank == 0 && (id < p.head || id >= p.head + p.nvec * VE)))) continue;
-        float sum = 0.f;
-        int firstly = e;
-        for (int f = 0; f < A.k; ++f) {
-          if (q.id[f] != id) continue;
-          firstly = min(firstly, f);
-          sum += q.q[f];
-        }
-        if (firstly == e) put(g + id, grad_of<false, T>(as_float(p.x[id]), o, ks) - wt * sum);
+        if (id >= 0 && ((id >= c0 && id < c1) || (rank == 0 && (id < p.head || id >= p.head + p.nvec * VE))))
+          put(g + id, grad_of<false, T>(PASS == kFused ? q.x[e] : as_float(p.x[id]), o, ks) - wt * q.q[e]);
       }
     }
     __syncwarp();
@@ -702,7 +793,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
 template <typename T, int KIND, bool ENT, int PASS>
 __global__ void __launch_bounds__(ShapeOf<T, PASS>::kThreads, ShapeOf<T, PASS>::kCtas) loss_rows_kernel(const LossArgs A) {
   using S = ShapeOf<T, PASS>;
-  using Sh = LossShared<S>;
+  using Sh = LossShared<S, PASS == kFused>;
   extern __shared__ __align__(128) uint8_t dyn[];
   uint4* slots = reinterpret_cast<uint4*>(dyn);
   Sh& sh = *reinterpret_cast<Sh*>(dyn + S::kRingBytes);
@@ -854,7 +945,7 @@ Layout layout(int64_t batch, int64_t length) {
 template <typename T, int KIND, bool ENT, int PASS>
 int32_t launch_typed(const LossArgs& a, cudaStream_t st) {
   using S = ShapeOf<T, PASS>;
-  constexpr int kBytes = S::kRingBytes + (int)sizeof(LossShared<S>);
+  constexpr int kBytes = S::kRingBytes + (int)sizeof(LossShared<S, PASS == kFused>);
   static_assert((kBytes + 1024) * S::kCtas <= 233472, "an SM's shared memory");
   int sms = 0;
   const int32_t e = sm_count(&sms);
