@@ -305,15 +305,14 @@ struct TeacherRow {
 constexpr int kIdTable = 2 * PKV_MAX_TOP;
 
 // Measured on rows of 151 936 columns.  Sums or gradient alone: four CTAs of 128 threads that take 8 vectors at a time
-// (16-bit sums of 4 096 rows 213 us; before the sums' last change 227, where 256 threads x 2 CTAs took 238 and 512
-// threads x 4 vectors x 1 CTA 275).  Both in one launch, 16 bits: two CTAs an SM hide each other's turns between the
-// passes, and a larger chunk its waits (490 us; one CTA of 768 threads 494, 512 threads with 2 vectors 580); bound by
-// the two exponentials and their conversions a column as much as by HBM.  float32, half the exponentials a byte: one
-// CTA an SM, whose rows in flight stay in L2 until their second pass, a row to a pair of CTAs where even they would
-// not (8 192 rows 1.58 ms; without pairs 1.84, 512 threads in pairs 1.61, two CTAs an SM 2.23, four CTAs a row 3.56).
+// (16-bit sums of 4 096 rows 210 us; 160 threads x 3 CTAs 234, 96 x 5 251, 512 threads x 4 vectors x 1 CTA 275).  Both in
+// one launch: one CTA an SM, whose rows in flight stay in L2 until their second pass; 16 bits 454 us (512 threads 464,
+// 768 480, two CTAs of 384 threads 512, a row to a pair of CTAs 530), where two exponentials and their conversions a
+// column cost as much as HBM.  float32, half the exponentials a byte: fewer threads and more slots, and a row to a pair
+// of CTAs where the rows in flight would not stay in L2 (8 192 rows 1.58 ms; without pairs 1.84, 512 threads 1.61).
 template <typename T, int PASS> struct ShapeOf : Shape<128, 8, 3, 4> {};
 template <typename T> struct ShapeOf<T, kFused> : Shape<640, 4, 5, 1> {};
-template <> struct ShapeOf<float, kFused> : Shape<512, 4, 6, 1> {};
+template <> struct ShapeOf<float, kFused> : Shape<384, 4, 8, 1> {};
 constexpr int64_t kRowsInL2 = 64 << 20;  // bytes of rows in flight that come back from L2
 
 template <typename S, bool X>
@@ -342,13 +341,21 @@ __device__ __forceinline__ void send_peer(void* dst, uint64_t* bar, uint32_t ran
 
 // The order of copies, which the column warps follow.  Sums or gradient alone: a row's chunks in turn.  Both: a row's
 // chunks for its sums, then the first chunk of the row behind it (whose sums begin while this row's coefficients are
-// made), then the chunks that did not stay in the ring, again, for its gradient.  The last kSlots - 1 chunks stay; a
-// slot's next copy waits for that slot alone, so chunks are freed in any order.
-
+// made), then the chunks that did not stay in the ring, again, for its gradient.
+//
+// Copy l waits for the chunk of copy l - kSlots, so none may be waited for before it can be free.  `whole`: a row has at
+// most kSlots - 1 chunks, all stay, and kSlots copies before the next row's first one lies the row before.  Else the
+// last kSlots - 1 chunks stay, but never the first one (rows at another offset in their 16 bytes may have a chunk less):
+// it is free when its sums are made, as are all that lie kSlots or more before the next row's first one.
+template <typename T, typename S>
+__device__ __forceinline__ bool rows_whole(int vocab, int size) {
+  const int nvec = vocab / RowSplit<T>::VE, per = (nvec + size - 1) / size;
+  return (per + S::kChunk - 1) / S::kChunk <= S::kSlots - 1;
+}
 // How many chunks of a row are copied twice.
 template <int PASS, typename S>
-__device__ __forceinline__ int chunks_again(int chunks) {
-  return PASS == kFused ? chunks - min(chunks, S::kSlots - 1) : 0;
+__device__ __forceinline__ int chunks_again(int chunks, bool whole) {
+  return PASS == kFused && !whole ? max(chunks - (S::kSlots - 1), min(chunks, 1)) : 0;
 }
 
 // The copying warp (one lane of it).
@@ -357,6 +364,7 @@ __device__ __forceinline__ void copy_rows(const LossArgs& A, Sh& sh, uint4* slot
                                           int step, int n_active, int row0) {
   Ring<S::kSlots> r;
   int filled = 0;
+  const bool whole = rows_whole<T, S>(A.vocab, size);
   // Chunks read twice are asked to stay in L2 until then; the others leave it first.
   uint64_t keep_policy;
   asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep_policy));
@@ -384,13 +392,13 @@ __device__ __forceinline__ void copy_rows(const LossArgs& A, Sh& sh, uint4* slot
   for (int i = first; i < n_active; i += step) {
     const RowPart<T, S::kChunk> p(A, row, rank, size);
     if (i + step < n_active) row = A.list[i + step];
-    const int again = chunks_again<PASS, S>(p.chunks);
+    const int again = chunks_again<PASS, S>(p.chunks, whole);
     for (int c = PASS == kFused && i != first ? 1 : 0; c < p.chunks; ++c)
       if (!copy(p, c, c < again)) return;
     if (PASS != kFused) continue;
     if (i + step < n_active) {
       const RowPart<T, S::kChunk> next(A, row, rank, size);
-      if (next.chunks && !copy(next, 0, chunks_again<PASS, S>(next.chunks) > 0)) return;
+      if (next.chunks && !copy(next, 0, chunks_again<PASS, S>(next.chunks, whole) > 0)) return;
     }
     for (int c = 0; c < again; ++c)
       if (!copy(p, c, false)) return;
@@ -614,6 +622,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
   const int lane = tid & 31, warp = tid >> 5;
   const Scale2 ks = A.ks;
   Ring<S::kSlots> r, zero;  // the next copy; the row's first chunk
+  const bool whole = rows_whole<T, S>(A.vocab, size);
   const int end = PASS == kForward ? n_active : n;
   // Chunk c of a row, at r, into its sums.
   auto sum_chunk = [&](Fold<ENT>& fold, const RowPart<T, S::kChunk>& p, int c, bool done) {
@@ -653,7 +662,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
     const int edge_col = tid < p.head ? tid : tid + p.nvec * VE;
     const int par = it & 1;
     const uint32_t phase = (it >> 1) & 1;
-    const int again = chunks_again<PASS, S>(p.chunks);
+    const int again = chunks_again<PASS, S>(p.chunks, whole);
     Ring<S::kSlots> at_zero = zero;
     if (PASS != kBackward && i < n_active) {
       if (!begun) {
@@ -677,7 +686,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
         if (next.chunks) {
           fold = Fold<ENT>();
           zero = r;
-          sum_chunk(fold, next, 0, chunks_again<PASS, S>(next.chunks) > 0);
+          sum_chunk(fold, next, 0, chunks_again<PASS, S>(next.chunks, whole) > 0);
           begun = 1;
         }
       }

@@ -655,6 +655,40 @@ def test_int_masks_and_types_are_taken(cuda_device):
     torch.testing.assert_close(leaf.grad, g1, atol=1e-6, rtol=1e-5)
 
 
+@pytest.mark.parametrize("dtype,chunk,slots", [(BF16, 20480, 5), (F32, 6144, 8)])
+@pytest.mark.parametrize("chunks", [1, -1, 0, 2])
+def test_rows_of_changing_chunk_counts(cuda_device, dtype, chunk, slots, chunks):
+    """Odd rows start at every offset in their 16 bytes, so that some have a 16-byte vector, and here a chunk of the
+    kernels' ring, less than others: around one chunk, and around as many as the ring holds (slots - 1, slots, + 2).
+    Enough rows for several turns of every CTA."""
+    from randomrepo_b200 import losses
+
+    per = 16 // dtype.itemsize
+    v = (1 if chunks == 1 else slots + chunks) * chunk + per + 1
+    n = 330
+    g = torch.Generator(device=cuda_device).manual_seed(v)
+    logits = torch.randn(1, n, v, generator=g, device=cuda_device).to(dtype)
+    assert len({logits[0, i].data_ptr() % 16 for i in range(16)}) == per
+    tokens = torch.randint(0, v, (1, n), generator=g, device=cuda_device)
+    adv = torch.randn(1, n, generator=g, device=cuda_device)
+    got, grad = losses.policy_loss_and_grad(logits, tokens, adv, reduction="sum")
+    ids = torch.randint(0, v, (1, n, 5), generator=g, device=cuda_device)
+    teacher = torch.randn(1, n, 5, generator=g, device=cuda_device)
+    dis, dgrad = losses.distillation_loss_and_grad(logits, ids, teacher, reduction="sum")
+    for i in range(0, n, 30):
+        at = slice(i, i + 30)
+        rows = torch.log_softmax(logits[0, at].double(), -1)
+        pick = rows.gather(-1, tokens[0, at].unsqueeze(-1)).squeeze(-1)
+        torch.testing.assert_close(got.logprobs[0, at].double(), pick, atol=LP, rtol=0)
+        want = rows.exp()
+        want.scatter_add_(-1, tokens[0, at].unsqueeze(-1), -torch.ones_like(pick).unsqueeze(-1))
+        coef = adv[0, at].double().unsqueeze(-1)
+        _close_grad(grad[0, at], want * coef, coef, dtype)
+        q = torch.softmax(teacher[0, at].double(), -1)
+        want = rows.exp().scatter_add_(-1, ids[0, at], -q)
+        _close_grad(dgrad[0, at], want, torch.ones_like(coef) * 2, dtype)
+
+
 def test_rows_past_32_bits(cuda_device):
     """A tensor whose last rows start past 2^32 bytes and 2^31 elements."""
     from randomrepo_b200 import losses

@@ -217,3 +217,39 @@ def test_operators_have_fake_shapes():
         loss, s, m, grad = torch.ops.pkv.preference_loss(x, torch.empty((4, 9), dtype=torch.int64, device=dev), None,
                                                          None, 0.1, 0.0, False, 1.0)
         assert loss.shape == () and s.shape == (4,) and m.shape == (2,) and grad.shape == x.shape
+
+
+@pytest.mark.parametrize("slots", [4, 5, 8])
+def test_the_rings_order_never_waits_for_itself(slots):
+    """A model of the order in which a row's chunks are copied, looked at and freed when sums and gradient share a
+    launch (csrc/losses.cu): rows of up to three rings' length, some a chunk shorter than others.  Copy l waits until
+    the chunk of copy l - slots is free; every chunk that is looked at must have been copied by then."""
+    import random
+
+    for most in range(1, 3 * slots):
+        whole = most <= slots - 1
+        again = lambda n: 0 if whole else max(n - (slots - 1), min(n, 1))  # noqa: E731
+        for seed in range(60):
+            r = random.Random(seed)
+            rows = [most - r.randint(0, 1) for _ in range(r.randint(1, 12))]
+            copies, looks, begun = [], [], 0
+            for i, n in enumerate(rows):
+                following = i + 1 < len(rows) and rows[i + 1] > 0
+                copies += [(i, c, 0) for c in range(begun, n)]
+                for c in range(begun, n):
+                    looks.append(((i, c, 0), c < again(n)))
+                begun = int(following)
+                if following:
+                    copies.append((i + 1, 0, 0))
+                    looks.append(((i + 1, 0, 0), again(rows[i + 1]) > 0))
+                copies += [(i, c, 1) for c in range(again(n))]
+                looks += [((i, c, 0), True) for c in range(again(n), n)] + [((i, c, 1), True) for c in range(again(n))]
+            place = {c: k for k, c in enumerate(copies)}
+            free, copied = set(), 0
+            for chunk, done in looks:
+                while copied < len(copies) and (copied < slots or copied - slots in free):
+                    copied += 1
+                assert place[chunk] < copied and place[chunk] not in free, (rows, chunk)
+                if done:
+                    free.add(place[chunk])
+            assert len(free) == len(copies)
