@@ -21,7 +21,9 @@ columns (any batch and row strides, so that ``logits[:, :-1]`` needs no copy); p
 (``[T]``).  A row whose mask is 0 is not scored: its logits are not read, its outputs and its gradient are
 0; tokens there may be anything.  No scored row at all gives a loss of 0.  Losses and per-row outputs are
 float32; sums over rows are taken in 64 bits, in a fixed order.  Calls launch on the current stream of the
-logits' device, never synchronise, and can be captured in a CUDA graph.  There is no CPU path.
+logits' device, never synchronise, and can be captured in a CUDA graph (a captured training step best uses the
+``*_and_grad`` forms: PyTorch cannot capture a backward pass into leaves that another, eager graph still holds).
+There is no CPU path.
 """
 
 from __future__ import annotations
@@ -221,7 +223,7 @@ class _RowLoss(torch.autograd.Function):
         if grad_loss.dtype != torch.float32 or grad_loss.device != c.x.device:
             grad_loss = grad_loss.to(dtype=torch.float32, device=c.x.device)
         _launch(c.backward, c, grad, (grad_loss,))
-        return grad.view(logits.shape) if grad.dim() != logits.dim() else grad, None, None, None
+        return grad if grad.dim() == logits.dim() else grad.squeeze(0), None, None, None
 
 
 def _run(fn, c: _Call, logits: torch.Tensor, outputs: tuple):

@@ -527,6 +527,34 @@ def test_capture_streams_and_two_calls_at_once(cuda_device):
             assert torch.equal(r.loss, w.loss) and torch.equal(grad, wg)
 
 
+def test_captured_backward(cuda_device):
+    """Forward and backward of the differentiable form in one graph (its leaf in no other), replayed on new logits."""
+    from randomrepo_b200 import losses
+
+    logits, tokens, adv, old, ref, mask = _policy_case(2, 9, 4099, F16, cuda_device, "some", 8)
+    other = _policy_case(2, 9, 4099, F16, cuda_device, "some", 9)[0]
+
+    def step(x):
+        leaf = x.detach().requires_grad_()
+        out = losses.policy_loss(leaf, tokens, adv, old, mask, entropy_coef=0.01, scale=8.0)
+        return out.loss.detach(), torch.autograd.grad(out.loss, leaf)[0]
+
+    want = [step(logits), step(other)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(logits)
+    torch.cuda.current_stream().wait_stream(side)
+    x = logits.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grad = step(x)
+    for data, (wl, wg) in zip((logits, other), want):
+        x.copy_(data)
+        graph.replay()
+        assert torch.equal(loss, wl) and torch.equal(grad, wg)
+
+
 def test_backward_twice_and_through_a_model(cuda_device):
     """retain_graph backward passes give the same gradient; a small head trains through the loss."""
     from randomrepo_b200 import losses
@@ -653,6 +681,10 @@ def test_int_masks_and_types_are_taken(cuda_device):
     leaf = logits[0].detach().requires_grad_()
     losses.policy_loss(leaf, tokens[0], adv[0], old[0], mask[0], reduction="sum").loss.backward()
     torch.testing.assert_close(leaf.grad, g1, atol=1e-6, rtol=1e-5)
+    leaf = logits[0].detach().requires_grad_()  # [T, V] rows apart, at an odd place
+    losses.policy_loss(leaf[1::2, 3:], tokens[0, 1::2] % 298, adv[0, 1::2], reduction="sum").loss.backward()
+    _, g2 = losses.policy_loss_and_grad(logits[0, 1::2, 3:], tokens[0, 1::2] % 298, adv[0, 1::2], reduction="sum")
+    torch.testing.assert_close(leaf.grad[1::2, 3:], g2, atol=1e-6, rtol=1e-5)
 
 
 @pytest.mark.parametrize("dtype,chunk,slots", [(BF16, 20480, 5), (F32, 6144, 8)])
