@@ -313,7 +313,12 @@ constexpr int kIdTable = 2 * PKV_MAX_TOP;
 template <typename T, int PASS> struct ShapeOf : Shape<128, 8, 3, 4> {};
 template <typename T> struct ShapeOf<T, kFused> : Shape<640, 4, 5, 1> {};
 template <> struct ShapeOf<float, kFused> : Shape<384, 4, 8, 1> {};
-constexpr int64_t kRowsInL2 = 64 << 20;  // bytes of rows in flight that come back from L2
+// Short rows, sums and gradient: four CTAs an SM, for each row is a chain of latencies.  8 192 rows against the shapes
+// above: 1 000 16-bit columns 63 / 176 us, 10 000 127 / 212, 50 000 367 / 402, 80 000 559 / 546; float32 1 000 63 / 153,
+// 20 000 246 / 305, 35 000 469 / 423.
+using ShortShape = Shape<128, 4, 5, 4>;
+constexpr int64_t kShortRow = 112 << 10;   // bytes
+constexpr int64_t kRowsInL2 = 64 << 20;    // bytes of rows in flight that come back from L2
 
 template <typename S, bool X>
 struct alignas(128) LossShared {
@@ -799,9 +804,8 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
 // ring, the rest is read again while it is in L2.  One warp copies, one takes a finished row's sums to its
 // coefficients, the others work on the columns.  Few rows are spread over clusters: each CTA has a part of the
 // columns, and the parts' sums cross by distributed shared memory.
-template <typename T, int KIND, bool ENT, int PASS>
-__global__ void __launch_bounds__(ShapeOf<T, PASS>::kThreads, ShapeOf<T, PASS>::kCtas) loss_rows_kernel(const LossArgs A) {
-  using S = ShapeOf<T, PASS>;
+template <typename T, int KIND, bool ENT, int PASS, typename S>
+__global__ void __launch_bounds__(S::kThreads, S::kCtas) loss_rows_kernel(const LossArgs A) {
   using Sh = LossShared<S, PASS == kFused>;
   extern __shared__ __align__(128) uint8_t dyn[];
   uint4* slots = reinterpret_cast<uint4*>(dyn);
@@ -951,15 +955,14 @@ Layout layout(int64_t batch, int64_t length) {
   return l;
 }
 
-template <typename T, int KIND, bool ENT, int PASS>
-int32_t launch_typed(const LossArgs& a, cudaStream_t st) {
-  using S = ShapeOf<T, PASS>;
+template <typename T, int KIND, bool ENT, int PASS, typename S>
+int32_t launch_shape(const LossArgs& a, cudaStream_t st) {
   constexpr int kBytes = S::kRingBytes + (int)sizeof(LossShared<S, PASS == kFused>);
   static_assert((kBytes + 1024) * S::kCtas <= 233472, "an SM's shared memory");
   int sms = 0;
   const int32_t e = sm_count(&sms);
   if (e != PKV_OK) return e;
-  auto* kernel = loss_rows_kernel<T, KIND, ENT, PASS>;
+  auto* kernel = loss_rows_kernel<T, KIND, ENT, PASS, S>;
   static bool ready[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -974,6 +977,13 @@ int32_t launch_typed(const LossArgs& a, cudaStream_t st) {
   if (PASS == kFused && S::kCtas == 1 && c == 1 && rows > sms && sms * row_bytes > kRowsInL2) c = 2;
   const int grid = (int)std::min<int64_t>(rows, sms * S::kCtas / c) * c;
   return launch_after(kernel, grid, S::kThreads, c, kBytes, a, st, "loss rows launch");
+}
+
+template <typename T, int KIND, bool ENT, int PASS>
+int32_t launch_typed(const LossArgs& a, cudaStream_t st) {
+  if constexpr (PASS == kFused)
+    if ((int64_t)a.vocab * (int64_t)sizeof(T) <= kShortRow) return launch_shape<T, KIND, ENT, PASS, ShortShape>(a, st);
+  return launch_shape<T, KIND, ENT, PASS, ShapeOf<T, PASS>>(a, st);
 }
 
 template <int KIND, bool ENT, int PASS>

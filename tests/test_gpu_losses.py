@@ -687,7 +687,7 @@ def test_int_masks_and_types_are_taken(cuda_device):
     torch.testing.assert_close(leaf.grad[1::2, 3:], g2, atol=1e-6, rtol=1e-5)
 
 
-@pytest.mark.parametrize("dtype,chunk,slots", [(BF16, 20480, 5), (F32, 6144, 8)])
+@pytest.mark.parametrize("dtype,chunk,slots", [(BF16, 20480, 5), (F32, 6144, 8), (F16, 4096, 5), (F32, 2048, 5)])
 @pytest.mark.parametrize("chunks", [1, -1, 0, 2])
 def test_rows_of_changing_chunk_counts(cuda_device, dtype, chunk, slots, chunks):
     """Odd rows start at every offset in their 16 bytes, so that some have a 16-byte vector, and here a chunk of the
@@ -697,7 +697,7 @@ def test_rows_of_changing_chunk_counts(cuda_device, dtype, chunk, slots, chunks)
 
     per = 16 // dtype.itemsize
     v = (1 if chunks == 1 else slots + chunks) * chunk + per + 1
-    n = 330
+    n = 330 if v > 60000 else 1500
     g = torch.Generator(device=cuda_device).manual_seed(v)
     logits = torch.randn(1, n, v, generator=g, device=cuda_device).to(dtype)
     assert len({logits[0, i].data_ptr() % 16 for i in range(16)}) == per
@@ -707,8 +707,8 @@ def test_rows_of_changing_chunk_counts(cuda_device, dtype, chunk, slots, chunks)
     ids = torch.randint(0, v, (1, n, 5), generator=g, device=cuda_device)
     teacher = torch.randn(1, n, 5, generator=g, device=cuda_device)
     dis, dgrad = losses.distillation_loss_and_grad(logits, ids, teacher, reduction="sum")
-    for i in range(0, n, 30):
-        at = slice(i, i + 30)
+    for i in range(0, n, 150):
+        at = slice(i, i + 150)
         rows = torch.log_softmax(logits[0, at].double(), -1)
         pick = rows.gather(-1, tokens[0, at].unsqueeze(-1)).squeeze(-1)
         torch.testing.assert_close(got.logprobs[0, at].double(), pick, atol=LP, rtol=0)
