@@ -73,7 +73,7 @@ struct LossArgs {
   Tokens2<float> tlse;
   float *logprobs, *kl_out, *entropy, *loss;
   double* row_val;        // [rows]: weighted loss (policy, distillation) or log-probability (preference)
-  float4* rec;            // [rows] {m, a, b, h} for a later backward pass (distillation: {m, a, w T, log q's norm})
+  float4* rec;            // [rows] {m, a, b, h} for a later backward pass (distillation: {m, a, w T, -})
   const float* upstream;  // device scalar the gradient is multiplied by, or null
 };
 
@@ -414,9 +414,10 @@ __device__ __forceinline__ void copy_rows(const LossArgs& A, Sh& sh, uint4* slot
 template <typename T, int PASS, typename S, typename Sh>
 __device__ __forceinline__ void teacher_rows(const LossArgs& A, Sh& sh, int rank, int size, int first, int step,
                                              int n_active, int row0, int lane) {
-  int it = 0;
-  for (int i = first; i < n_active; i += step, ++it) {
-    const RowPart<T, S::kChunk> p(A, it ? A.list[i] : row0, rank, size);
+  int row = row0;
+  for (int i = first, it = 0; i < n_active; i += step, ++it) {
+    const RowPart<T, S::kChunk> p(A, row, rank, size);
+    if (i + step < n_active) row = A.list[i + step];
     auto& o = sh.teacher[it & 1];
     if (it >= 2) wait_or_mark(&sh.teacher_empty[it & 1], ((it >> 1) & 1) ^ 1, sh);
     constexpr int kPer = PKV_MAX_TOP / 32;
@@ -505,7 +506,12 @@ __device__ __forceinline__ void teacher_rows(const LossArgs& A, Sh& sh, int rank
         if (j < A.k) o.q[j] = all[e], o.id[j] = later[e] ? -1 : ids[e];
       }
     }
-    qs = warp_sum_d(qs), qx = warp_sum_d(qx), ql = warp_sum_d(ql);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {  // (the three together: latency is this warp's cost)
+      const double a = __shfl_xor_sync(0xffffffffu, qs, off), b = __shfl_xor_sync(0xffffffffu, qx, off);
+      const double c = __shfl_xor_sync(0xffffffffu, ql, off);
+      qs += a, qx += b, ql += c;
+    }
     if (lane == 0) o.q_sum = qs, o.qx = qx, o.qlogq = ql;
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.teacher_full[it & 1]);
