@@ -73,7 +73,7 @@ struct LossArgs {
   Tokens2<float> tlse;
   float *logprobs, *kl_out, *entropy, *loss;
   double* row_val;        // [rows]: weighted loss (policy, distillation) or log-probability (preference)
-  float4* rec;            // [rows] {m, a, b, h} for a later backward pass (distillation: {m, a, w T, -})
+  float4* rec;            // [rows] {m, a, b, h} for a later backward pass (distillation: {m, a, w T, -}) of x's type
   const float* upstream;  // device scalar the gradient is multiplied by, or null
 };
 
@@ -255,6 +255,17 @@ __global__ void __launch_bounds__(1024) loss_plan_kernel(const PlanArgs A) {
 // ---------------------------------------------------------------------------
 // Rows.
 
+// 16-bit gradients leave x k.lo out of a column's y, which the sum s has: e comes out smaller by 2^(x k.lo), the same
+// factor for all columns that count (those near m: (x - m) k.lo is at most 2^-23 of a y of 30 or so).  It goes into the
+// row's a and b, for at a column of a large h or q, where p is near it, half a step of 16 bits would not hide it.
+template <typename T>
+__device__ __forceinline__ void fold_low(RowGrad& o, Scale2 k) {
+  if (sizeof(T) == 4 || far_out(center(o.m, k))) return;
+  const float y = o.m * k.lo, f = ex2(y);
+  o.a = fmaf(o.b, y, o.a) * f;
+  o.b *= f;
+}
+
 // N columns of the gradient, the list's columns apart.
 template <bool ENT, typename T, int N>
 __device__ __forceinline__ void grad_columns(float (&x)[N], const RowGrad& o, Scale2 k) {
@@ -272,7 +283,7 @@ __device__ __forceinline__ void grad_columns(float (&x)[N], const RowGrad& o, Sc
   for (int i = 0; i < N; i += 2) {
     const f32x2 xx = pair(x[i], i + 1 < N ? x[i + 1] : 0.f);
     f32x2 y2 = fma2(xx, hi, cc);
-    if (sizeof(T) == 4) y2 = fma2(xx, lo, y2);  // (half a step of 16 bits hides it)
+    if (sizeof(T) == 4) y2 = fma2(xx, lo, y2);  // (16 bits: in a and b)
     const float2 y = unpair(y2);
     const f32x2 e = pair(ex2(y.x), ex2(y.y));
     const float2 v = unpair(mul2(e, ENT ? fma2(b, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), a) : a));
@@ -596,6 +607,7 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
           A.row_val[row] = w * l;
         }
       }
+      fold_low<T>(o, ks);
       if (PASS == kForward) {
         if (write && A.rec)
           A.rec[row] = KIND == kDistill ? make_float4(o.m, o.a, wt, 0.f) : make_float4(o.m, o.a, o.b, o.h);
