@@ -54,21 +54,27 @@ __device__ __forceinline__ float ex2(float y) {
   return e;
 }
 
-// Columns x of a row are taken as y = x k + c, c = -(max x) k rounded once:
+// Columns x of a row are taken as y = x k + c, c = -(max x) hi rounded once:
 // one fused multiply-add a column, and what is made of y later starts from
-// the same c.  Where max x k leaves the range in which that is safe (masks of
-// a type's lowest value everywhere), y = (x - max x) k.
+// the same c.  Its rounding and max x lo stay in every y, up to 2^-24 + 2^-23
+// of c: 18 at 1e8, which the sums hold.  Rows beyond that (masks of -1e9 or a
+// type's lowest value everywhere) take y = (x - max x) k.
 __device__ __forceinline__ float center(float m, Scale2 k) { return __fmul_rn(-m, k.hi); }  // (rounded: never part of another FMA)
-__device__ __forceinline__ bool far_out(float c) { return !(fabsf(c) < 1e30f); }
+__device__ __forceinline__ bool far_out(float c) { return !(fabsf(c) < 1e8f); }
 // The running sums of a set of columns: m = max x, s = sum 2^y, w = sum 2^y y.
 struct RowSum {
   float m, s, w;
 };
 
-// d: the exponent that takes sums from a reference m to another.
+// d: the exponent that takes sums from a reference m to a larger one.
 __device__ __forceinline__ float rescale_exponent(float m, float m_new, Scale2 k) {
-  const float c = center(m_new, k);
-  return far_out(c) ? (m - m_new) * k.hi : c - center(m, k);
+  if (m == -INFINITY) return -INFINITY;
+  const float c = center(m_new, k), from = center(m, k);
+  if (far_out(c) != far_out(from)) {  // (what stays in c is in the y of one of them alone)
+    const float n = far_out(c) ? m : m_new, in_c = far_out(c) ? from : c, stays = fmaf(n, k.lo, fmaf(n, k.hi, in_c));
+    return (m - m_new) * k.hi + (far_out(c) ? -stays : stays);
+  }
+  return far_out(c) ? (m - m_new) * k.hi : c - from;
 }
 
 __device__ __forceinline__ void sum_rescale(RowSum& a, float m_new, float d, float f) {

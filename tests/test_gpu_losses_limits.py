@@ -5,6 +5,8 @@ Definitions are torch operations in 64 bits; each tolerance is derived where it 
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -76,3 +78,69 @@ def test_a_certain_tokens_gradient(cuda_device, dtype, temperature, top, gap, en
     losses.distillation_loss(leaf, ids, teacher, temperature=temperature, reduction="sum").loss.backward()
     # (q is an expf of a float32 argument of at most 12: 2^-20 of q)
     compare(grad, leaf.grad, want, torch.tensor(3 * t, device=cuda_device))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_rows_of_large_values(cuda_device, dtype):
+    """Rows whose values times the scale are far past what a float32 exponent's reference holds (a mask of -1e9 in every
+    column, the largest float16 at a low temperature): uniform, and exact where neighbouring values differ.
+
+    log p: a column's exponent is at most 40 where it counts, rounded three times (40 x 3 x 2^-24 ln 2 = 5e-6), its
+    approximate 2^y is off by 2^-22 and a sum of up to 1000 columns in float32 by at most 16 additions a thread and
+    their merges (32 x 2^-24 = 2e-6): below 1e-5.  Gradients: that of p."""
+    from randomrepo_b200 import losses
+
+    v = 1000
+    values = {BF16: [-1e9, 1e9, 3e7, -1e30, 1e37], F16: [-65504.0, 65504.0, 30000.0], F32: [-1e9, 1e9, 123456789.0, -1e30, 1e37]}[dtype]
+    for temperature in (1.0, 0.1, 1e-2, 1e-4, 1e-6):
+        t = _float(temperature)
+        x = torch.tensor(values).to(dtype).unsqueeze(1).repeat(1, v).unsqueeze(0)
+        # Some columns a step of the type below the others.
+        x[:, :, 100:900] = torch.nextafter(x[:, :, 100:900], torch.tensor(-math.inf, dtype=dtype)) if dtype != BF16 else x[:, :, 100:900]
+        x = x.to(cuda_device)
+        tokens = torch.full(x.shape[:2], 3, device=cuda_device)
+        rows = torch.log_softmax(x.double() / t, -1)
+        got, grad = losses.policy_loss_and_grad(x, tokens, torch.ones(1, device=cuda_device), temperature=temperature,
+                                                reduction="sum", scale=t)
+        want = rows.exp()
+        want[..., 3] -= 1
+        assert (got.logprobs.double() - rows[..., 3]).abs().max() <= 1e-5, (temperature, got.logprobs, rows[..., 3])
+        off = (grad.double() - want).abs()
+        tol = want.abs() * (_half(dtype) + 1e-5) + 1e-5 * rows.exp() + 2.0**-22 + (2.0**-25 if dtype == F16 else 0)
+        assert (off <= tol).all(), (temperature, off.max())
+        _, _, lse = losses.top_logits(x, 3, temperature=temperature)
+        ref = (x.double() / t).logsumexp(-1)
+        assert ((lse.double() - ref).abs() <= 1e-5 + 2.0**-23 * ref.abs()).logical_or(lse == ref.float()).all()
+        ids = torch.tensor([5, 77], device=cuda_device).expand(*x.shape[:2], 2)
+        q = torch.zeros(*x.shape[:2], 2, device=cuda_device)
+        dis, _ = losses.distillation_loss_and_grad(x, ids, q, temperature=temperature, reduction="sum")
+        per = t * t * (-math.log(2) - rows[..., [5, 77]].mean(-1))
+        assert ((dis.kl.double() - per).abs() <= t * t * 1.2e-5 + 2.0**-22 * per.abs()).all()
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 2.0])
+def test_rows_across_the_far_border(cuda_device, temperature):
+    """float32 values on both sides of where the kernels begin to subtract before they scale, in ascending and
+    descending order (every warp's reference crosses it), 8 T apart at the least; bounds as above with more columns:
+    50 001 of them in up to 80 additions a thread (1e-5 more)."""
+    from randomrepo_b200 import losses
+
+    v, t = 50001, _float(temperature)
+    border = 1e8 * t / math.log2(math.e)
+    g = torch.Generator().manual_seed(5)
+    steps = torch.randint(-6, 7, (v,), generator=g).float() * 8
+    for sign in (1.0, -1.0):
+        base = torch.tensor(sign * border, dtype=F32)
+        rows = torch.stack([base + steps, (base + steps).sort().values, (base + steps).sort(descending=True).values])
+        x = rows.unsqueeze(0).to(cuda_device)
+        tokens = x.argmax(-1)
+        want = torch.log_softmax(x.double() / t, -1).gather(-1, tokens.unsqueeze(-1)).squeeze(-1)
+        got, grad = losses.policy_loss_and_grad(x, tokens, torch.ones(1, device=cuda_device), temperature=temperature,
+                                                reduction="sum", scale=t)
+        assert (got.logprobs.double() - want).abs().max() <= 2e-5, (got.logprobs, want)
+        p = torch.softmax(x.double() / t, -1)
+        p.scatter_add_(-1, tokens.unsqueeze(-1), -torch.ones_like(want).unsqueeze(-1))
+        assert (grad.double() - p).abs().max() <= 2e-5
+        _, _, lse = losses.top_logits(x, 3, temperature=temperature)
+        ref = (x.double() / t).logsumexp(-1)
+        assert ((lse.double() - ref).abs() <= 2e-5 + 2.0**-23 * ref.abs()).logical_or(lse == ref.float()).all()
