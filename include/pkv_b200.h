@@ -677,7 +677,8 @@ int32_t pkv_spec_accept(const float* target_logits, const float* draft_logits, i
  * then), which multiplies by the device scalar *upstream.  Gradients of rows
  * and the loss are the same bits from call to call.  A scored row whose token
  * lies outside [0, vocab) makes its log-probability, its gradient row and the
- * loss NaN.  The workspace is device scratch of
+ * loss NaN.  Should a kernel's bounded wait run out, the loss is NaN, and so
+ * is what a later *_backward call writes for scored rows.  The workspace is device scratch of
  * pkv_loss_workspace_bytes(batch, length) bytes, 256-byte aligned, no initial
  * contents needed; calls sharing one run in stream order.
  * ------------------------------------------------------------------------- */

@@ -46,7 +46,7 @@ struct Tokens2 {
 struct LossHeader {
   int32_t n_active;
   int32_t ticket;
-  int32_t error;  // a bounded wait gave up: the loss becomes NaN
+  int32_t error;  // a bounded wait gave up: the loss, and gradients made after it, become NaN
 };
 
 struct LossArgs {
@@ -536,7 +536,8 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
                                           int n_active, int n, int row0, int lane) {
   const bool write = lane == 0 && rank == 0;
   const Scale2 ks = A.ks;
-  const float up = A.upstream ? *A.upstream : 1.f;
+  // (records that a launch left without all its sums give no gradient)
+  const float up = PASS == kBackward && *(volatile int32_t*)&A.hdr->error ? NAN : A.upstream ? *A.upstream : 1.f;
   int row_next = row0;
   int64_t tok_next = 0;
   if (KIND != kDistill && first < n_active) tok_next = A.tokens.at(row_next / A.length, row_next % A.length);
@@ -896,6 +897,7 @@ struct PairArgs {
   const uint8_t* mask;
   int64_t mb, mt;
   int32_t batch, length, normalised;
+  const LossHeader* hdr;
   const float* ref;
   float beta, smoothing, scale;
   const double* row_val;
@@ -909,8 +911,9 @@ __global__ void __launch_bounds__(1024) loss_pair_kernel(const PairArgs A) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const double start = A.hdr->error ? (double)NAN : 0.0;  // (a NaN goes from the sums into all there is)
   for (int b = warp; b < A.batch; b += 32) {
-    double sum = 0.0;
+    double sum = start;
     for (int t = lane; t < A.length; t += 32)
       if (A.mask == nullptr || A.mask[b * A.mb + t * A.mt] != 0) sum += A.row_val[b * A.length + t];
 #pragma unroll
@@ -1150,7 +1153,7 @@ extern "C" int32_t pkv_preference_loss(const pkv_loss_rows* r, const pkv_prefere
   if ((st = launch_plan(r, l, ws, PKV_SUM, 1.f, s)) != PKV_OK) return st;
   if (!empty_rows(r) && (st = launch_rows<kPreference, false, kForward>(a, r->dtype, s)) != PKV_OK) return st;
   PairArgs q{r->mask, r->mask_batch_stride, r->mask_row_stride, r->batch, r->length, p->length_normalised,
-             p->ref_logprobs, p->beta, p->label_smoothing, p->scale,
+             a.hdr, p->ref_logprobs, p->beta, p->label_smoothing, p->scale,
              reinterpret_cast<const double*>(ws + l.row_val), reinterpret_cast<const int32_t*>(ws + l.seq_n),
              reinterpret_cast<double*>(ws + l.seq_sum), reinterpret_cast<float*>(ws + l.seq_g), logprobs, margins, loss};
   if ((st = launch_after(loss_pair_kernel, 1, 1024, 1, 0, q, s, "preference pairs launch")) != PKV_OK) return st;

@@ -5,6 +5,7 @@ Definitions are torch operations in 64 bits; each tolerance is derived where it 
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -144,3 +145,85 @@ def test_rows_across_the_far_border(cuda_device, temperature):
         _, _, lse = losses.top_logits(x, 3, temperature=temperature)
         ref = (x.double() / t).logsumexp(-1)
         assert ((lse.double() - ref).abs() <= 2e-5 + 2.0**-23 * ref.abs()).logical_or(lse == ref.float()).all()
+
+
+def _header(call_ws):
+    """The workspace's header as 32-bit words: scored rows, ticket, error."""
+    return call_ws[:12].view(torch.int32)
+
+
+class _Array(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64)]
+
+
+class _Rows(ctypes.Structure):
+    _fields_ = [("logits", _Array), ("grad", _Array), ("mask", _Array), ("batch", ctypes.c_int32),
+                ("length", ctypes.c_int32), ("vocab", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("temperature", ctypes.c_float)]
+
+
+class _Preference(ctypes.Structure):
+    _fields_ = [("tokens", _Array), ("ref", ctypes.c_void_p), ("beta", ctypes.c_float), ("smoothing", ctypes.c_float),
+                ("normalised", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
+def _array2(t):
+    return _Array(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def test_an_error_of_the_forward_pass_makes_gradients_nan(cuda_device):
+    """A wait that gave up in the forward launch leaves its mark in the workspace; a later backward pass is NaN."""
+    from randomrepo_b200 import losses
+
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(2, 5, 301, generator=g).to(cuda_device)
+    tokens = torch.randint(0, 301, (2, 5), generator=g).to(cuda_device)
+    ids = torch.randint(0, 301, (2, 5, 4), generator=g).to(cuda_device)
+    teacher = torch.randn(2, 5, 4, generator=g).to(cuda_device)
+    mask = torch.ones(2, 5, dtype=torch.bool, device=cuda_device)
+    mask[1, 3] = False
+    for call in (lambda z: losses.policy_loss(z, tokens, torch.ones(2, device=cuda_device), None, mask),
+                 lambda z: losses.policy_loss(z, tokens, torch.ones(2, device=cuda_device), None, mask, entropy_coef=0.1),
+                 lambda z: losses.preference_loss(z, tokens, mask),
+                 lambda z: losses.distillation_loss(z, ids, teacher, mask)):
+        leaf = x.clone().requires_grad_()
+        out = call(leaf)
+        (grad,) = torch.autograd.grad(out.loss, leaf, retain_graph=True)
+        assert grad.isfinite().all()
+        ws = [s for s in out.loss.grad_fn.saved_tensors if s is not None and s.dtype == torch.uint8]
+        assert len(ws) == 1
+        _header(ws[0].data)[2] = 1  # (.data: not a change that the saved tensors' check should see)
+        (grad,) = torch.autograd.grad(out.loss, leaf)
+        assert grad[mask].isnan().all() and (grad[~mask] == 0).all()
+
+
+def test_an_error_of_the_preference_sums_is_loud(cuda_device):
+    """The mark of a wait that gave up in the sums' launch, set here by a copy while that launch runs (1.2 GB of rows:
+    0.3 ms and more after the plan has cleared it): loss, margins, sums and the gradient are NaN.  The copy may come too
+    late, so there are several trials; without a mark nothing is ever NaN."""
+    from randomrepo_b200 import _lib
+    from randomrepo_b200._lib import lib
+
+    b, t, v = 2, 4096, 151936
+    x = torch.zeros(b, t, v, dtype=BF16, device=cuda_device)
+    grad = torch.empty_like(x)
+    tokens = torch.zeros(b, t, dtype=torch.int64, device=cuda_device)
+    rows = _Rows(logits=_array2(x), grad=_array2(grad), batch=b, length=t, vocab=v, dtype=_lib.PKV_BF16, temperature=1.0)
+    terms = _Preference(tokens=_array2(tokens), beta=0.1, scale=1.0)
+    n = lib.pkv_loss_workspace_bytes(b, t)
+    ws = torch.empty(n, dtype=torch.uint8, device=cuda_device)
+    out = torch.empty(4, device=cuda_device)
+    mark = torch.ones(1, dtype=torch.int32).pin_memory()
+    side = torch.cuda.Stream()
+    for _ in range(8):
+        torch.cuda.synchronize()
+        st = lib.pkv_preference_loss(ctypes.byref(rows), ctypes.byref(terms), out.data_ptr(), out.data_ptr() + 4,
+                                     out.data_ptr() + 12, ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
+        assert st == 0, _lib.last_error()
+        with torch.cuda.stream(side):
+            _header(ws)[2:3].copy_(mark, non_blocking=True)
+        torch.cuda.synchronize()
+        if out.isnan().any():
+            break
+    assert out.isnan().all()
+    assert grad[0, 0].isnan().all() and grad[1, -1].isnan().all()
