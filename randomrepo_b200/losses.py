@@ -111,16 +111,14 @@ def _rows_like(t: torch.Tensor, rows: torch.Size, dev: torch.device, dtype: torc
     return t
 
 
-def _advantages(t: torch.Tensor, rows: torch.Size, dev: torch.device, what: str):
-    """Advantages [B, T], [B, 1] or [B] (one a sequence) as float32, and their pointer and strides."""
+def _advantages(t: torch.Tensor, rows: torch.Size, dev: torch.device, what: str) -> torch.Tensor:
+    """Advantages [B, T], [B, 1] or [B] (one a sequence) as float32."""
     if isinstance(t, torch.Tensor) and t.shape != rows and t.device == dev and not (rows[0] == 1 and t.dim() == 1
                                                                                 and t.shape[0] == rows[1]):
         if tuple(t.shape) not in ((rows[0],), (rows[0], 1)):
             raise ValueError(f"{what}: advantages must be [batch, length] or [batch], got {tuple(t.shape)}")
-        t = t.to(torch.float32)
-        return t, (t.data_ptr(), t.stride(0), 0)
-    t = _rows_like(t, rows, dev, torch.float32, what, "advantages")
-    return t, _array(t)
+        return t.to(torch.float32)
+    return _rows_like(t, rows, dev, torch.float32, what, "advantages")
 
 
 def _mask(mask: torch.Tensor | None, rows: torch.Size, dev: torch.device, what: str) -> torch.Tensor | None:
@@ -163,26 +161,48 @@ def _grad_like(x: torch.Tensor) -> torch.Tensor:
     return flat.as_strided((b, n, v), (max(sb, span), max(sn, v), 1), at)
 
 
-class _Call:
-    """One loss call: the packed rows and terms, its tensors, and the workspace a backward pass reads."""
+class _Kind(NamedTuple):
+    """A loss: its entry points, inputs(rows, dev, what, *tensors): the terms' tensors, checked, terms(numbers, *tensors): the
+    terms, packed."""
 
-    __slots__ = ("x", "mask", "temperature", "terms", "keep", "ws", "nbytes", "backward")
+    what: str
+    forward: object
+    backward: object
+    inputs: object
+    terms: object
 
-    def __init__(self, x, mask, temperature, terms, keep, backward, what):
-        temperature = float(temperature)
-        if not 1e-6 <= temperature <= 1e6:
-            raise ValueError(f"{what}: the temperature must lie in [1e-6, 1e6]")
-        self.x, self.mask, self.temperature = x, mask, temperature
-        self.terms, self.keep, self.backward = terms, keep, backward
-        b, n, _ = x.shape
-        self.nbytes = lib.pkv_loss_workspace_bytes(b, n)
-        if self.nbytes < 0:
-            raise ValueError(f"{what}: too many rows")
-        self.ws = torch.empty(self.nbytes, dtype=torch.uint8, device=x.device)
 
-    def rows(self, grad: torch.Tensor | None) -> bytes:
-        x = self.x
-        return _ROWS.pack(*_array(x), *_array(grad), *_array(self.mask), *x.shape, _DTYPES[x.dtype], self.temperature)
+class _Call(NamedTuple):
+    """One loss call, apart from its tensors: a differentiable call's graph node keeps it, and what that node keeps of
+    tensors are saved ones alone (freed by the backward pass, and seen by saved-tensor hooks)."""
+
+    kind: _Kind
+    numbers: tuple
+    temperature: float
+
+
+class _Tensors(NamedTuple):
+    """A call's tensors: rows [B, T, V], mask, the terms' inputs, outputs, and the workspace a backward pass reads."""
+
+    x: torch.Tensor
+    mask: torch.Tensor | None
+    inputs: tuple
+    outputs: tuple
+    ws: torch.Tensor
+
+
+def _temperature(temperature: float, what: str) -> float:
+    temperature = float(temperature)
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"{what}: the temperature must lie in [1e-6, 1e6]")
+    return temperature
+
+
+def _workspace(batch: int, length: int, dev: torch.device, what: str) -> torch.Tensor:
+    nbytes = lib.pkv_loss_workspace_bytes(batch, length)
+    if nbytes < 0:
+        raise ValueError(f"{what}: too many rows")
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
 
 
 def _on_device(x: torch.Tensor, fn, *args) -> None:
@@ -197,68 +217,119 @@ def _on_device(x: torch.Tensor, fn, *args) -> None:
         _lib.raise_for_status(st)
 
 
-def _launch(fn, c: _Call, grad, outputs: tuple) -> None:
+def _launch(fn, x: torch.Tensor, temperature: float, grad: torch.Tensor | None, mask: tuple, terms: bytes,
+            outputs: tuple, ws: torch.Tensor) -> None:
     """``fn(rows, terms, *outputs, workspace)`` on the logits' device and its current stream."""
-    _on_device(c.x, fn, c.rows(grad), c.terms, *[None if t is None else t.data_ptr() for t in outputs],
-               c.ws.data_ptr(), c.nbytes)
+    rows = _ROWS.pack(*_array(x), *_array(grad), *mask, *x.shape, _DTYPES[x.dtype], temperature)
+    _on_device(x, fn, rows, terms, *[None if o is None else o.data_ptr() for o in outputs], ws.data_ptr(), ws.numel())
+
+
+def _forward(c: _Call, t: _Tensors, grad: torch.Tensor | None) -> tuple:
+    """The forward call; its packed mask and terms."""
+    kind = c.kind
+    mask, terms = _array(t.mask), kind.terms(c.numbers, *t.inputs)
+    _launch(kind.forward, t.x, c.temperature, grad, mask, terms, t.outputs, t.ws)
+    return mask, terms
+
+
+def _unpacked(kind: _Kind, shape: torch.Size, dtype: torch.dtype, dev: torch.device, logits, mask, ws, inputs) -> tuple:
+    """(rows, mask, inputs, workspace) of saved tensors that are not the call's own any more (a hook moved them to the
+    host and back, or they were computed anew), checked as those were: the kernels would read past smaller ones."""
+    if logits.shape != shape or logits.dtype != dtype or logits.device != dev:
+        raise ValueError(f"logits {tuple(logits.shape)} of {logits.dtype} on {logits.device}")
+    if ws.device != dev or ws.dtype != torch.uint8:
+        raise ValueError("another workspace")
+    x = logits if len(shape) == 3 else logits.unsqueeze(0)
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    rows = x.shape[:2]
+    return x, _mask(mask, rows, dev, kind.what), kind.inputs(rows, dev, kind.what, *inputs), ws.contiguous()
 
 
 class _RowLoss(torch.autograd.Function):
     """Forward: the loss call without a gradient.  Backward: the rows again, times the upstream gradient."""
 
     @staticmethod
-    def forward(ctx, logits, call, fn, outputs):
-        _launch(fn, call, None, outputs)
-        ctx.call = call
-        ctx.save_for_backward(logits, call.ws, *[t for t in call.keep if t is not None])
-        return outputs[0]
+    def forward(ctx, logits, call, t):
+        at = logits.data_ptr(), logits.stride(), t.ws.data_ptr(), _forward(call, t, None)
+        ctx.call = call, at, logits.shape, logits.dtype, t.x.device
+        ctx.save_for_backward(logits, t.mask, t.ws, *t.inputs)
+        return t.outputs[0]
 
     @staticmethod
     def backward(ctx, grad_loss):
         if torch.is_grad_enabled():  # (create_graph=True)
             raise RuntimeError("the vocabulary-row losses are differentiable once")
-        logits = ctx.saved_tensors[0]  # (also checks that nothing was changed in place since)
-        c = ctx.call
-        grad = _grad_like(c.x)
-        if grad_loss.dtype != torch.float32 or grad_loss.device != c.x.device:
-            grad_loss = grad_loss.to(dtype=torch.float32, device=c.x.device)
-        _launch(c.backward, c, grad, (grad_loss,))
-        return grad if grad.dim() == logits.dim() else grad.squeeze(0), None, None, None
+        (kind, numbers, temperature), at, shape, dtype, dev = ctx.call
+        logits, mask, ws, *inputs = ctx.saved_tensors  # (also checks that nothing was changed in place since)
+        try:
+            packed = _array(mask), kind.terms(numbers, *inputs)
+        except (ValueError, IndexError):  # (not even of as many dims)
+            packed = None
+        own = (logits.data_ptr(), logits.stride(), ws.data_ptr(), packed) == at
+        if own and logits.shape == shape and logits.dtype == dtype:
+            x = logits if len(shape) == 3 else logits.unsqueeze(0)
+        else:
+            try:
+                x, mask, inputs, ws = _unpacked(kind, shape, dtype, dev, logits, mask, ws, inputs)
+            except ValueError as e:
+                raise RuntimeError(f"{kind.what}: a saved-tensor hook gave back something else: {e}") from e
+            packed = _array(mask), kind.terms(numbers, *inputs)
+        grad = _grad_like(x)
+        if grad_loss.dtype != torch.float32 or grad_loss.device != dev:
+            grad_loss = grad_loss.to(dtype=torch.float32, device=dev)
+        _launch(kind.backward, x, temperature, grad, *packed, (grad_loss,), ws)
+        return grad if len(shape) == 3 else grad.squeeze(0), None, None
 
 
-def _run(fn, c: _Call, logits: torch.Tensor, outputs: tuple):
+def _run(c: _Call, logits: torch.Tensor, t: _Tensors) -> tuple:
     """The outputs of a differentiable call: the loss, and per-row values without a gradient."""
     if logits.requires_grad and torch.is_grad_enabled():
-        return (_RowLoss.apply(logits, c, fn, outputs), *outputs[1:])
-    _launch(fn, c, None, outputs)
-    return outputs
+        return (_RowLoss.apply(logits, c, t), *t.outputs[1:])
+    _forward(c, t, None)
+    return t.outputs
 
 
-def _run_with_grad(fn, c: _Call, logits: torch.Tensor, outputs: tuple) -> torch.Tensor:
-    grad = _grad_like(c.x)
-    _launch(fn, c, grad, outputs)
+def _run_with_grad(c: _Call, logits: torch.Tensor, t: _Tensors) -> torch.Tensor:
+    grad = _grad_like(t.x)
+    _forward(c, t, grad)
     return grad if grad.dim() == logits.dim() else grad.squeeze(0)
+
+
+def _policy_inputs(rows, dev, what, tokens, advantages, old_logprobs, ref_logprobs) -> tuple:
+    tok = _rows_like(tokens, rows, dev, torch.int64, what, "tokens")
+    adv = _advantages(advantages, rows, dev, what)
+    old = None if old_logprobs is None else _rows_like(old_logprobs, rows, dev, torch.float32, what, "old_logprobs")
+    ref = None if ref_logprobs is None else _rows_like(ref_logprobs, rows, dev, torch.float32, what, "ref_logprobs")
+    return tok, adv, old, ref
+
+
+def _policy_terms(numbers, tok, adv, old, ref) -> bytes:
+    each = adv.data_ptr(), adv.stride(0), adv.stride(1) if adv.shape == tok.shape else 0
+    return _POLICY.pack(*_array(tok), *each, *_array(old), *_array(ref), *numbers)
+
+
+_POLICY_KIND = _Kind("policy_loss", lib.pkv_policy_loss, lib.pkv_policy_loss_backward, _policy_inputs,
+                    _policy_terms)
 
 
 def _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef, entropy_coef,
             temperature, reduction, scale):
-    what = "policy_loss"
+    what = _POLICY_KIND.what
     x = _logits(logits, what)
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError(f"{what}: clip_low and clip_high must be >= 0")
     rows, dev = x.shape[:2], x.device
-    tok = _rows_like(tokens, rows, dev, torch.int64, what, "tokens")
-    adv, adv_array = _advantages(advantages, rows, dev, what)
-    old = None if old_logprobs is None else _rows_like(old_logprobs, rows, dev, torch.float32, what, "old_logprobs")
-    ref = None if ref_logprobs is None else _rows_like(ref_logprobs, rows, dev, torch.float32, what, "ref_logprobs")
+    inputs = _policy_inputs(rows, dev, what, tokens, advantages, old_logprobs, ref_logprobs)
     m = _mask(mask, rows, dev, what)
-    terms = _POLICY.pack(*_array(tok), *adv_array, *_array(old), *_array(ref), clip_low, clip_high, kl_coef,
-                         entropy_coef, _reduction(reduction, what), scale)
-    c = _Call(x, m, temperature, terms, (tok, adv, old, ref, m), lib.pkv_policy_loss_backward, what)
+    numbers = (float(clip_low), float(clip_high), float(kl_coef), float(entropy_coef), _reduction(reduction, what),
+               float(scale))
+    c = _Call(_POLICY_KIND, numbers, _temperature(temperature, what))
+    ws = _workspace(*rows, dev, what)
     lp = torch.empty(*logits.shape[:-1], dtype=torch.float32, device=dev)
-    outputs = (lp.new_empty(()), lp, None if ref is None else torch.empty_like(lp),
+    outputs = (lp.new_empty(()), lp, None if ref_logprobs is None else torch.empty_like(lp),
                torch.empty_like(lp) if entropy_coef else None)
-    return c, outputs
+    return c, _Tensors(x, m, inputs, outputs, ws)
 
 
 def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Tensor,
@@ -276,9 +347,9 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Te
     r is 1, with the gradient of lp.  ``reduction``: "token_mean" over all scored rows, "sequence_mean" the mean over
     sequences with a scored row of their rows' mean, or "sum".  All inputs but ``logits`` are constants.
     """
-    c, outputs = _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef,
-                         entropy_coef, temperature, reduction, scale)
-    return PolicyLoss(*_run(lib.pkv_policy_loss, c, logits, outputs))
+    c, t = _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef,
+                   entropy_coef, temperature, reduction, scale)
+    return PolicyLoss(*_run(c, logits, t))
 
 
 def policy_loss_and_grad(logits: torch.Tensor, tokens: torch.Tensor, advantages: torch.Tensor,
@@ -287,32 +358,45 @@ def policy_loss_and_grad(logits: torch.Tensor, tokens: torch.Tensor, advantages:
                          kl_coef: float = 0.0, entropy_coef: float = 0.0, temperature: float = 1.0,
                          reduction: str = "token_mean", scale: float = 1.0) -> tuple[PolicyLoss, torch.Tensor]:
     """``policy_loss`` and its gradient with respect to ``logits`` (their type), in one pass over HBM."""
-    c, outputs = _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef,
-                         entropy_coef, temperature, reduction, scale)
-    grad = _run_with_grad(lib.pkv_policy_loss, c, logits, outputs)
-    return PolicyLoss(*outputs), grad
+    c, t = _policy(logits, tokens, advantages, old_logprobs, mask, ref_logprobs, clip_low, clip_high, kl_coef,
+                   entropy_coef, temperature, reduction, scale)
+    grad = _run_with_grad(c, logits, t)
+    return PolicyLoss(*t.outputs), grad
+
+
+def _preference_inputs(rows, dev, what, tokens, ref) -> tuple:
+    tok = _rows_like(tokens, rows, dev, torch.int64, what, "tokens")
+    if ref is not None:
+        if not isinstance(ref, torch.Tensor) or ref.device != dev or tuple(ref.shape) != (rows[0],):
+            raise ValueError(f"{what}: ref_logprobs must be [2 * pairs] on the logits' device")
+        ref = ref.to(torch.float32).contiguous()
+    return tok, ref
+
+
+def _preference_terms(numbers, tok, ref) -> bytes:
+    return _PREFERENCE.pack(*_array(tok), 0 if ref is None else ref.data_ptr(), *numbers)
+
+
+_PREFERENCE_KIND = _Kind("preference_loss", lib.pkv_preference_loss, lib.pkv_preference_loss_backward,
+                         _preference_inputs, _preference_terms)
 
 
 def _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, length_normalised, scale):
-    what = "preference_loss"
+    what = _PREFERENCE_KIND.what
     x = _logits(logits, what)
     if logits.dim() != 3 or x.shape[0] % 2:
         raise ValueError(f"{what}: logits must be [2 * pairs, length, vocab], the chosen answers first")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"{what}: label_smoothing must lie in [0, 1]")
     rows, dev = x.shape[:2], x.device
-    tok = _rows_like(tokens, rows, dev, torch.int64, what, "tokens")
+    inputs = _preference_inputs(rows, dev, what, tokens, ref_logprobs)
     m = _mask(mask, rows, dev, what)
-    ref = ref_logprobs
-    if ref is not None:
-        if not isinstance(ref, torch.Tensor) or ref.device != x.device or tuple(ref.shape) != (x.shape[0],):
-            raise ValueError(f"{what}: ref_logprobs must be [2 * pairs] on the logits' device")
-        ref = ref.to(torch.float32).contiguous()
-    terms = _PREFERENCE.pack(*_array(tok), 0 if ref is None else ref.data_ptr(), beta, label_smoothing,
-                             int(bool(length_normalised)), scale)
-    c = _Call(x, m, 1.0, terms, (tok, ref, m), lib.pkv_preference_loss_backward, what)
+    numbers = (float(beta), float(label_smoothing), int(bool(length_normalised)), float(scale))
+    c = _Call(_PREFERENCE_KIND, numbers, 1.0)
+    ws = _workspace(*rows, dev, what)
     sums = torch.empty(rows[0], dtype=torch.float32, device=dev)
-    return c, (sums.new_empty(()), sums, torch.empty(rows[0] // 2, dtype=torch.float32, device=dev))
+    outputs = sums.new_empty(()), sums, torch.empty(rows[0] // 2, dtype=torch.float32, device=dev)
+    return c, _Tensors(x, m, inputs, outputs, ws)
 
 
 def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | None = None,
@@ -328,8 +412,8 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tens
 
     averaged over the pairs.  A sequence without a scored row has S = 0.
     """
-    c, outputs = _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, length_normalised, scale)
-    return PreferenceLoss(*_run(lib.pkv_preference_loss, c, logits, outputs))
+    c, t = _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, length_normalised, scale)
+    return PreferenceLoss(*_run(c, logits, t))
 
 
 def preference_loss_and_grad(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | None = None,
@@ -337,43 +421,57 @@ def preference_loss_and_grad(logits: torch.Tensor, tokens: torch.Tensor, mask: t
                              label_smoothing: float = 0.0, length_normalised: bool = False,
                              scale: float = 1.0) -> tuple[PreferenceLoss, torch.Tensor]:
     """``preference_loss`` and its gradient with respect to ``logits`` (their type)."""
-    c, outputs = _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, length_normalised, scale)
-    grad = _run_with_grad(lib.pkv_preference_loss, c, logits, outputs)
-    return PreferenceLoss(*outputs), grad
+    c, t = _preference(logits, tokens, mask, ref_logprobs, beta, label_smoothing, length_normalised, scale)
+    grad = _run_with_grad(c, logits, t)
+    return PreferenceLoss(*t.outputs), grad
 
 
-def _teacher_list(t: torch.Tensor, lead: torch.Size, dev: torch.device, dtype: torch.dtype, what: str,
+def _teacher_list(t: torch.Tensor, rows: torch.Size, dev: torch.device, dtype: torch.dtype, what: str,
                   name: str) -> torch.Tensor:
-    """A teacher's list [..., k] of the rows ``lead`` as [B, T, k] of ``dtype`` with contiguous entries."""
+    """A teacher's list as [B, T, k] (``rows`` and k; [T, k] for one sequence) of ``dtype`` with contiguous entries."""
     if not isinstance(t, torch.Tensor) or t.device != dev:
         raise ValueError(f"{what}: {name} must be on the logits' device")
+    if t.dim() == 2 and rows[0] == 1:
+        t = t.unsqueeze(0)
     shape = t.shape
-    if len(shape) != len(lead) + 1 or shape[:-1] != lead or not 1 <= shape[-1] <= _MAX_TOP:
-        raise ValueError(f"{what}: {name} must be {list(lead)} + [k], k from 1 to {_MAX_TOP}, got {tuple(shape)}")
+    if len(shape) != 3 or shape[:-1] != rows or not 1 <= shape[-1] <= _MAX_TOP:
+        raise ValueError(f"{what}: {name} must be {list(rows)} + [k], k from 1 to {_MAX_TOP}, got {tuple(shape)}")
     if t.dtype != dtype:
         if dtype == torch.int64 and (t.is_floating_point() or t.dtype == torch.bool):
             raise ValueError(f"{what}: {name} must be integers")
         t = t.to(dtype)
     if t.stride(-1) != 1 and shape[-1] > 1:
         t = t.contiguous()
-    return t.unsqueeze(0) if len(shape) == 2 else t
+    return t
 
 
-def _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale):
-    what = "distillation_loss"
-    x = _logits(logits, what)
-    lead, rows, dev = logits.shape[:-1], x.shape[:2], x.device
-    ids = _teacher_list(teacher_ids, lead, dev, torch.int64, what, "teacher_ids")
-    tl = _teacher_list(teacher_logits, lead, dev, torch.float32, what, "teacher_logits")
+def _distillation_inputs(rows, dev, what, teacher_ids, teacher_logits, teacher_lse) -> tuple:
+    ids = _teacher_list(teacher_ids, rows, dev, torch.int64, what, "teacher_ids")
+    tl = _teacher_list(teacher_logits, rows, dev, torch.float32, what, "teacher_logits")
     if ids.shape != tl.shape:
         raise ValueError(f"{what}: teacher_ids and teacher_logits must have the same shape")
     lse = None if teacher_lse is None else _rows_like(teacher_lse, rows, dev, torch.float32, what, "teacher_lse")
+    return ids, tl, lse
+
+
+def _distillation_terms(numbers, ids, tl, lse) -> bytes:
+    return _DISTILLATION.pack(*_array(ids), *_array(tl), ids.shape[-1], *_array(lse), *numbers)
+
+
+_DISTILLATION_KIND = _Kind("distillation_loss", lib.pkv_distillation_loss, lib.pkv_distillation_loss_backward,
+                           _distillation_inputs, _distillation_terms)
+
+
+def _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale):
+    what = _DISTILLATION_KIND.what
+    x = _logits(logits, what)
+    rows, dev = x.shape[:2], x.device
+    inputs = _distillation_inputs(rows, dev, what, teacher_ids, teacher_logits, teacher_lse)
     m = _mask(mask, rows, dev, what)
-    terms = _DISTILLATION.pack(*_array(ids), *_array(tl), ids.shape[-1], *_array(lse), _reduction(reduction, what),
-                               scale)
-    c = _Call(x, m, temperature, terms, (ids, tl, lse, m), lib.pkv_distillation_loss_backward, what)
-    kl = torch.empty(*lead, dtype=torch.float32, device=dev)
-    return c, (kl.new_empty(()), kl)
+    c = _Call(_DISTILLATION_KIND, (_reduction(reduction, what), float(scale)), _temperature(temperature, what))
+    ws = _workspace(*rows, dev, what)
+    kl = torch.empty(*logits.shape[:-1], dtype=torch.float32, device=dev)
+    return c, _Tensors(x, m, inputs, (kl.new_empty(()), kl), ws)
 
 
 def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
@@ -391,8 +489,8 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     and 0 for a row whose entries are all absent (it counts in the means).  An id past the vocabulary makes the
     loss and its row's gradient NaN.  ``reduction`` as in ``policy_loss``.
     """
-    c, outputs = _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale)
-    return DistillationLoss(*_run(lib.pkv_distillation_loss, c, logits, outputs))
+    c, t = _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale)
+    return DistillationLoss(*_run(c, logits, t))
 
 
 def distillation_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
@@ -400,9 +498,9 @@ def distillation_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, 
                                temperature: float = 1.0, reduction: str = "token_mean",
                                scale: float = 1.0) -> tuple[DistillationLoss, torch.Tensor]:
     """``distillation_loss`` and its gradient with respect to ``logits`` (their type), in one pass over HBM."""
-    c, outputs = _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale)
-    grad = _run_with_grad(lib.pkv_distillation_loss, c, logits, outputs)
-    return DistillationLoss(*outputs), grad
+    c, t = _distillation(logits, teacher_ids, teacher_logits, mask, teacher_lse, temperature, reduction, scale)
+    grad = _run_with_grad(c, logits, t)
+    return DistillationLoss(*t.outputs), grad
 
 
 def top_logits(logits: torch.Tensor, k: int, *,
@@ -415,9 +513,7 @@ def top_logits(logits: torch.Tensor, k: int, *,
     k = int(k)
     if not 1 <= k <= min(_MAX_TOP, x.shape[-1]):
         raise ValueError(f"{what}: k must be from 1 to {min(_MAX_TOP, x.shape[-1])}")
-    temperature = float(temperature)
-    if not 1e-6 <= temperature <= 1e6:
-        raise ValueError(f"{what}: the temperature must lie in [1e-6, 1e6]")
+    temperature = _temperature(temperature, what)
     shape = logits.shape[:-1]
     values = torch.empty(*shape, k, dtype=torch.float32, device=x.device)
     tokens = torch.empty(*shape, k, dtype=torch.int64, device=x.device)

@@ -227,3 +227,85 @@ def test_an_error_of_the_preference_sums_is_loud(cuda_device):
             break
     assert out.isnan().all()
     assert grad[0, 0].isnan().all() and grad[1, -1].isnan().all()
+
+
+def _differentiable_calls(dev):
+    """(name, call) of the three losses over rows [2, 4, 301], with inputs that need no conversion and some that do."""
+    from randomrepo_b200 import losses
+
+    g = torch.Generator().manual_seed(12)
+    tokens = torch.randint(0, 301, (2, 4), generator=g).to(dev)
+    old = (-6 + torch.randn(2, 4, generator=g)).to(dev)
+    adv = torch.randn(2, generator=g).to(dev)
+    mask = (torch.rand(4, 2, generator=g) < 0.8).to(dev).t()
+    ids = torch.randint(0, 301, (2, 4, 6), generator=g).to(dev)
+    teacher = torch.randn(2, 4, 12, generator=g).to(dev)[..., ::2]
+    ref = torch.randn(2, generator=g).to(dev)
+    return [lambda z: losses.policy_loss(z, tokens, adv, old, mask, ref_logprobs=old + 0.1, kl_coef=0.1, temperature=0.8),
+            lambda z: losses.policy_loss(z, tokens.int(), adv.unsqueeze(1), old.double(), mask.long(), entropy_coef=0.1),
+            lambda z: losses.preference_loss(z, tokens, mask, ref, beta=0.3, length_normalised=True),
+            lambda z: losses.distillation_loss(z, ids, teacher, mask, temperature=2.0),
+            lambda z: losses.distillation_loss(z, ids.int(), teacher, None, teacher_lse=old.abs())]
+
+
+def test_the_backward_pass_frees_the_logits(cuda_device):
+    """The loss may outlive its backward pass (a log keeps it); the logits and the workspace do not."""
+    g = torch.Generator().manual_seed(1)
+    head = torch.randn(2, 4, 301, generator=g).to(cuda_device).requires_grad_()
+    for call in _differentiable_calls(cuda_device):
+        call(head).loss.backward()  # (head.grad is there from now on)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        logits = head * 1.5
+        size = torch.cuda.memory_allocated() - before
+        out = call(logits)
+        del logits
+        out.loss.backward()
+        # What is left: the loss and the rows' values, 512 bytes each at the least.
+        assert torch.cuda.memory_allocated() - before <= 4 * 512 < size
+        assert out.loss.isfinite()
+        head.grad = torch.zeros_like(head)
+
+
+def test_saved_tensor_hooks_are_heard(cuda_device):
+    """Tensors that were offloaded to the host come back for the backward pass; recomputed ones likewise."""
+    from torch.utils.checkpoint import checkpoint
+
+    g = torch.Generator().manual_seed(6)
+    data = torch.randn(2, 4, 301, generator=g).to(cuda_device)
+    for call in _differentiable_calls(cuda_device):
+        leaf = data.clone().requires_grad_()
+        (want,) = torch.autograd.grad(call(leaf * 1.5).loss, leaf)
+        before = torch.cuda.memory_allocated()
+        with torch.autograd.graph.save_on_cpu():
+            logits = leaf * 1.5
+            out = call(logits)
+        size = logits.numel() * 4
+        del logits
+        assert torch.cuda.memory_allocated() - before < size  # (the logits are on the host alone)
+        (got,) = torch.autograd.grad(out.loss, leaf)
+        assert torch.equal(got, want)
+        (got,) = torch.autograd.grad(checkpoint(lambda z: call(z * 1.5).loss, leaf, use_reentrant=False), leaf)
+        assert torch.equal(got, want)
+
+        # What a hook hands back is what is read.
+        def double(t):
+            return t * 2 if t.shape == data.shape else t
+
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), double):
+            out = call(leaf)
+        (got,) = torch.autograd.grad(out.loss, leaf)
+        assert not torch.equal(got, torch.autograd.grad(call(leaf).loss, leaf)[0])
+
+        # Another shape, type or device than was saved would be read out of bounds: refused before a launch.
+        for wrong in (lambda t: t.cpu(), lambda t: t[:1] if t.dim() == 3 else t, lambda t: t.double()):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), wrong):
+                out = call(leaf)
+            with pytest.raises(RuntimeError, match="hook"):
+                torch.autograd.grad(out.loss, leaf)
+        # The same values in another order of memory are taken.
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), lambda t: t.mT.contiguous().mT if t.dim() > 1 else
+                                                      t.repeat_interleave(2)[::2] if t.dtype != torch.uint8 else t):
+            out = call(leaf)
+        (got,) = torch.autograd.grad(out.loss, leaf)
+        torch.testing.assert_close(got, torch.autograd.grad(call(leaf).loss, leaf)[0], atol=0, rtol=0)

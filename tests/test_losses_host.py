@@ -253,3 +253,27 @@ def test_the_rings_order_never_waits_for_itself(slots):
                 if done:
                     free.add(place[chunk])
             assert len(free) == len(copies)
+
+
+def test_the_graph_holds_no_tensor_beside_the_saved_ones(monkeypatch):
+    """What a differentiable call leaves on its graph node is saved tensors: they go with the backward pass and pass
+    through saved-tensor hooks.  (The launches are left out.)"""
+    from torch.multiprocessing.reductions import StorageWeakRef
+
+    packed = []
+    monkeypatch.setattr(losses, "_on_device", lambda x, fn, *args: packed.append((fn, args)))
+    tok, adv, per_row = torch.zeros(2, 3, dtype=torch.int64), torch.ones(2), torch.zeros(2, 3)
+    ids = torch.zeros(2, 3, 4, dtype=torch.int64)
+    for call in (lambda z: losses.policy_loss(z, tok, adv, per_row, per_row != 1, ref_logprobs=per_row),
+                 lambda z: losses.preference_loss(z, tok, None, adv),
+                 lambda z: losses.distillation_loss(z, ids, ids.float(), None, teacher_lse=per_row)):
+        x = torch.randn(2, 3, 8).requires_grad_()
+        logits = _fake(x * 2)
+        gone = StorageWeakRef(logits.untyped_storage())
+        loss = call(logits).loss
+        del logits
+        assert not gone.expired()
+        packed.clear()
+        (grad,) = torch.autograd.grad(loss, x)
+        assert gone.expired() and grad.shape == x.shape
+        assert len(packed) == 1
