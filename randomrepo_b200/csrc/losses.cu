@@ -554,8 +554,9 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
       const float4 rec = A.rec[row];
       const float f = up * (A.seq_g ? A.seq_g[b] : 1.f);
       if (KIND == kDistill) {
-        o = RowGrad{rec.x, rec.y * f, 0.f, 0.f, -1, f == 0.f};
         wt = rec.z * f;
+        o = RowGrad{rec.x, rec.y * f, 0.f, 0.f, -1, false};
+        o.zero = f == 0.f || (o.a == 0.f && wt == 0.f);  // (the second: no share in the list)
       } else {
         o = RowGrad{rec.x, rec.y * f, rec.z * f, rec.w * f, known ? (int)q.tok : -1, false};
         o.zero = o.a == 0.f && o.b == 0.f && o.h == 0.f;
@@ -591,18 +592,21 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
       } else {
         wait_or_mark(&sh.teacher_full[par], phase, sh);
         const auto& te = sh.teacher[par];
-        // sum q (log q - log p), log p = (x k + c - log2 s) ln 2
+        // sum q (log q - log p), log p = (x k + c - log2 s) ln 2.  Where no entry has a share (none is there, or all
+        // underflow) that is 0 and so is the gradient, whatever the row's columns are.
         const double w = (double)q.w, tt = (double)A.temperature;
+        const bool none = te.q_sum == 0.0 && te.qx == te.qx;
         const float c = center(a.m, ks);
         double qp = te.qx * A.kd + te.q_sum * ((double)c - log2_sum(a.s));  // sum q log2 p
-        if (far_out(c) && qp == qp) {
+        if (far_out(c) && te.qx == te.qx) {
           qp = 0.0;
           for (int f = 0; f < A.k; ++f)
             if (te.id[f] >= 0 && te.q[f] > 0.f) qp += (double)te.q[f] * log2_prob(A, a, as_float(x[te.id[f]]));
         }
-        const double l = tt * tt * (te.qlogq - qp * kLn2d);
-        wt = (float)(w * tt);
-        o = RowGrad{a.m, l == l ? wt * (float)te.q_sum / a.s : NAN, 0.f, 0.f, -1, false};
+        const double l = none ? 0.0 : tt * tt * (te.qlogq - qp * kLn2d);
+        wt = none ? 0.f : (float)(w * tt);
+        o = RowGrad{a.m, l == l ? wt * (float)te.q_sum / a.s : NAN, 0.f, 0.f, -1, none};
+        if (none) o.a = 0.f;  // (not 0 / s)
         if (write) {
           A.kl_out[row] = (float)l;
           A.row_val[row] = w * l;

@@ -309,3 +309,50 @@ def test_saved_tensor_hooks_are_heard(cuda_device):
             out = call(leaf)
         (got,) = torch.autograd.grad(out.loss, leaf)
         torch.testing.assert_close(got, torch.autograd.grad(call(leaf).loss, leaf)[0], atol=0, rtol=0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_rows_without_a_teacher_entry(cuda_device, dtype):
+    """A scored row whose entries are all absent (or have no share left) adds nothing and has a zero gradient, whatever
+    its logits are: the lowest value, -inf, NaN in every column.  A NaN share and an id past the vocabulary stay loud."""
+    from randomrepo_b200 import losses
+
+    v, k = 300, 5
+    g = torch.Generator().manual_seed(3)
+    fills = [torch.finfo(dtype).min, -math.inf, math.nan, math.inf, torch.finfo(dtype).max, 0.0]
+    x = torch.randn(len(fills) + 1, 2, v, generator=g)
+    for i, f in enumerate(fills):
+        x[i, 1] = f
+    x = x.to(dtype).to(cuda_device)
+    ids = torch.randint(0, v, (len(fills) + 1, 2, k), generator=g).to(cuda_device)
+    teacher = torch.randn(len(fills) + 1, 2, k, generator=g).to(cuda_device)
+    absent, low = ids.clone(), teacher.clone()
+    absent[:, 1] = -1
+    low[:, 1] = -math.inf
+    far = torch.zeros(len(fills) + 1, 2, device=cuda_device)
+    far[:, 1] = 1e30  # (the teacher's row has all its mass elsewhere: every share underflows)
+    rows = x[:, 0].double()
+    for i, t, lse in ((absent, teacher, None), (ids, low, None), (ids, teacher, far)):
+        q = torch.softmax(t[:, 0].double(), -1) if lse is None else t[:, 0].double().exp()
+        lq = q.log()
+        per = (q * (lq - torch.log_softmax(rows, -1).gather(-1, i[:, 0]))).sum(-1)
+        want = torch.softmax(rows, -1) * q.sum(-1, keepdim=True)
+        want.scatter_add_(-1, i[:, 0], -q)
+        got, grad = losses.distillation_loss_and_grad(x, i, t, teacher_lse=lse, reduction="sum")
+        leaf = x.detach().requires_grad_()
+        out = losses.distillation_loss(leaf, i, t, teacher_lse=lse, reduction="sum")
+        (own,) = torch.autograd.grad(out.loss, leaf)
+        for res, d in ((got, grad), (out, own)):
+            empty = [r for r in range(len(fills) + 1) if lse is None or r != 2]  # (a share of 0 times NaN is NaN)
+            assert (res.kl[empty, 1] == 0).all() and (d[empty, 1] == 0).all()
+            if lse is not None:
+                assert res.kl[2, 1].isnan() and res.loss.isnan() and d[2, 1].isnan().all()
+                continue
+            # (a share and a log-probability are off by at most 2e-5 of a term, as in the other tests of this loss)
+            size = (q * (lq.abs() + 20)).sum(-1)
+            assert ((res.kl[:, 0].double() - per).abs() <= 2.5e-5 * size).all()
+            assert abs(float(res.loss.detach()) - float(per.sum())) <= 2.5e-5 * float(size.sum())
+            assert ((d[:, 0].double() - want).abs() <= want.abs() * _half(dtype) + 2.5e-5 * q.sum(-1, keepdim=True)).all()
+    ids[0, 1], teacher[1, 1, 2] = v, math.nan
+    for f in (losses.distillation_loss_and_grad(x, ids, teacher)[0], losses.distillation_loss(x, ids, teacher)):
+        assert f.loss.isnan() and f.kl[:2, 1].isnan().all()
