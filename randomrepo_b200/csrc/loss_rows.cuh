@@ -68,13 +68,12 @@ struct RowSum {
 
 // d: the exponent that takes sums from a reference m to a larger one.
 __device__ __forceinline__ float rescale_exponent(float m, float m_new, Scale2 k) {
-  if (m == -INFINITY) return -INFINITY;
   const float c = center(m_new, k), from = center(m, k);
-  if (far_out(c) != far_out(from)) {  // (what stays in c is in the y of one of them alone)
-    const float n = far_out(c) ? m : m_new, in_c = far_out(c) ? from : c, stays = fmaf(n, k.lo, fmaf(n, k.hi, in_c));
-    return (m - m_new) * k.hi + (far_out(c) ? -stays : stays);
-  }
-  return far_out(c) ? (m - m_new) * k.hi : c - from;
+  if (!far_out(c) && (!far_out(from) || m == -INFINITY)) return c - from;
+  if (far_out(c) && (far_out(from) || m == -INFINITY)) return (m - m_new) * k.hi;
+  // One on each side: what stays in c is in the y of one of them alone.
+  const float n = far_out(c) ? m : m_new, in_c = far_out(c) ? from : c, stays = fmaf(n, k.lo, fmaf(n, k.hi, in_c));
+  return (m - m_new) * k.hi + (far_out(c) ? -stays : stays);
 }
 
 __device__ __forceinline__ void sum_rescale(RowSum& a, float m_new, float d, float f) {
