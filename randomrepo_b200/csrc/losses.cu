@@ -96,8 +96,14 @@ struct RowTerms {
   float x_tok, w, adv, old, ref;
 };
 
+// A row's values beside its gradient: log p, d = ref - log p, the loss without its KL term, the entropy.
+struct PolicyRow {
+  double lp, d;
+  float l, h;
+};
+
 template <bool ENT>
-__device__ __forceinline__ RowGrad policy_tail(const LossArgs& A, int row, RowSum r, const RowTerms& q, bool write) {
+__device__ __forceinline__ RowGrad policy_tail(const LossArgs& A, RowSum r, const RowTerms& q, PolicyRow& v) {
   const int64_t tok = q.tok;
   const bool known = tok >= 0 && tok < A.vocab;
   const double log2s = log2_sum(r.s);
@@ -110,34 +116,37 @@ __device__ __forceinline__ RowGrad policy_tail(const LossArgs& A, int row, RowSu
   float l = adv == 0.f ? 0.f : -used * adv;
   float g = (cut || adv == 0.f) ? 0.f : -ratio * adv;
   if (!(lp == lp)) l = g = NAN;
-  float kl = 0.f;
-  if (A.ref.p) {
-    const float d = (float)((double)q.ref - lp);
-    const float em = expm1f(d);
-    kl = em - d;
-    l = fmaf(A.kl_coef, kl, l);
-    g = fmaf(-A.kl_coef, em, g);
-  }
+  v.lp = lp, v.d = (double)q.ref - lp, v.h = 0.f;
+  if (A.ref.p) g = fmaf(-A.kl_coef, expm1f((float)v.d), g);
   g *= w * A.inv_t;
   const float inv_s = 1.f / r.s;
   RowGrad o{r.m, -g * inv_s, 0.f, g, known ? (int)tok : -1, false};
-  float h = 0.f;
   if (ENT) {
     const double mean = (double)r.w / (double)r.s;
-    h = (float)((log2s - mean) * kLn2d);
+    v.h = (float)((log2s - mean) * kLn2d);
     const float c = A.ent_coef * w * A.inv_t;
-    l = fmaf(-A.ent_coef, h, l);
+    l = fmaf(-A.ent_coef, v.h, l);
     o.a = fmaf(c * inv_s, (float)(-kLn2d * mean), o.a);  // H - ln2 log2 s = -ln2 w / s
     o.b = c * kLn2 * inv_s;
   }
   o.zero = !ENT && g == 0.f;
-  if (write) {
-    A.logprobs[row] = (float)lp;
-    if (A.kl_out) A.kl_out[row] = kl;
-    if (ENT && A.entropy) A.entropy[row] = h;
-    A.row_val[row] = (double)w * (double)l;
-  }
+  v.l = l;
   return o;
+}
+
+// Written when the gradient's coefficients are on their way.  The KL estimate e^d - d - 1 in 64 bits: near the
+// reference it is d^2 / 2, of which a float32 difference has no digits left below d = 1e-7 (and 1e-4 of it at 1e-3).
+template <bool ENT>
+__device__ __forceinline__ void write_policy(const LossArgs& A, int row, float w, const PolicyRow& v) {
+  float l = v.l, kl = 0.f;
+  if (A.ref.p) {
+    kl = (float)(expm1(v.d) - v.d);
+    l = fmaf(A.kl_coef, kl, l);
+  }
+  A.logprobs[row] = (float)v.lp;
+  if (A.kl_out) A.kl_out[row] = kl;
+  if (ENT && A.entropy) A.entropy[row] = v.h;
+  A.row_val[row] = (double)w * (double)l;
 }
 
 // ---------------------------------------------------------------------------
@@ -260,8 +269,8 @@ __global__ void __launch_bounds__(1024) loss_plan_kernel(const PlanArgs A) {
 // row's a and b, for at a column of a large h or q, where p is near it, half a step of 16 bits would not hide it.
 template <typename T>
 __device__ __forceinline__ void fold_low(RowGrad& o, Scale2 k) {
-  if (sizeof(T) == 4 || far_out(center(o.m, k))) return;
-  const float y = o.m * k.lo, f = ex2(y);
+  if (sizeof(T) == 4) return;
+  const float y = far_out(center(o.m, k)) ? 0.f : o.m * k.lo, f = ex2(y);
   o.a = fmaf(o.b, y, o.a) * f;
   o.b *= f;
 }
@@ -550,6 +559,7 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
     if (KIND != kDistill && i + step < n_active) tok_next = A.tokens.at(row_next / A.length, row_next % A.length);
     RowGrad o{0.f, 0.f, 0.f, 0.f, -1, false};
     float wt = 0.f;
+    PolicyRow val;
     if (PASS == kBackward) {
       const float4 rec = A.rec[row];
       const float f = up * (A.seq_g ? A.seq_g[b] : 1.f);
@@ -585,7 +595,7 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
         a = warp_merge(RowSum{v.x, v.y, v.z}, size, ks);
       }
       if (KIND == kPolicy) {
-        o = policy_tail<ENT>(A, row, a, q, write);
+        o = policy_tail<ENT>(A, a, q, val);
       } else if (KIND == kPreference) {
         o = RowGrad{a.m, -1.f / a.s, 0.f, 1.f, 0, false};
         if (write) A.row_val[row] = known ? log2_prob(A, a, q.x_tok) * kLn2d : (double)NAN;
@@ -616,6 +626,7 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
       if (PASS == kForward) {
         if (write && A.rec)
           A.rec[row] = KIND == kDistill ? make_float4(o.m, o.a, wt, 0.f) : make_float4(o.m, o.a, o.b, o.h);
+        if (KIND == kPolicy && write) write_policy<ENT>(A, row, q.w, val);
         if (KIND == kDistill) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.teacher_empty[par]);
@@ -629,6 +640,7 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
       sh.grad_wt[par] = wt;
       mbar_arrive(&sh.grad_full[par]);
     }
+    if (KIND == kPolicy && PASS == kFused && write) write_policy<ENT>(A, row, q.w, val);
   }
   // Rows that are not scored have zeros.
   if (PASS != kBackward && rank == 0) {

@@ -356,3 +356,24 @@ def test_rows_without_a_teacher_entry(cuda_device, dtype):
     ids[0, 1], teacher[1, 1, 2] = v, math.nan
     for f in (losses.distillation_loss_and_grad(x, ids, teacher)[0], losses.distillation_loss(x, ids, teacher)):
         assert f.loss.isnan() and f.kl[:2, 1].isnan().all()
+
+
+def test_a_small_divergence_from_the_reference(cuda_device):
+    """The KL estimate e^d - d - 1 near d = 0, on rows of one column: log p is 0 exactly and d is the reference's value.
+    From 64 bits: 2^-52 |d| of cancellation against d^2 / 2, and the output's own half step: 2^-24 + 2^-51 / |d|."""
+    from randomrepo_b200 import losses
+
+    d = torch.tensor([1e-1, 1e-2, 1e-3, 1e-4, 1e-5, 1e-6, 3.0, 0.0], dtype=torch.float64)
+    d = torch.cat([d, -d]).float().to(cuda_device).unsqueeze(0)
+    x = torch.zeros(1, 16, 1, device=cuda_device)
+    tokens = torch.zeros(1, 16, dtype=torch.int64, device=cuda_device)
+    exact = d.double()
+    # e^d - d - 1 by its series where |d| is small (the terms fall by more than |d| / 3 each).
+    small = sum(exact**i / math.factorial(i) for i in range(2, 8))
+    want = torch.where(exact.abs() < 0.05, small, torch.expm1(exact) - exact)
+    kw = dict(ref_logprobs=d, kl_coef=0.5, reduction="sum")
+    adv = torch.zeros(1, device=cuda_device)
+    for got in (losses.policy_loss_and_grad(x, tokens, adv, **kw)[0], losses.policy_loss(x, tokens, adv, **kw)):
+        assert (got.kl >= 0).all()
+        tol = want * (2.0**-24 + 2.0**-51 / exact.abs().clamp(min=1e-30))
+        assert ((got.kl.double() - want).abs() <= tol).all(), (got.kl.double() / want - 1)
