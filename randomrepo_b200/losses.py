@@ -32,6 +32,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib
@@ -79,6 +80,9 @@ class DistillationLoss(NamedTuple):
 
 def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
     """``logits`` as [B, T, V], checked."""
+    if forward_ad._current_level >= 0 and isinstance(logits, torch.Tensor) and (
+            forward_ad.unpack_dual(logits).tangent is not None):
+        raise RuntimeError(f"{what}: the vocabulary rows have no forward-mode derivative")
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError(f"{what}: logits must be a CUDA tensor (the vocabulary kernels have no CPU path)")
     if logits.dtype not in _DTYPES:

@@ -377,3 +377,23 @@ def test_a_small_divergence_from_the_reference(cuda_device):
         assert (got.kl >= 0).all()
         tol = want * (2.0**-24 + 2.0**-51 / exact.abs().clamp(min=1e-30))
         assert ((got.kl.double() - want).abs() <= tol).all(), (got.kl.double() / want - 1)
+
+
+def test_forward_mode_is_refused(cuda_device):
+    """A dual tensor's tangent is not dropped without a word."""
+    import torch.autograd.forward_ad as fwad
+
+    from randomrepo_b200 import losses
+
+    x = torch.randn(2, 4, 33, device=cuda_device)
+    tokens = torch.zeros(2, 4, dtype=torch.int64, device=cuda_device)
+    with fwad.dual_level():
+        assert losses.preference_loss(x, tokens).loss.isfinite()
+        dual = fwad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: losses.policy_loss(dual, tokens, x[:, 0, 0]), lambda: losses.preference_loss(dual, tokens),
+                     lambda: losses.policy_loss_and_grad(dual, tokens, x[:, 0, 0]),
+                     lambda: losses.distillation_loss(dual, tokens.unsqueeze(-1), x[..., :1]),
+                     lambda: losses.preference_loss(dual.requires_grad_(), tokens)):
+            with pytest.raises(RuntimeError, match="forward"):
+                call()
+    assert losses.preference_loss(x, tokens).loss.isfinite()

@@ -277,3 +277,17 @@ def test_the_graph_holds_no_tensor_beside_the_saved_ones(monkeypatch):
         (grad,) = torch.autograd.grad(loss, x)
         assert gone.expired() and grad.shape == x.shape
         assert len(packed) == 1
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwad
+
+    x, tok = _fake(torch.zeros(2, 3, 8)), torch.zeros(2, 3, dtype=torch.int64)
+    with fwad.dual_level():
+        dual = _fake(fwad.make_dual(torch.zeros(2, 3, 8), torch.ones(2, 3, 8)))
+        for call in (lambda: losses.policy_loss(dual, tok, torch.zeros(2)), lambda: losses.preference_loss_and_grad(dual, tok),
+                     lambda: losses.distillation_loss(dual, tok.unsqueeze(-1), x[..., :1]), lambda: losses.top_logits(dual, 2)):
+            with pytest.raises(RuntimeError, match="forward"):
+                call()
+        with pytest.raises(ValueError, match="k must"):  # (others are taken, up to the next check)
+            losses.top_logits(x, 9)
