@@ -150,17 +150,22 @@ def _reduction(name: str, what: str) -> int:
 
 def _grad_like(x: torch.Tensor) -> torch.Tensor:
     """An uninitialised gradient for logits [B, T, V] whose rows start as many bytes past a 16-byte boundary as
-    the logits' do, so that both move in 16-byte vectors: dense where whole rows are such vectors or the logits
-    are dense themselves, else with the logits' strides."""
+    the logits' do, so that both move in 16-byte vectors: dense where such rows are, else with the logits' strides
+    (rows that overlap or lie far apart: dense, wherever they start)."""
     b, n, v = x.shape
-    dense = v * x.element_size() % 16 == 0 or (x.is_contiguous() and x.data_ptr() % 16 == 0)
-    if dense or x.numel() == 0:
+    size, numel = x.element_size(), x.numel()
+    at = x.data_ptr() % 16 // size
+    alike = x.is_contiguous()
+    if not alike:
+        sb, sn = (x.stride(0) if b > 1 else 0), (x.stride(1) if n > 1 else 0)
+        alike = v * size % 16 == 0 and sb * size % 16 == 0 and sn * size % 16 == 0
+    if numel == 0 or (alike and at == 0):
         return torch.empty(b, n, v, dtype=x.dtype, device=x.device)  # (faster than a tuple of sizes)
-    sb, sn = (x.stride(0) if b > 1 else 0), (x.stride(1) if n > 1 else 0)
+    if alike:
+        return torch.empty(numel + at, dtype=x.dtype, device=x.device)[at:].view(b, n, v)
     span = (n - 1) * sn + v
-    if (n > 1 and sn < v) or (b > 1 and sb < span) or (b - 1) * sb + span > 2 * x.numel() + 64:
+    if (n > 1 and sn < v) or (b > 1 and sb < span) or (b - 1) * sb + span > 2 * numel + 64:
         return torch.empty((b, n, v), dtype=x.dtype, device=x.device)  # overlapping or sparse rows
-    at = x.data_ptr() % 16 // x.element_size()
     flat = torch.empty((b - 1) * sb + span + 16, dtype=x.dtype, device=x.device)
     return flat.as_strided((b, n, v), (max(sb, span), max(sn, v), 1), at)
 

@@ -291,3 +291,19 @@ def test_forward_mode_is_refused():
                 call()
         with pytest.raises(ValueError, match="k must"):  # (others are taken, up to the next check)
             losses.top_logits(x, 9)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_rows_of_whole_vectors_start_like_the_logits(dtype):
+    """Rows of a multiple of 16 bytes that start elsewhere in their 16 bytes, all at the same place or each at its own."""
+    wide, step = torch.zeros(3, 4, 32, dtype=dtype), torch.zeros(3, 4, 21, dtype=dtype)
+    shifted = torch.zeros(3 * 4 * 16 + 1, dtype=dtype)[1:].view(3, 4, 16)
+    for x in (wide[..., 1:17], wide[:, 1:, 3:19], wide[::2, ::3, 1:25], wide[:, :1, 5:13], step[..., :16], step[:, 1:, 2:18],
+              step[:, :-1, 1:17].transpose(0, 1)[:, 1:2], shifted, shifted[1:], shifted[:, 1:]):
+        g = losses._grad_like(x)
+        assert g.shape == x.shape and g.stride(-1) == 1 and g.dtype == dtype
+        for i in range(x.shape[0]):
+            for j in range(x.shape[1]):
+                assert (g[i, j].data_ptr() - x[i, j].data_ptr()) % 16 == 0, (x.shape, x.stride(), i, j)
+        g.copy_(torch.arange(g.numel()).view(g.shape) % 251)
+        assert torch.equal(g, (torch.arange(g.numel()).view(g.shape) % 251).to(dtype))  # no two rows overlap
