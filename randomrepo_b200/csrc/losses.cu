@@ -948,7 +948,9 @@ __global__ void __launch_bounds__(1024) loss_pair_kernel(const PairArgs A) {
     const double m = (double)A.beta * ((A.seq_sum[p] - rc) - (A.seq_sum[p + pairs] - rr));
     const double eps = (double)A.smoothing;
     const double soft = log1p(exp(-fabs(m)));  // -log sigmoid(|m|)
-    loss += (1.0 - eps) * (soft + fmax(-m, 0.0)) + eps * (soft + fmax(m, 0.0));
+    // (a term of weight 0 adds nothing, also where a sequence of probability 0 makes it infinite)
+    if (eps < 1.0) loss += (1.0 - eps) * (soft + fmax(-m, 0.0));
+    if (eps > 0.0) loss += eps * (soft + fmax(m, 0.0));
     if (m != m) loss = m;  // (fmax drops a NaN)
     const double sig = m >= 0.0 ? 1.0 / (1.0 + exp(-m)) : exp(m) / (1.0 + exp(m));
     const double neg = m >= 0.0 ? exp(-m) / (1.0 + exp(-m)) : 1.0 / (1.0 + exp(m));  // 1 - sig, without the loss of digits

@@ -397,3 +397,29 @@ def test_forward_mode_is_refused(cuda_device):
             with pytest.raises(RuntimeError, match="forward"):
                 call()
     assert losses.preference_loss(x, tokens).loss.isfinite()
+
+
+def test_a_margin_without_bound(cuda_device):
+    """A rejected answer of probability 0 (a masked token in it): nothing is left to learn, the loss is 0; a chosen one:
+    the loss is infinite and the slope is beta.  With smoothing both are infinite."""
+    from randomrepo_b200 import losses
+
+    x = torch.zeros(4, 2, 9, device=cuda_device)
+    x[2, 1, 5] = -math.inf  # rejected, of pair 0
+    x[1, 0, 5] = -math.inf  # chosen, of pair 1
+    tokens = torch.full((4, 2), 5, device=cuda_device)
+    pair = torch.tensor([0, 2], device=cuda_device)
+    got, grad = losses.preference_loss_and_grad(x[pair], tokens[pair], beta=0.5)
+    assert float(got.loss) == 0.0 and float(got.margins[0]) == math.inf and (grad == 0).all()
+    leaf = x[pair].requires_grad_()
+    out = losses.preference_loss(leaf, tokens[pair], beta=0.5)
+    out.loss.backward()
+    assert out.loss.item() == 0.0 and (leaf.grad == 0).all()
+    got, grad = losses.preference_loss_and_grad(x[[1, 3]], tokens[[1, 3]], beta=0.5)
+    assert float(got.loss) == math.inf and float(got.margins[0]) == -math.inf
+    p = torch.softmax(x[[1, 3]].double(), -1)
+    p[..., 5] -= 1
+    p[1] *= -1
+    torch.testing.assert_close(grad.double(), 0.5 * p, atol=1e-7, rtol=1e-6)
+    got, _ = losses.preference_loss_and_grad(x[pair], tokens[pair], beta=0.5, label_smoothing=0.1)
+    assert float(got.loss) == math.inf
