@@ -328,8 +328,10 @@ constexpr int kIdTable = 2 * PKV_MAX_TOP;
 // (16-bit sums of 4 096 rows 210 us; 160 threads x 3 CTAs 234, 96 x 5 251, 512 threads x 4 vectors x 1 CTA 275).  Both in
 // one launch: one CTA an SM, whose rows in flight stay in L2 until their second pass; 16 bits 454 us (512 threads 464,
 // 768 480, two CTAs of 384 threads 512, a row to a pair of CTAs 530), where two exponentials and their conversions a
-// column cost as much as HBM.  float32, half the exponentials a byte: fewer threads and more slots, and a row to a pair
-// of CTAs where the rows in flight would not stay in L2 (8 192 rows 1.58 ms; without pairs 1.84, 512 threads 1.61).
+// column cost as much as HBM.  float32, half the exponentials a byte: fewer threads and more slots (8 192 rows 1.58 ms;
+// 512 threads 1.61).  A row to a pair of CTAs where the rows in flight would not stay in L2; us of 4 096 rows with /
+// without: float32 116 000 columns 690 / 675, 128 000 725 / 764, 152 064 845 / 950; 16 bits 232 000 696 / 684,
+// 256 000 775 / 773 (with an entropy term 890 / 805), 288 000 850 / 914; 2 048 of 512 000 776 / 929.
 template <typename T, int PASS> struct ShapeOf : Shape<128, 8, 3, 4> {};
 template <typename T> struct ShapeOf<T, kFused> : Shape<640, 4, 5, 1> {};
 template <> struct ShapeOf<float, kFused> : Shape<384, 4, 8, 1> {};
@@ -338,7 +340,7 @@ template <> struct ShapeOf<float, kFused> : Shape<384, 4, 8, 1> {};
 // 20 000 246 / 305, 35 000 469 / 423.
 using ShortShape = Shape<128, 4, 5, 4>;
 constexpr int64_t kShortRow = 112 << 10;   // bytes
-constexpr int64_t kRowsInL2 = 64 << 20;    // bytes of rows in flight that come back from L2
+constexpr int64_t kRowsInL2 = 72 << 20;    // bytes of rows in flight that come back from L2
 
 template <typename S, bool X>
 struct alignas(128) LossShared {

@@ -423,3 +423,41 @@ def test_a_margin_without_bound(cuda_device):
     torch.testing.assert_close(grad.double(), 0.5 * p, atol=1e-7, rtol=1e-6)
     got, _ = losses.preference_loss_and_grad(x[pair], tokens[pair], beta=0.5, label_smoothing=0.1)
     assert float(got.loss) == math.inf
+
+
+@pytest.mark.parametrize("dtype,v", [(F32, 130001), (BF16, 260009), (F16, 300007)])
+def test_rows_of_a_pair_of_ctas(cuda_device, dtype, v):
+    """Rows long enough for a pair of CTAs each, more of them than there are pairs, at every offset in their 16 bytes.
+
+    A thread adds at most 600 columns and 2^5 x 2^4 x 2 sums are merged: 2.5e-5 of the sum at the most (rounding and the
+    approximate 2^y); a gradient entry's coefficient is 1 or 2 here."""
+    from randomrepo_b200 import losses
+
+    n = 200
+    g = torch.Generator(device=cuda_device).manual_seed(v)
+    x = (torch.randn(1, n, v, generator=g, device=cuda_device) * 2).to(dtype)
+    tokens = torch.randint(0, v, (1, n), generator=g, device=cuda_device)
+    adv = torch.where(torch.rand(1, n, generator=g, device=cuda_device) < 0.5, 1.0, -1.0)
+    ids = torch.randint(0, v, (1, n, 9), generator=g, device=cuda_device)
+    teacher = torch.randn(1, n, 9, generator=g, device=cuda_device)
+    mask = torch.rand(1, n, generator=g, device=cuda_device) < 0.9
+    got, grad = losses.policy_loss_and_grad(x, tokens, adv, None, mask, reduction="sum")
+    _, ent = losses.policy_loss_and_grad(x, tokens, adv, None, mask, entropy_coef=0.1, reduction="sum")
+    dis, dgrad = losses.distillation_loss_and_grad(x, ids, teacher, mask, reduction="sum")
+    for at in torch.arange(n, device=cuda_device).split(50):
+        rows = torch.log_softmax(x[0, at].double(), -1)
+        seen = mask[0, at].unsqueeze(-1)
+        pick = rows.gather(-1, tokens[0, at].unsqueeze(-1))
+        assert ((got.logprobs[0, at].double().unsqueeze(-1) - pick) * seen).abs().max() <= 2.5e-5
+        p = rows.exp()
+        hot = torch.zeros_like(p).scatter_(-1, tokens[0, at].unsqueeze(-1), 1.0)
+        entropy = -(p * rows).sum(-1, keepdim=True)
+        want = (p - hot) * adv[0, at].double().unsqueeze(-1)
+        q = torch.softmax(teacher[0, at].double(), -1)
+        each = ((grad, want), (ent, want + 0.1 * p * (rows + entropy)), (dgrad, p.scatter_add(-1, ids[0, at], -q)))
+        for have, wanted in each:
+            wanted = wanted * seen
+            tol = wanted.abs() * (_half(dtype) + 2.5e-5) + 5e-5 * p + 2.0**-22 + (2.0**-25 if dtype == F16 else 0)
+            assert ((have[0, at].double() - wanted).abs() <= tol).all()
+        per = (q * (q.log() - rows.gather(-1, ids[0, at]))).sum(-1, keepdim=True)
+        assert ((dis.kl[0, at].double().unsqueeze(-1) - per) * seen).abs().max() <= 5e-5
