@@ -461,3 +461,31 @@ def test_rows_of_a_pair_of_ctas(cuda_device, dtype, v):
             assert ((have[0, at].double() - wanted).abs() <= tol).all()
         per = (q * (q.log() - rows.gather(-1, ids[0, at]))).sum(-1, keepdim=True)
         assert ((dis.kl[0, at].double().unsqueeze(-1) - per) * seen).abs().max() <= 5e-5
+
+
+def test_the_mean_of_log_probabilities(cuda_device):
+    """Their errors do not add up over a sequence: the mean error of 4 096 rows' is that of their float32 outputs.
+
+    The outputs lie in (-4, -1): a rounding is uniform in +-2^-23 at the most, rms 2^-22 / sqrt(12) = 6.9e-8, of the
+    mean of 4 096 1.1e-9; five times that is 5.5e-9.  The kernels' own mean error is held to 1e-8, and a log2f's
+    rounding (a step of 6e-8, its mean a sixth of that at the most) adds 1e-8: 2.6e-8.  Without the low half of the
+    scale, the correction of the approximate 2^y or the exact merges the mean is off by 4e-8 to 1e-7."""
+    from randomrepo_b200 import losses
+
+    n, v = 4096, 20011
+    for dtype in (F32, BF16):
+        for temperature in (1.0, 0.7):
+            t = _float(temperature)
+            g = torch.Generator(device=cuda_device).manual_seed(9)
+            x = torch.randn(1, n, v, generator=g, device=cuda_device)
+            spot = 0.5 * torch.rand(n, generator=g, device=cuda_device) - 2.0
+            x[0, :, 0] = t * ((x[0, :, 1:].double() / t).logsumexp(-1).float() + spot)
+            x = x.to(dtype)
+            tokens = torch.zeros(1, n, dtype=torch.int64, device=cuda_device)
+            want = torch.cat([torch.log_softmax(c.double() / t, -1)[..., 0] for c in x[0].split(512)])
+            assert (want < -1).all() and (want > -4).all()
+            adv = torch.zeros(1, device=cuda_device)
+            for got in (losses.policy_loss_and_grad(x, tokens, adv, temperature=temperature)[0],
+                        losses.policy_loss(x, tokens, adv, temperature=temperature)):
+                off = (got.logprobs[0].double() - want).mean()
+                assert abs(float(off)) <= 2.6e-8, (dtype, temperature, float(off))
