@@ -479,8 +479,9 @@ __device__ __forceinline__ void teacher_rows(const LossArgs& A, Sh& sh, int rank
     twice = __any_sync(0xffffffffu, twice);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    // The norm in 64 bits: log q would lose digits to a rounded one.
-    double norm = 0.0;
+    // log q = (v - base) / T - norm, in 64 bits (it would lose digits to a rounded norm) and from the largest entry (an
+    // entry may be a type's lowest value, in all of which the norm's logarithm would be lost).
+    double base = 0.0, norm = 0.0;
     if (A.tlse.p) {
       norm = (double)A.tlse.at(p.b, p.t);
     } else if (top > -INFINITY) {
@@ -488,7 +489,8 @@ __device__ __forceinline__ void teacher_rows(const LossArgs& A, Sh& sh, int rank
 #pragma unroll
       for (int e = 0; e < kPer; ++e)
         if (v[e] != -INFINITY) sum += (double)expf((float)(((double)v[e] - (double)top) * A.inv_td));
-      norm = (double)top * A.inv_td + log(warp_sum_d(sum));
+      base = (double)top;
+      norm = log(warp_sum_d(sum));
     }
     double qs = 0.0, qx = 0.0, ql = 0.0;
 #pragma unroll
@@ -496,7 +498,7 @@ __device__ __forceinline__ void teacher_rows(const LossArgs& A, Sh& sh, int rank
       const int j = lane + 32 * e;
       float q = 0.f;
       if (v[e] != -INFINITY) {
-        const double lq = (double)v[e] * A.inv_td - norm;
+        const double lq = ((double)v[e] - base) * A.inv_td - norm;
         q = expf((float)lq);
         qs += (double)q;
         if (q != 0.f || x[e] != x[e]) {

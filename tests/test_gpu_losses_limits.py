@@ -489,3 +489,34 @@ def test_the_mean_of_log_probabilities(cuda_device):
                         losses.policy_loss(x, tokens, adv, temperature=temperature)):
                 off = (got.logprobs[0].double() - want).mean()
                 assert abs(float(off)) <= 2.6e-8, (dtype, temperature, float(off))
+
+
+@pytest.mark.parametrize("value", [torch.finfo(F32).min, torch.finfo(F32).max, -1e30, 1e20, -1e9, 0.0])
+def test_a_teachers_list_of_one_value(cuda_device, value):
+    """Entries that are all a mask's value are a uniform list, beside rows where one entry stands above them.
+
+    kl = log p of the student against log q = -log k: 2.5e-5 for log p, 2^-22 for q; a gradient entry p - q likewise."""
+    from randomrepo_b200 import losses
+
+    v, k = 700, 12
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(1, 3, v, generator=g).to(cuda_device)
+    ids = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(3)]).unsqueeze(0).to(cuda_device)
+    teacher = torch.full((1, 3, k), value, device=cuda_device)
+    if value < 0:
+        teacher[0, 1, 4] = torch.finfo(F32).max
+    else:
+        teacher[0, 1] = 0.0
+    teacher[0, 2, 3:] = -math.inf
+    for temperature in (1.0, 0.5):
+        q = torch.softmax(teacher.double() / temperature, -1)
+        rows = torch.log_softmax(x.double() / temperature, -1)
+        per = temperature**2 * (torch.special.xlogy(q, q) - q * rows.gather(-1, ids)).sum(-1)
+        want = temperature * rows.exp().scatter_add(-1, ids, -q)
+        leaf = x.clone().requires_grad_()
+        out = losses.distillation_loss(leaf, ids, teacher, temperature=temperature, reduction="sum")
+        got, grad = losses.distillation_loss_and_grad(x, ids, teacher, temperature=temperature, reduction="sum")
+        (own,) = torch.autograd.grad(out.loss, leaf)
+        for res, d in ((got, grad), (out, own)):
+            assert ((res.kl.double() - per).abs() <= 2.6e-5 + 2.0**-20 * per.abs()).all(), (res.kl, per)
+            assert ((d.double() - want).abs() <= 2.6e-5 * (want.abs() + rows.exp()) + 2.0**-22).all()
