@@ -30,8 +30,9 @@
 namespace pkv {
 namespace {
 
-// Two CTAs an SM: 256 threads read the columns, 128 pick the row before.  (One group doing both: 391 us against
-// 341 us for 4 096 rows of 151 936 16-bit columns and k = 64, since the columns waited for each row's picking.)
+// Two CTAs an SM: 256 threads read the columns, 128 pick the row before.  4 096 rows of 151 936 16-bit columns and
+// k = 64 take 295 us.  (One group doing both was slower, 391 us against 341 with the picking of that time, since the
+// columns waited for each row's picking.)
 using TopShape = Shape<256, 4, 4, 2>;
 constexpr int kTopThreads = TopShape::kGroup;
 constexpr int kTopWarps = TopShape::kWarps;

@@ -32,7 +32,8 @@ head_dim, dtype code]`` (the ``pkv_pool_geom`` of the C ABI).
 * ``policy_loss(...)``, ``preference_loss(...)``, ``distillation_loss(...)``
   ``-> (loss, per-row outputs, dlogits)``: the vocabulary-row losses with
   their gradients (``randomrepo_b200.losses.*_loss_and_grad``; outputs a call
-  does not have are empty), and ``top_logits(logits, k, temperature) ->
+  does not have are empty; ``logits.backward(dlogits)`` goes on from there,
+  PyTorch refuses to differentiate through the operators themselves), and ``top_logits(logits, k, temperature) ->
   (values, tokens, lse)``.
 """
 

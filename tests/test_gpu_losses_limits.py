@@ -520,3 +520,52 @@ def test_a_teachers_list_of_one_value(cuda_device, value):
         for res, d in ((got, grad), (out, own)):
             assert ((res.kl.double() - per).abs() <= 2.6e-5 + 2.0**-20 * per.abs()).all(), (res.kl, per)
             assert ((d.double() - want).abs() <= 2.6e-5 * (want.abs() + rows.exp()) + 2.0**-22).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_whole_rows_with_shifted_tokens(cuda_device, dtype):
+    """Next-token rows without a slice: the tokens and per-row inputs shifted by one, the last position not scored.  The
+    loss and the gradient down to the whole logits are those of ``logits[:, :-1]`` (each sum is off by 2.5e-5 at most)."""
+    from torch.nn.functional import pad
+
+    from randomrepo_b200 import losses
+
+    b, t, v = 3, 9, 1003
+    g = torch.Generator().manual_seed(4)
+    data = (torch.randn(b, t, v, generator=g) * 2).to(dtype).to(cuda_device)
+    input_ids = torch.randint(0, v, (b, t), generator=g).to(cuda_device)
+    completion = (torch.rand(b, t, generator=g) < 0.7).to(cuda_device)
+    adv = torch.randn(b, generator=g).to(cuda_device)
+    old, ref = (-8 + 0.1 * torch.randn(b, t - 1, generator=g).to(cuda_device) for _ in range(2))
+    kw = dict(kl_coef=0.05, entropy_coef=0.01)
+    leaf = data.clone().requires_grad_()
+    cut = losses.policy_loss(leaf[:, :-1], input_ids[:, 1:], adv, old, completion[:, 1:], ref_logprobs=ref, **kw)
+    (want,) = torch.autograd.grad(cut.loss, leaf)
+    mask = completion.roll(-1, 1)
+    mask[:, -1] = False
+    leaf = data.clone().requires_grad_()
+    out = losses.policy_loss(leaf, input_ids.roll(-1, 1), adv, pad(old, (0, 1)), mask, ref_logprobs=pad(ref, (0, 1)), **kw)
+    (got,) = torch.autograd.grad(out.loss, leaf)
+    torch.testing.assert_close(out.logprobs[:, :-1], cut.logprobs, atol=5e-5, rtol=0)
+    assert (out.logprobs[:, -1] == 0).all() and (got[:, -1] == 0).all()
+    torch.testing.assert_close(out.loss, cut.loss, atol=1e-4, rtol=1e-4)
+    torch.testing.assert_close(got.float(), want.float(), atol=1e-6, rtol=1e-4 + torch.finfo(dtype).eps)
+
+
+def test_operators_hand_the_gradient_out(cuda_device):
+    """``torch.ops.pkv`` losses return their gradient; to differentiate through them is an error, not a zero."""
+    import randomrepo_b200.ops  # noqa: F401 - registers the operators
+
+    leaf = torch.randn(2, 3, 65, device=cuda_device).requires_grad_()
+    tokens = torch.zeros(2, 3, dtype=torch.int64, device=cuda_device)
+    adv = torch.ones(2, device=cuda_device)
+    rows = leaf * 2
+    for out in (torch.ops.pkv.policy_loss(rows, tokens, adv, None, None, None, 0.2, 0.2, 0.0, 0.0, 1.0, "sum", 1.0),
+                torch.ops.pkv.preference_loss(rows, tokens, None, None, 0.1, 0.0, False, 1.0),
+                torch.ops.pkv.distillation_loss(rows, tokens.unsqueeze(-1), adv.view(2, 1, 1).expand(2, 3, 1), None, None,
+                                                1.0, "sum", 1.0)):
+        with pytest.raises(RuntimeError, match="autograd"):
+            out[0].backward(retain_graph=True)
+        leaf.grad = None
+        rows.backward(out[-1].detach(), retain_graph=True)
+        assert torch.equal(leaf.grad, 2 * out[-1].detach())
