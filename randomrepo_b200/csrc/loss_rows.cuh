@@ -61,9 +61,12 @@ __device__ __forceinline__ float ex2(float y) {
 // type's lowest value everywhere) take y = (x - max x) k.
 __device__ __forceinline__ float center(float m, Scale2 k) { return __fmul_rn(-m, k.hi); }  // (rounded: never part of another FMA)
 __device__ __forceinline__ bool far_out(float c) { return !(fabsf(c) < 1e8f); }
-// The running sums of a set of columns: m = max x, s = sum 2^y, w = sum 2^y y.
+// The running sums of a set of columns: m near max x, s = sum 2^y, w = sum 2^y y.  D: s between threads, in whose merges
+// 32 bits lose 4e-8 of a row's sum (rms).
+template <typename D>
 struct RowSum {
-  float m, s, w;
+  D s;
+  float m, w;
 };
 
 // d: the exponent that takes sums from a reference m to a larger one.
@@ -76,8 +79,9 @@ __device__ __forceinline__ float rescale_exponent(float m, float m_new, Scale2 k
   return (m - m_new) * k.hi + (far_out(c) ? -stays : stays);
 }
 
-__device__ __forceinline__ void sum_rescale(RowSum& a, float m_new, float d, float f) {
-  a.w = f > 0.f ? f * fmaf(d, a.s, a.w) : 0.f;  // (a NaN stays in s)
+template <typename D>
+__device__ __forceinline__ void sum_rescale(RowSum<D>& a, float m_new, float d, D f) {
+  a.w = f > 0 ? (float)f * fmaf(d, (float)a.s, a.w) : 0.f;  // (a NaN stays in s)
   a.s *= f;
   a.m = m_new;
 }
@@ -90,6 +94,7 @@ __device__ __forceinline__ double log2_sum(float s) {
   const float f = frexpf(s, &e);
   return (double)e + (double)log2f(f) + (double)(7.2e-8f * (1.f - 1.f / s));
 }
+__device__ __forceinline__ double log2_sum(double s) { return log2(s) + 7.2e-8 * (1.0 - 1.0 / s); }
 
 // Columns [0, head) and [head + VE nvec, vocab) of a row are outside its 16-byte-aligned body.
 template <typename T>
@@ -199,55 +204,88 @@ __device__ __forceinline__ float top_of(const uint4 (&v)[N]) {
 // The running sums of a thread.  m is a column near the largest so far: as long as no column's 2^y passes 2^20 it
 // stays, so that the sums are rarely rescaled.  c is its center, +inf where there is none (no column yet, or far out).
 // The lanes of a warp that add whole chunks share their m: their sums then merge without the approximate 2^d.
-template <bool ENT>
+//
+// EXACT: a column that is most of its row must not cost the small ones added after it their digits, nor be an approximate
+// 2^y itself (1.1e-7 of the row's sum, rms).  m gives way from 2^4 on, and the large columns among those that it is taken
+// from have a sum of their own in 64 bits.  (Others are not most of a row: m is the largest of a thousand columns.)
+template <bool ENT, bool EXACT = false>
 struct Fold {
+  using Sum = std::conditional_t<EXACT, double, float>;
   float m = -INFINITY, c = INFINITY;
   f32x2 s0 = 0ull, s1 = 0ull, w = 0ull;
+  double large = 0.0;
 
-  __device__ __forceinline__ RowSum sum() const {
+  __device__ __forceinline__ RowSum<float> lanes() const {
     const float2 t = unpair(add2(s0, s1)), u = unpair(w);
-    return RowSum{m, t.x + t.y, ENT ? u.x + u.y : 0.f};
+    return RowSum<float>{t.x + t.y, m, ENT ? u.x + u.y : 0.f};
+  }
+  __device__ __forceinline__ RowSum<Sum> sum() const {
+    const RowSum<float> a = lanes();
+    if constexpr (EXACT) return RowSum<Sum>{(double)a.s + large, a.m, a.w};
+    return RowSum<Sum>{(Sum)a.s, a.m, a.w};
+  }
+  __device__ __forceinline__ void take_large(float& e) {
+    if (e > 0.5f) large += (double)e, e = 0.f;
   }
 
   // Add columns whose largest is `top`.  WHOLE: all lanes of the warp do.
   template <bool WHOLE, int N>
   __device__ __forceinline__ void add(const float (&x)[N], float top, Scale2 k) {
-    const bool passed = !(fmaf(top, k.hi, c) <= 20.f);
+    const bool passed = !(fmaf(top, k.hi, c) <= (EXACT ? 4.f : 20.f));
     if (WHOLE ? __any_sync(0xffffffffu, passed) : passed) {
-      RowSum a = sum();
-      if (WHOLE) {
-        top = fmaxf(top, m);
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      }
-      if (!(top > -INFINITY)) {  // nothing but -inf, or NaN
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (x[i] != x[i]) a.s = NAN;
-      } else {
-        if (top > m) {
-          const float d = rescale_exponent(m, top, k);
-          sum_rescale(a, top, d, ex2(d));
-        }
-        m = a.m;
-        const float at = center(m, k);
-        c = far_out(at) ? INFINITY : at;
-        if (far_out(at)) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float y = (x[i] - m) * k.hi, e = ex2(y);
-            a.s += e;
-            if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
-          }
-        }
-      }
-      s0 = pair(a.s, 0.f), s1 = 0ull, w = pair(a.w, 0.f);
+      refer<WHOLE>(x, top, k);
       if (c == INFINITY) return;
+      if (EXACT) {
+        add_columns<true>(x, k);
+        return;
+      }
     }
+    add_columns<false>(x, k);
+  }
+
+  // Take a reference of which `top` is within reach.  Far out, with the columns' sums.
+  template <bool WHOLE, int N>
+  __device__ __forceinline__ void refer(const float (&x)[N], float top, Scale2 k) {
+    RowSum<float> a = lanes();
+    if (WHOLE) {
+      top = fmaxf(top, m);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    }
+    if (!(top > -INFINITY)) {  // nothing but -inf, or NaN
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (x[i] != x[i]) a.s = NAN;
+    } else {
+      if (top > m) {
+        const float d = rescale_exponent(m, top, k), f = EXACT ? (float)exp2((double)d) : ex2(d);
+        if (EXACT && ENT) a.w = f > 0.f ? fmaf(d, (float)large, a.w) : 0.f;
+        sum_rescale(a, top, d, f);
+        if (EXACT) large *= (double)f;
+      }
+      m = a.m;
+      const float at = center(m, k);
+      c = far_out(at) ? INFINITY : at;
+      if (far_out(at)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float y = (x[i] - m) * k.hi, e = ex2(y);
+          a.s += e;
+          if (ENT) a.w = fmaf(e, fmaxf(y, -1e30f), a.w);
+        }
+      }
+    }
+    s0 = pair(a.s, 0.f), s1 = 0ull, w = pair(a.w, 0.f);
+  }
+
+  template <bool LARGE, int N>
+  __device__ __forceinline__ void add_columns(const float (&x)[N], Scale2 k) {
     if constexpr (N == 1) {
-      const float y = fmaf(x[0], k.lo, fmaf(x[0], k.hi, c)), e = ex2(y);
-      s0 = add2(s0, pair(e, 0.f));
+      const float y = fmaf(x[0], k.lo, fmaf(x[0], k.hi, c));
+      float e = ex2(y);
       if (ENT) w = add2(w, pair(e * fmaxf(y, -1e30f), 0.f));
+      if (LARGE) take_large(e);
+      s0 = add2(s0, pair(e, 0.f));
     } else {
       static_assert(N % 4 == 0, "columns go in pairs, to two sums");
       const f32x2 cc = pair(c, c), hi = pair(k.hi, k.hi), lo = pair(k.lo, k.lo);
@@ -255,12 +293,13 @@ struct Fold {
       for (int i = 0; i < N; i += 2) {
         const f32x2 xx = pair(x[i], x[i + 1]);
         const float2 y = unpair(fma2(xx, lo, fma2(xx, hi, cc)));
-        const f32x2 e = pair(ex2(y.x), ex2(y.y));
+        float e0 = ex2(y.x), e1 = ex2(y.y);
+        if (ENT) w = fma2(pair(e0, e1), pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), w);
+        if (LARGE) take_large(e0), take_large(e1);
         if (i & 2)
-          s1 = add2(s1, e);
+          s1 = add2(s1, pair(e0, e1));
         else
-          s0 = add2(s0, e);
-        if (ENT) w = fma2(e, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), w);
+          s0 = add2(s0, pair(e0, e1));
       }
     }
   }
@@ -352,12 +391,13 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 
 // The sums of `width` lanes (a power of two), on a common reference.  The factors are exact ones: the approximate 2^d is
 // 5e-8 low on average, and a row's sum passes here up to three times.
-__device__ __forceinline__ RowSum warp_merge(RowSum a, int width, Scale2 k) {
+template <typename D>
+__device__ __forceinline__ RowSum<D> warp_merge(RowSum<D> a, int width, Scale2 k) {
   float m = a.m;
   for (int off = width / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   if (a.m != m) {  // (no column anywhere: s is 0, or the NaN of a NaN column)
     const float d = rescale_exponent(a.m, m, k);
-    sum_rescale(a, m, d, (float)exp2((double)d));
+    sum_rescale(a, m, d, (D)exp2((double)d));
   }
   for (int off = width / 2; off > 0; off >>= 1) {
     a.s += __shfl_xor_sync(0xffffffffu, a.s, off);

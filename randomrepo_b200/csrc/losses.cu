@@ -85,7 +85,8 @@ struct RowGrad {
 };
 
 // log2 of a column's probability, in 64 bits.
-__device__ __forceinline__ double log2_prob(const LossArgs& A, const RowSum& r, float x) {
+template <typename D>
+__device__ __forceinline__ double log2_prob(const LossArgs& A, const RowSum<D>& r, float x) {
   const float c = center(r.m, A.ks);
   return (far_out(c) ? ((double)x - (double)r.m) * A.kd : (double)x * A.kd + (double)c) - log2_sum(r.s);
 }
@@ -102,8 +103,8 @@ struct PolicyRow {
   float l, h;
 };
 
-template <bool ENT>
-__device__ __forceinline__ RowGrad policy_tail(const LossArgs& A, RowSum r, const RowTerms& q, PolicyRow& v) {
+template <bool ENT, typename D>
+__device__ __forceinline__ RowGrad policy_tail(const LossArgs& A, const RowSum<D>& r, const RowTerms& q, PolicyRow& v) {
   const int64_t tok = q.tok;
   const bool known = tok >= 0 && tok < A.vocab;
   const double log2s = log2_sum(r.s);
@@ -119,7 +120,7 @@ __device__ __forceinline__ RowGrad policy_tail(const LossArgs& A, RowSum r, cons
   v.lp = lp, v.d = (double)q.ref - lp, v.h = 0.f;
   if (A.ref.p) g = fmaf(-A.kl_coef, expm1f((float)v.d), g);
   g *= w * A.inv_t;
-  const float inv_s = 1.f / r.s;
+  const float inv_s = 1.f / (float)r.s;
   RowGrad o{r.m, -g * inv_s, 0.f, g, known ? (int)tok : -1, false};
   if (ENT) {
     const double mean = (double)r.w / (double)r.s;
@@ -342,12 +343,12 @@ using ShortShape = Shape<128, 4, 5, 4>;
 constexpr int64_t kShortRow = 112 << 10;   // bytes
 constexpr int64_t kRowsInL2 = 72 << 20;    // bytes of rows in flight that come back from L2
 
-template <typename S, bool X>
+template <typename S, bool X, typename D>
 struct alignas(128) LossShared {
   uint64_t full[S::kSlots], empty[S::kSlots];
   uint64_t part_full[2], part_empty[2], grad_full[2], grad_empty[2], teacher_full[2], teacher_empty[2], peers[2];
   float4 peer[2][kMaxCluster];
-  RowSum part[2][32];
+  RowSum<D> part[2][32];
   RowGrad grad[2];
   float grad_wt[2];
   double sum[32];
@@ -355,6 +356,23 @@ struct alignas(128) LossShared {
   TeacherRow<X> teacher[2];
   int32_t ids[kIdTable];  // the ids of a list, by their hash
 };
+
+// Sums alone, which may be added up over a sequence (the preference loss), are exact; beside a gradient, where a CTA's
+// instructions are what bounds it, their error is below that of the float32 outputs.
+template <int PASS>
+using SumOf = std::conditional_t<PASS == kForward, double, float>;
+
+template <typename D>
+__device__ __forceinline__ float4 sum_bits(const RowSum<D>& a) {
+  if constexpr (sizeof(D) == 4) return make_float4(a.m, a.s, a.w, 0.f);
+  const double s = a.s;
+  return make_float4(a.m, __int_as_float(__double2loint(s)), a.w, __int_as_float(__double2hiint(s)));
+}
+template <typename D>
+__device__ __forceinline__ RowSum<D> sum_of_bits(float4 v) {
+  if constexpr (sizeof(D) == 4) return RowSum<D>{v.y, v.x, v.z};
+  return RowSum<D>{(D)__hiloint2double(__float_as_int(v.w), __float_as_int(v.y)), v.x, v.z};
+}
 
 // 16 bytes into the same shared-memory place of CTA `rank` of the cluster, counted on its barrier.
 __device__ __forceinline__ void send_peer(void* dst, uint64_t* bar, uint32_t rank, float4 v) {
@@ -585,23 +603,24 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
         if (A.ref.p) q.ref = A.ref.at(b, t);
       }
       wait_or_mark(&sh.part_full[par], phase, sh);
-      RowSum a = warp_merge(lane < S::kWarps ? sh.part[par][lane] : RowSum{-INFINITY, 0.f, 0.f}, 32, ks);
+      using D = SumOf<PASS>;
+      RowSum<D> a = warp_merge(lane < S::kWarps ? sh.part[par][lane] : RowSum<D>{0, -INFINITY, 0.f}, 32, ks);
       if (lane == 0) mbar_arrive(&sh.part_empty[par]);
       if (size > 1) {
         if (lane == 0 && !*(volatile int*)&sh.gave_up) {  // (a CTA that gave up leaves its peers to do so)
           mbar_arrive_expect_tx(&sh.peers[par], 16 * size);
           for (int c = 0; c < size; ++c)
-            send_peer(&sh.peer[par][rank], &sh.peers[par], c, make_float4(a.m, a.s, a.w, 0.f));
+            send_peer(&sh.peer[par][rank], &sh.peers[par], c, sum_bits(a));
         }
         __syncwarp();
         wait_or_mark<true>(&sh.peers[par], phase, sh);
         const float4 v = sh.peer[par][lane & (size - 1)];
-        a = warp_merge(RowSum{v.x, v.y, v.z}, size, ks);
+        a = warp_merge(sum_of_bits<D>(v), size, ks);
       }
       if (KIND == kPolicy) {
         o = policy_tail<ENT>(A, a, q, val);
       } else if (KIND == kPreference) {
-        o = RowGrad{a.m, -1.f / a.s, 0.f, 1.f, 0, false};
+        o = RowGrad{a.m, -1.f / (float)a.s, 0.f, 1.f, 0, false};
         if (write) A.row_val[row] = known ? log2_prob(A, a, q.x_tok) * kLn2d : (double)NAN;
       } else {
         wait_or_mark(&sh.teacher_full[par], phase, sh);
@@ -619,7 +638,7 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
         }
         const double l = none ? 0.0 : tt * tt * (te.qlogq - qp * kLn2d);
         wt = none ? 0.f : (float)(w * tt);
-        o = RowGrad{a.m, l == l ? wt * (float)te.q_sum / a.s : NAN, 0.f, 0.f, -1, none};
+        o = RowGrad{a.m, l == l ? wt * (float)te.q_sum / (float)a.s : NAN, 0.f, 0.f, -1, none};
         if (none) o.a = 0.f;  // (not 0 / s)
         if (write) {
           A.kl_out[row] = (float)l;
@@ -668,8 +687,9 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
   Ring<S::kSlots> r, zero;  // the next copy; the row's first chunk
   const bool whole = rows_whole<T, S>(A.vocab, size);
   const int end = PASS == kForward ? n_active : n;
+  using Sums = Fold<ENT, PASS == kForward>;
   // Chunk c of a row, at r, into its sums.
-  auto sum_chunk = [&](Fold<ENT>& fold, const RowPart<T, S::kChunk>& p, int c, bool done) {
+  auto sum_chunk = [&](Sums& fold, const RowPart<T, S::kChunk>& p, int c, bool done) {
     wait_or_mark(&sh.full[r.slot], r.phase, sh);
     const uint4* in = slots + r.slot * S::kChunk;
     const int nv = min(S::kChunk, p.nv - c * S::kChunk);
@@ -695,7 +715,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
     }
     r.next();
   };
-  Fold<ENT> fold;
+  Sums fold;
   int begun = 0;  // chunks of the row that are in its sums already (0 or 1)
   int row = row0;
   for (int i = first, it = 0; i < end; i += step) {
@@ -710,7 +730,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
     Ring<S::kSlots> at_zero = zero;
     if (PASS != kBackward && i < n_active) {
       if (!begun) {
-        fold = Fold<ENT>();
+        fold = Sums();
         at_zero = r;
       }
       for (int c = begun; c < p.chunks; ++c) sum_chunk(fold, p, c, PASS == kForward || c < again);
@@ -718,7 +738,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
         const float f[1] = {as_float(p.x[edge_col])};
         fold.template add<false>(f, f[0], ks);
       }
-      const RowSum a = warp_merge(fold.sum(), 32, ks);
+      const auto a = warp_merge(fold.sum(), 32, ks);
       if (it >= 2) wait_or_mark(&sh.part_empty[par], phase ^ 1, sh);
       if (lane == 0) {
         sh.part[par][warp] = a;
@@ -728,7 +748,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
       if (PASS == kFused && i + step < n_active) {
         const RowPart<T, S::kChunk> next(A, row, rank, size);
         if (next.chunks) {
-          fold = Fold<ENT>();
+          fold = Sums();
           zero = r;
           sum_chunk(fold, next, 0, chunks_again<PASS, S>(next.chunks, whole) > 0);
           begun = 1;
@@ -845,7 +865,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
 // columns, and the parts' sums cross by distributed shared memory.
 template <typename T, int KIND, bool ENT, int PASS, typename S>
 __global__ void __launch_bounds__(S::kThreads, S::kCtas) loss_rows_kernel(const LossArgs A) {
-  using Sh = LossShared<S, PASS == kFused>;
+  using Sh = LossShared<S, PASS == kFused, SumOf<PASS>>;
   extern __shared__ __align__(128) uint8_t dyn[];
   uint4* slots = reinterpret_cast<uint4*>(dyn);
   Sh& sh = *reinterpret_cast<Sh*>(dyn + S::kRingBytes);
@@ -1000,7 +1020,7 @@ Layout layout(int64_t batch, int64_t length) {
 
 template <typename T, int KIND, bool ENT, int PASS, typename S>
 int32_t launch_shape(const LossArgs& a, cudaStream_t st) {
-  constexpr int kBytes = S::kRingBytes + (int)sizeof(LossShared<S, PASS == kFused>);
+  constexpr int kBytes = S::kRingBytes + (int)sizeof(LossShared<S, PASS == kFused, SumOf<PASS>>);
   static_assert((kBytes + 1024) * S::kCtas <= 233472, "an SM's shared memory");
   int sms = 0;
   const int32_t e = sm_count(&sms);

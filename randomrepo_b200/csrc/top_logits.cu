@@ -69,7 +69,7 @@ struct alignas(128) TopShared {
   alignas(16) uint64_t keys[kTopCap];
   uint64_t best[PKV_MAX_TOP];                 // this CTA's list, largest first
   alignas(16) float tops[2][kTopGroups][kTopThreads];  // a group's largest value
-  RowSum sum[2][kTopWarps], all;
+  RowSum<float> sum[2][kTopWarps], all;
   uint16_t hits[kTopCap];                     // groups that reach the threshold
   float4 range[kPickWarps];
   uint32_t part[kPickWarps];
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
   __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int n = A.batch * A.length, first = blockIdx.x / size, step = gridDim.x / size;
-  auto write = [&](int row, const RowSum& a, uint64_t key, int at) {
+  auto write = [&](int row, const RowSum<float>& a, uint64_t key, int at) {
     const bool bad = *(volatile int*)&sh.gave_up;  // (a wait that ran out: no list)
     A.values[(int64_t)row * A.k + at] = bad ? NAN : unordered((uint32_t)(key >> 32));
     A.tokens[(int64_t)row * A.k + at] = bad ? -1 : (int64_t)(0xffffffffu - (uint32_t)key);
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
         const float f[1] = {as_float(p.x[tid < p.head ? tid : tid + p.nvec * VE])};
         fold.template add<false>(f, f[0], A.ks);
       }
-      const RowSum a = warp_merge(fold.sum(), 32, A.ks);
+      const RowSum<float> a = warp_merge(fold.sum(), 32, A.ks);
       if (lane == 0) sh.sum[par][warp] = a;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.row_full[par]);
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
       const TopPart<T> p(A, row, rank, size);
       const int edge = rank == 0 ? A.vocab - p.nvec * VE : 0, par = it & 1;
       wait_or_mark(&sh.row_full[par], (it >> 1) & 1, sh);
-      const RowSum all = warp_merge(lane < kTopWarps ? sh.sum[par][lane] : RowSum{-INFINITY, 0.f, 0.f}, 32, A.ks);
+      const RowSum<float> all = warp_merge(lane < kTopWarps ? sh.sum[par][lane] : RowSum<float>{0.f, -INFINITY, 0.f}, 32, A.ks);
       const int m = part_list<T>(p, edge, A.k, all.s == all.s, par, sh);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.row_empty[par]);
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kTopCta, TopShape::kCtas) top_logits_kernel(co
   if (rank == 0) {
     __shared__ int s_n[kMaxCluster];
     uint64_t* lists = reinterpret_cast<uint64_t*>(dyn);  // (the ring is done)
-    const RowSum all = warp_merge(lane < size ? cluster_peer(&sh, lane)->all : RowSum{-INFINITY, 0.f, 0.f}, 32, A.ks);
+    const RowSum<float> all = warp_merge(lane < size ? cluster_peer(&sh, lane)->all : RowSum<float>{0.f, -INFINITY, 0.f}, 32, A.ks);
     for (int q = 0; q < size; ++q) {
       const TopShared* peer = cluster_peer(&sh, q);
       if (tid == 0) s_n[q] = peer->best_n;
