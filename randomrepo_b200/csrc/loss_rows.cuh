@@ -54,6 +54,19 @@ __device__ __forceinline__ float ex2(float y) {
   return e;
 }
 
+// 2^d to a rounding: the series of e^(r ln 2) around the nearest integer, whose next term is 5e-9.
+__device__ __forceinline__ float pow2(float d) {
+  const float n = rintf(d), r = d - n;
+  float p = 1.52527338e-5f;
+  p = fmaf(p, r, 1.54035304e-4f);
+  p = fmaf(p, r, 1.33335581e-3f);
+  p = fmaf(p, r, 9.61812911e-3f);
+  p = fmaf(p, r, 5.55041087e-2f);
+  p = fmaf(p, r, 0.240226507f);
+  p = fmaf(p, r, 0.693147181f);
+  return d < -126.f ? 0.f : fmaf(p, r, 1.f) * __int_as_float(((int)n + 127) << 23);
+}
+
 // Columns x of a row are taken as y = x k + c, c = -(max x) hi rounded once:
 // one fused multiply-add a column, and what is made of y later starts from
 // the same c.  Its rounding and max x lo stay in every y, up to 2^-24 + 2^-23
@@ -206,14 +219,15 @@ __device__ __forceinline__ float top_of(const uint4 (&v)[N]) {
 // The lanes of a warp that add whole chunks share their m: their sums then merge without the approximate 2^d.
 //
 // EXACT: a column that is most of its row must not cost the small ones added after it their digits, nor be an approximate
-// 2^y itself (1.1e-7 of the row's sum, rms).  m gives way from 2^4 on, and the large columns among those that it is taken
-// from have a sum of their own in 64 bits.  (Others are not most of a row: m is the largest of a thousand columns.)
+// 2^y itself (1.1e-7 of the row's sum, rms).  m gives way from 2^4 on, and the sums of the columns that it is taken from
+// go to a 64-bit one at once.  (Others are not most of a row: m is the largest of a thousand columns.)
 template <bool ENT, bool EXACT = false>
 struct Fold {
+  static_assert(!(ENT && EXACT), "w is of 32 bits");
   using Sum = std::conditional_t<EXACT, double, float>;
   float m = -INFINITY, c = INFINITY;
   f32x2 s0 = 0ull, s1 = 0ull, w = 0ull;
-  double large = 0.0;
+  double kept = 0.0;
 
   __device__ __forceinline__ RowSum<float> lanes() const {
     const float2 t = unpair(add2(s0, s1)), u = unpair(w);
@@ -221,26 +235,28 @@ struct Fold {
   }
   __device__ __forceinline__ RowSum<Sum> sum() const {
     const RowSum<float> a = lanes();
-    if constexpr (EXACT) return RowSum<Sum>{(double)a.s + large, a.m, a.w};
+    if constexpr (EXACT) return RowSum<Sum>{(double)a.s + kept, a.m, a.w};
     return RowSum<Sum>{(Sum)a.s, a.m, a.w};
-  }
-  __device__ __forceinline__ void take_large(float& e) {
-    if (e > 0.5f) large += (double)e, e = 0.f;
   }
 
   // Add columns whose largest is `top`.  WHOLE: all lanes of the warp do.
   template <bool WHOLE, int N>
   __device__ __forceinline__ void add(const float (&x)[N], float top, Scale2 k) {
     const bool passed = !(fmaf(top, k.hi, c) <= (EXACT ? 4.f : 20.f));
-    if (WHOLE ? __any_sync(0xffffffffu, passed) : passed) {
+    const bool refers = WHOLE ? __any_sync(0xffffffffu, passed) : passed;
+    if (refers) {
       refer<WHOLE>(x, top, k);
       if (c == INFINITY) return;
-      if (EXACT) {
-        add_columns<true>(x, k);
-        return;
-      }
     }
-    add_columns<false>(x, k);
+    add_columns(x, k);
+    if (EXACT && refers) keep();
+  }
+
+  // Move the sums to the 64-bit one.
+  __device__ __forceinline__ void keep() {
+    const float2 a = unpair(add2(s0, s1));
+    kept += (double)a.x + (double)a.y;
+    s0 = s1 = 0ull;
   }
 
   // Take a reference of which `top` is within reach.  Far out, with the columns' sums.
@@ -258,10 +274,9 @@ struct Fold {
         if (x[i] != x[i]) a.s = NAN;
     } else {
       if (top > m) {
-        const float d = rescale_exponent(m, top, k), f = EXACT ? (float)exp2((double)d) : ex2(d);
-        if (EXACT && ENT) a.w = f > 0.f ? fmaf(d, (float)large, a.w) : 0.f;
+        const float d = rescale_exponent(m, top, k), f = EXACT ? pow2(d) : ex2(d);
         sum_rescale(a, top, d, f);
-        if (EXACT) large *= (double)f;
+        if (EXACT) kept *= (double)f;
       }
       m = a.m;
       const float at = center(m, k);
@@ -275,17 +290,17 @@ struct Fold {
         }
       }
     }
-    s0 = pair(a.s, 0.f), s1 = 0ull, w = pair(a.w, 0.f);
+    s0 = pair(EXACT ? 0.f : a.s, 0.f), s1 = 0ull, w = pair(a.w, 0.f);
+    if (EXACT && a.s != 0.f) kept += (double)a.s;
   }
 
-  template <bool LARGE, int N>
+  template <int N>
   __device__ __forceinline__ void add_columns(const float (&x)[N], Scale2 k) {
     if constexpr (N == 1) {
       const float y = fmaf(x[0], k.lo, fmaf(x[0], k.hi, c));
-      float e = ex2(y);
-      if (ENT) w = add2(w, pair(e * fmaxf(y, -1e30f), 0.f));
-      if (LARGE) take_large(e);
+      const float e = ex2(y);
       s0 = add2(s0, pair(e, 0.f));
+      if (ENT) w = add2(w, pair(e * fmaxf(y, -1e30f), 0.f));
     } else {
       static_assert(N % 4 == 0, "columns go in pairs, to two sums");
       const f32x2 cc = pair(c, c), hi = pair(k.hi, k.hi), lo = pair(k.lo, k.lo);
@@ -293,13 +308,12 @@ struct Fold {
       for (int i = 0; i < N; i += 2) {
         const f32x2 xx = pair(x[i], x[i + 1]);
         const float2 y = unpair(fma2(xx, lo, fma2(xx, hi, cc)));
-        float e0 = ex2(y.x), e1 = ex2(y.y);
-        if (ENT) w = fma2(pair(e0, e1), pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), w);
-        if (LARGE) take_large(e0), take_large(e1);
+        const f32x2 e = pair(ex2(y.x), ex2(y.y));
         if (i & 2)
-          s1 = add2(s1, pair(e0, e1));
+          s1 = add2(s1, e);
         else
-          s0 = add2(s0, pair(e0, e1));
+          s0 = add2(s0, e);
+        if (ENT) w = fma2(e, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), w);
       }
     }
   }

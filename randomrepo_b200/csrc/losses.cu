@@ -357,10 +357,12 @@ struct alignas(128) LossShared {
   int32_t ids[kIdTable];  // the ids of a list, by their hash
 };
 
-// Sums alone, which may be added up over a sequence (the preference loss), are exact; beside a gradient, where a CTA's
-// instructions are what bounds it, their error is below that of the float32 outputs.
-template <int PASS>
-using SumOf = std::conditional_t<PASS == kForward, double, float>;
+// The preference loss adds a row's log-probability up over its sequence: its sums are exact ones.  Others' errors (1e-7 at
+// the most, rms) are below the rounding of the float32 outputs that they end in.
+template <int KIND, int PASS>
+constexpr bool kExactSums = KIND == kPreference && PASS == kForward;
+template <int KIND, int PASS>
+using SumOf = std::conditional_t<kExactSums<KIND, PASS>, double, float>;
 
 template <typename D>
 __device__ __forceinline__ float4 sum_bits(const RowSum<D>& a) {
@@ -603,8 +605,10 @@ __device__ __forceinline__ void term_rows(const LossArgs& A, Sh& sh, int rank, i
         if (A.ref.p) q.ref = A.ref.at(b, t);
       }
       wait_or_mark(&sh.part_full[par], phase, sh);
-      using D = SumOf<PASS>;
-      RowSum<D> a = warp_merge(lane < S::kWarps ? sh.part[par][lane] : RowSum<D>{0, -INFINITY, 0.f}, 32, ks);
+      using D = SumOf<KIND, PASS>;
+      constexpr int kWide = S::kWarps > 16 ? 32 : S::kWarps > 4 ? 16 : 4;  // (as few rounds as there are sums)
+      const int part = lane & (kWide - 1);
+      RowSum<D> a = warp_merge(part < S::kWarps ? sh.part[par][part] : RowSum<D>{0, -INFINITY, 0.f}, kWide, ks);
       if (lane == 0) mbar_arrive(&sh.part_empty[par]);
       if (size > 1) {
         if (lane == 0 && !*(volatile int*)&sh.gave_up) {  // (a CTA that gave up leaves its peers to do so)
@@ -687,7 +691,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
   Ring<S::kSlots> r, zero;  // the next copy; the row's first chunk
   const bool whole = rows_whole<T, S>(A.vocab, size);
   const int end = PASS == kForward ? n_active : n;
-  using Sums = Fold<ENT, PASS == kForward>;
+  using Sums = Fold<ENT, kExactSums<KIND, PASS>>;
   // Chunk c of a row, at r, into its sums.
   auto sum_chunk = [&](Sums& fold, const RowPart<T, S::kChunk>& p, int c, bool done) {
     wait_or_mark(&sh.full[r.slot], r.phase, sh);
@@ -865,7 +869,7 @@ __device__ __forceinline__ void column_rows(const LossArgs& A, Sh& sh, const uin
 // columns, and the parts' sums cross by distributed shared memory.
 template <typename T, int KIND, bool ENT, int PASS, typename S>
 __global__ void __launch_bounds__(S::kThreads, S::kCtas) loss_rows_kernel(const LossArgs A) {
-  using Sh = LossShared<S, PASS == kFused, SumOf<PASS>>;
+  using Sh = LossShared<S, PASS == kFused, SumOf<KIND, PASS>>;
   extern __shared__ __align__(128) uint8_t dyn[];
   uint4* slots = reinterpret_cast<uint4*>(dyn);
   Sh& sh = *reinterpret_cast<Sh*>(dyn + S::kRingBytes);
@@ -1020,7 +1024,7 @@ Layout layout(int64_t batch, int64_t length) {
 
 template <typename T, int KIND, bool ENT, int PASS, typename S>
 int32_t launch_shape(const LossArgs& a, cudaStream_t st) {
-  constexpr int kBytes = S::kRingBytes + (int)sizeof(LossShared<S, PASS == kFused, SumOf<PASS>>);
+  constexpr int kBytes = S::kRingBytes + (int)sizeof(LossShared<S, PASS == kFused, SumOf<KIND, PASS>>);
   static_assert((kBytes + 1024) * S::kCtas <= 233472, "an SM's shared memory");
   int sms = 0;
   const int32_t e = sm_count(&sms);

@@ -573,27 +573,24 @@ def test_operators_hand_the_gradient_out(cuda_device):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_sums_of_rows_with_a_large_column(cuda_device, dtype):
-    """Sums that may be added up over a sequence: log-probabilities of tokens that are much of their row, read to 64 bits
-    through the KL estimate at d = 1e-3 (d is its root, and its error half of a float32's: 3e-11).
+    """Sums that are added up over a sequence: answers of one token that is much of its row.  A margin against the exact
+    sums as the reference is two rows' errors (the float32 reference is taken off in 64 bits, the margin is rounded to
+    2^-24 of itself).
 
     A column's exponent of 16 to 32 units is rounded twice, to 2^-20 at most: rms 5.4e-7 of its 2^y; a hundred columns
-    and more share what the token leaves of the row: 5.4e-8.  With a mean error of 2.6e-8: 6e-8.  A sum of the token's
+    and more share what the token leaves of the row: 5.4e-8.  A mean error of 2.6e-8: 6e-8 a row.  A sum of the token's
     2^y and the small ones beside it in 32 bits, or an approximate 2^y of the token, is off by 1e-7."""
     from randomrepo_b200 import losses
 
     n, v = 4096, 20011
     g = torch.Generator(device=cuda_device).manual_seed(3)
-    tokens = torch.randint(0, v, (1, n), generator=g, device=cuda_device)
-    x = 2 * torch.randn(1, n, v, generator=g, device=cuda_device)
-    x.scatter_add_(-1, tokens.unsqueeze(-1), 6 + 7 * torch.rand(1, n, 1, generator=g, device=cuda_device))
+    tokens = torch.randint(0, v, (n, 1), generator=g, device=cuda_device)
+    x = 2 * torch.randn(n, 1, v, generator=g, device=cuda_device)
+    x.scatter_add_(-1, tokens.unsqueeze(-1), 6 + 7 * torch.rand(n, 1, 1, generator=g, device=cuda_device))
     x = x.to(dtype)
-    exact = torch.cat([torch.log_softmax(c.double(), -1).gather(-1, t.unsqueeze(-1))
-                       for c, t in zip(x[0].split(512), tokens[0].split(512))]).view(1, n)
-    ref = (exact + 1e-3).float()
-    adv = torch.zeros(1, device=cuda_device)
-    kl = losses.policy_loss(x, tokens, adv, ref_logprobs=ref, kl_coef=1.0).kl.double()
-    d = (2 * kl).sqrt()
-    for _ in range(6):
-        d = d - (torch.expm1(d) - d - kl) / torch.expm1(d)
-    off = ref.double() - d - exact
-    assert off.pow(2).mean().sqrt() <= 6e-8 and off.mean().abs() <= 2.6e-8, (off.mean(), off.std())
+    exact = torch.cat([torch.log_softmax(c[:, 0].double(), -1).gather(-1, t) for c, t in zip(x.split(512), tokens.split(512))])
+    ref = exact[:, 0].float()
+    got = losses.preference_loss(x, tokens, None, ref, beta=1.0)
+    left = exact[:, 0] - ref.double()
+    off = got.margins.double() - (left[: n // 2] - left[n // 2:])
+    assert off.pow(2).mean().sqrt() <= 6e-8 * math.sqrt(2), off.std()
