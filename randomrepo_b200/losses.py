@@ -124,7 +124,7 @@ def _advantages(t: torch.Tensor, rows: torch.Size, dev: torch.device, what: str)
                                                                                 and t.shape[0] == rows[1]):
         if tuple(t.shape) not in ((rows[0],), (rows[0], 1)):
             raise ValueError(f"{what}: advantages must be [batch, length] or [batch], got {tuple(t.shape)}")
-        return t.to(torch.float32)
+        return t if t.dtype == torch.float32 else t.to(torch.float32)
     return _rows_like(t, rows, dev, torch.float32, what, "advantages")
 
 
@@ -156,14 +156,14 @@ def _grad_like(x: torch.Tensor) -> torch.Tensor:
     the logits' do, so that both move in 16-byte vectors: dense where such rows are, else with the logits' strides
     (rows that overlap or lie far apart: dense, wherever they start)."""
     b, n, v = x.shape
+    alike, at = x.is_contiguous(), x.data_ptr() % 16
+    if alike and at == 0:
+        return torch.empty(b, n, v, dtype=x.dtype, device=x.device)  # (faster than a tuple of sizes)
     size, numel = x.element_size(), x.numel()
-    at = x.data_ptr() % 16 // size
-    alike = x.is_contiguous()
+    at //= size
     if not alike:
         sb, sn = (x.stride(0) if b > 1 else 0), (x.stride(1) if n > 1 else 0)
         alike = v * size % 16 == 0 and sb * size % 16 == 0 and sn * size % 16 == 0
-    if numel == 0 or (alike and at == 0):
-        return torch.empty(b, n, v, dtype=x.dtype, device=x.device)  # (faster than a tuple of sizes)
     if alike:
         return torch.empty(numel + at, dtype=x.dtype, device=x.device)[at:].view(b, n, v)
     span = (n - 1) * sn + v
