@@ -54,9 +54,9 @@ __device__ __forceinline__ float ex2(float y) {
   return e;
 }
 
-// 2^d to a rounding: the series of e^(r ln 2) around the nearest integer, whose next term is 5e-9.
+// 2^d for d < 127, to 7e-8 of itself: the Taylor series of e^(r ln 2) around the nearest integer, whose next term is 5e-9.
 __device__ __forceinline__ float pow2(float d) {
-  const float n = rintf(d), r = d - n;
+  const float n = rintf(fmaxf(d, -126.f)), r = d - n;
   float p = 1.52527338e-5f;
   p = fmaf(p, r, 1.54035304e-4f);
   p = fmaf(p, r, 1.33335581e-3f);
